@@ -18,6 +18,7 @@
  *   - matrices are row-major; activations of the layer chain are
  *     [features x B] with the batch contiguous (include/sparse_onnx.hpp:148-154),
  *     4-D tensors are [C][H][W][B] (src/layers/conv_kernels.cpp:342-347).
+ *   - arrays are fp32 unless an operator takes an element type (SO_F32, SO_F16, SO_BF16).
  *   - all arithmetic is fp32; every output element is produced by the same
  *     rounding sequence as the reference (bias first, then one fused
  *     multiply-add per stored nonzero in ascending slot order), except so_matvec
@@ -344,6 +345,60 @@ so_status so_reverse_axes3(so_ctx *ctx, const float *dSrc, uint32_t d0, uint32_t
  * rows hold 4, 8 or a multiple of 16 entries (what the convolution kernels' batch tiles need). */
 so_status so_copy_rows(so_ctx *ctx, const float *dSrc, size_t src_stride, uint32_t rows, uint32_t cols,
                        float *dDst, size_t dst_stride, int zero_fill);
+
+/* ---- layer norm -------------------------------------------------------------
+ * No counterpart in the reference.  Activations are [F x B], batch contiguous, their rows x_stride (y_stride, ...)
+ * elements apart, of one of the element types below; parameters, statistics and their gradients are fp32, and so is
+ * all arithmetic: a result of 16 bits is rounded once. */
+enum { SO_F32 = 0, SO_F16 = 1, SO_BF16 = 2 };
+
+/* For every column b: mean_b = sum_f X / F, rstd_b = 1 / sqrt(sum_f (X - mean)^2 / F + eps),
+ * Y = (X - mean) * rstd * gamma_f + beta_f.  dGamma NULL: ones, dBeta NULL: zeros.  dMean, dRstd [B]: what
+ * so_layer_norm_grad takes, or NULL.  dY may be dX with the same stride; other overlaps are not allowed.  B may be 0, F may not.  A column
+ * with an infinity or NaN gives NaN throughout, the others are not touched by it. */
+so_status so_layer_norm(so_ctx *ctx, int type, uint32_t F, uint32_t B, const void *dX, size_t x_stride,
+                        const float *dGamma, const float *dBeta, float eps, void *dY, size_t y_stride,
+                        float *dMean, float *dRstd);
+/* Its gradient: with g = dY * gamma and h = (X - mean) * rstd, dX = rstd * (g - sum_f g / F - h * sum_f (g h) / F),
+ * dgamma_f = sum_b dY h, dbeta_f = sum_b dY, written, not added to.  Any of the three may be NULL.  dDx may be dX or dDy
+ * with the same stride.  With B = 0 dgamma and dbeta are zeros.  Sums are taken in the same order on every call. */
+so_status so_layer_norm_grad(so_ctx *ctx, int type, uint32_t F, uint32_t B, const void *dX, size_t x_stride,
+                             const void *dDy, size_t dy_stride, const float *dGamma, const float *dMean,
+                             const float *dRstd, void *dDx, size_t dx_stride, float *dDgamma, float *dDbeta);
+/* Grows the context's workspace to what both need for F x B: before recording them into a graph, as so_matmul_reserve. */
+so_status so_layer_norm_reserve(so_ctx *ctx, int type, uint32_t F, uint32_t B);
+
+/* ---- microscaled 4-bit floating point -------------------------------------------
+ * No counterpart in the reference.  A matrix in 4.25 bits per entry: blocks of 32 entries along a row (the last one
+ * filled up with zeros), each entry one of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} as a code 0..7, 8 more for minus, times the
+ * block's scale 2^(s - 127), s a byte.  Codes are row-major, 16 bytes a block, the even entry of two in a byte's low half
+ * (16-byte aligned); scales row-major, a byte a block.  s = 255 stands for a block that is not a number.
+ *
+ * Quantisation: s = max(e, 2) - 2 with e the biased fp32 exponent of the block's largest magnitude, entries divided by
+ * the scale and rounded to the nearest value, ties to the even code, beyond 6 to 6.  A block with an infinity or a NaN
+ * gets s = 255 and codes 0. */
+so_status so_mxfp4_quantize(so_ctx *ctx, int type, const void *dX, size_t x_stride, uint32_t rows, uint32_t cols,
+                            uint8_t *dCodes, uint8_t *dScales);
+/* The values that codes and scales stand for, rounded to `type` (bf16 holds them exactly, fp16 not beyond its range). */
+so_status so_mxfp4_dequantize(so_ctx *ctx, const uint8_t *dCodes, const uint8_t *dScales, uint32_t rows, uint32_t cols,
+                              int type, void *dY, size_t y_stride);
+
+/* A matrix W [m x n] for products, laid out for the matrix cores from row-major codes and scales in device memory, which
+ * are free for reuse once the stream has passed the call.  Takes 17 bytes for 32 entries, n rounded up to 256. */
+typedef struct so_mxfp4 so_mxfp4;
+so_status so_mxfp4_create(so_ctx *ctx, const uint8_t *dCodes, const uint8_t *dScales, uint32_t m, uint32_t n, so_mxfp4 **out);
+so_status so_mxfp4_free(so_ctx *ctx, so_mxfp4 *W);
+so_status so_mxfp4_dims(const so_mxfp4 *W, uint32_t *m, uint32_t *n);
+/* Y [m x C] = act(W Q(X) + bias): so_matmul with both operands in 4 bits.  X [n x C] and Y are of `type`, rows x_stride
+ * and y_stride elements apart; Q quantises X as above in blocks of 32 of its rows, within the call.  Products and the sums of a
+ * block are exact, blocks are added in fp32, in the same order on every call; Y is rounded once.  dBias [m] may be NULL.
+ * A block of X that is not a number makes its column of Y NaN, one of W its row. */
+so_status so_mxfp4_matmul(so_ctx *ctx, const so_mxfp4 *W, int type, const void *dX, size_t x_stride, uint32_t C,
+                          const float *dBias, void *dY, size_t y_stride, int act);
+/* Grows the context's workspace to what C columns need: before recording a product into a graph, as so_matmul_reserve. */
+so_status so_mxfp4_matmul_reserve(so_ctx *ctx, const so_mxfp4 *W, uint32_t C);
+/* y [m] = W x + bias with x in fp32 as it is: the form for a single token, bound by the 4.25 bits per entry of W. */
+so_status so_mxfp4_matvec(so_ctx *ctx, const so_mxfp4 *W, const float *dx, const float *dBias, float *dy);
 
 /* ---- launch graphs -------------------------------------------------------
  * Record every launch made on the context between begin and end into one

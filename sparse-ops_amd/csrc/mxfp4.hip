@@ -1,0 +1,249 @@
+// Microscaled 4-bit floating point (csrc/mxfp4.h): quantisation and its way back on caller-owned arrays, the weights' handle, and the quantisation of a product's activations.
+#include "lane_moves.h"
+#include "mxfp4.h"
+
+#include <new>
+#include <type_traits>
+
+namespace {
+
+constexpr int kBlock = 256;
+
+// Row-major to codes and scales.  A lane takes 16 bytes of a row, a block is 8 lanes of fp32 or 4 of a 16-bit type; a block that the row ends in is filled with zeros.
+template <class T>
+__global__ __launch_bounds__(kBlock)
+void mx_quantize_kernel(const T *__restrict__ X, size_t ldx, uint32_t cols, uint32_t groups, uint64_t total, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales)
+{
+    constexpr int V = so_elements<T>::V, L = 32 / V;
+    for (uint64_t u = (uint64_t)blockIdx.x * kBlock + threadIdx.x; u < total; u += (uint64_t)gridDim.x * kBlock) {
+        const uint64_t row = u / groups;
+        const uint32_t g = (uint32_t)(u - row * groups), c = g * V;
+        typename so_elements<T>::plain x = {};
+        if (c < cols) x = so_group_load(X + row * ldx + c, cols - c);
+        float f[V];
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            f[e] = (float)x[e];
+            top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+        }
+        top = so_lanes::reduce<L>(top, so_lanes::Max());          // groups and total are multiples of L: all lanes of a block are here
+        const uint32_t s = so_mx_scale(top);
+        const float scale = so_mx_power(s);
+        if constexpr (V == 4) {
+            const float v[8] = {f[0], f[1], f[2], f[3], 0.0f, 0.0f, 0.0f, 0.0f};
+            reinterpret_cast<uint16_t *>(codes)[u] = s == 255u ? 0 : (uint16_t)so_mx_codes(v, scale);
+        } else {
+            reinterpret_cast<uint32_t *>(codes)[u] = s == 255u ? 0 : so_mx_codes(f, scale);
+        }
+        if (u % L == 0) scales[u / L] = (uint8_t)s;
+    }
+}
+
+// And back.
+template <class T>
+__global__ __launch_bounds__(kBlock)
+void mx_dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, uint32_t cols, uint32_t groups, uint64_t total, T *__restrict__ Y, size_t ldy)
+{
+    constexpr int V = so_elements<T>::V, L = 32 / V;
+    for (uint64_t u = (uint64_t)blockIdx.x * kBlock + threadIdx.x; u < total; u += (uint64_t)gridDim.x * kBlock) {
+        const uint64_t row = u / groups;
+        const uint32_t g = (uint32_t)(u - row * groups), c = g * V;
+        const uint32_t s = scales[u / L];
+        const uint32_t w = V == 4 ? reinterpret_cast<const uint16_t *>(codes)[u] : reinterpret_cast<const uint32_t *>(codes)[u];
+        const float scale = so_mx_power(s);
+        float f[V];
+        const auto pair = [&](auto byte) {
+            constexpr int I = decltype(byte)::value;
+            const auto p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, I);
+            f[2 * I] = s == 255u ? __builtin_nanf("") : p[0];
+            f[2 * I + 1] = s == 255u ? __builtin_nanf("") : p[1];
+        };
+        pair(std::integral_constant<int, 0>());
+        pair(std::integral_constant<int, 1>());
+        if constexpr (V == 8) {
+            pair(std::integral_constant<int, 2>());
+            pair(std::integral_constant<int, 3>());
+        }
+        if (c < cols) so_group_store(Y + row * ldy + c, cols - c, f);
+    }
+}
+
+// Row-major codes and scales into tiles; a thread takes a block of a row, and for every eighth a word of scales.
+__global__ __launch_bounds__(kBlock)
+void mx_tile_kernel(const so_u32x4 *__restrict__ src, const uint8_t *__restrict__ src_scales, uint32_t m, uint32_t real, uint32_t blocks, uint64_t total, so_u32x4 *__restrict__ codes,
+                    uint32_t *__restrict__ scales)
+{
+    const uint64_t u = (uint64_t)blockIdx.x * kBlock + threadIdx.x;            // [tile][block][row]
+    if (u >= total) return;
+    const uint32_t r = (uint32_t)(u % kMxTile);
+    const uint64_t tb = u / kMxTile, tile = tb / blocks;
+    const uint32_t b = (uint32_t)(tb - tile * blocks);
+    const uint64_t row = tile * kMxTile + r;
+    const bool in = row < m && b < real;
+    so_u32x4 v = {0u, 0u, 0u, 0u};
+    if (in) v = src[row * real + b];
+    codes[u] = v;
+    if (b % kMxUnit >= 2) return;                                              // blocks 0 and 1 of a unit: the words of lanes r and 32 + r
+    uint32_t w = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) w |= (uint32_t)(row < m && b + 2 * j < real ? src_scales[row * real + b + 2 * j] : kMxZero) << (8 * j);
+    scales[(tile * (blocks / kMxUnit) + b / kMxUnit) * 64 + b % kMxUnit * 32 + r] = w;
+}
+
+// X [n x C] into tiles of columns: a thread takes one column and four blocks of a unit, all even or all odd ones, whose scales share a word.
+template <class T>
+__global__ __launch_bounds__(kBlock)
+void mx_columns_kernel(const T *__restrict__ X, size_t ldx, uint32_t n, uint32_t C, uint32_t blocks, uint64_t total, so_u32x4 *__restrict__ codes, uint32_t *__restrict__ scales)
+{
+    const uint64_t u = (uint64_t)blockIdx.x * kBlock + threadIdx.x;            // [unit][odd][column]
+    if (u >= total) return;
+    const uint64_t q = u / C;
+    const uint32_t c = (uint32_t)(u - q * C), odd = (uint32_t)(q & 1), unit = (uint32_t)(q >> 1);
+    const uint64_t tile = c / kMxTile;
+    const uint32_t r = c % kMxTile;
+    uint32_t word = 0;
+    for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t b = unit * kMxUnit + 2 * j + odd;
+        const uint64_t k0 = (uint64_t)b * 32;
+        so_u32x4 v = {0u, 0u, 0u, 0u};
+        uint32_t s = kMxZero;
+        if (k0 < n) {
+            const T *p = X + k0 * ldx + c;
+            float f[32];
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                f[i] = k0 + i < n ? (float)p[(size_t)i * ldx] : 0.0f;
+                top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+            }
+            s = so_mx_scale(top);
+            if (s != 255u) {
+                const float scale = so_mx_power(s);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const float e[8] = {f[8 * g], f[8 * g + 1], f[8 * g + 2], f[8 * g + 3], f[8 * g + 4], f[8 * g + 5], f[8 * g + 6], f[8 * g + 7]};
+                    v[g] = so_mx_codes(e, scale);
+                }
+            }
+        }
+        codes[(tile * blocks + b) * kMxTile + r] = v;
+        word |= s << (8 * j);
+    }
+    scales[(tile * (blocks / kMxUnit) + unit) * 64 + odd * 32 + r] = word;
+}
+
+// Rows that lie without a gap and end with a block are one long row.
+struct Flat { uint64_t groups, total; };
+template <class T>
+Flat flat(uint32_t rows, uint32_t cols)
+{
+    const uint64_t groups = (uint64_t)so_ceil_div(cols, 32) * (32 / so_elements<T>::V);
+    return {groups, groups * rows};
+}
+
+uint32_t grid_of(uint64_t total) { return (uint32_t)std::min<uint64_t>((total + kBlock - 1) / kBlock, 1u << 20); }
+
+} // namespace
+
+extern "C" so_status so_mxfp4_quantize(so_ctx *ctx, int type, const void *dX, size_t x_stride, uint32_t rows, uint32_t cols, uint8_t *dCodes, uint8_t *dScales)
+{
+    SO_REQUIRE(ctx != nullptr, "so_mxfp4_quantize: ctx is null");
+    SO_REQUIRE(type >= SO_F32 && type <= SO_BF16, "so_mxfp4_quantize: unknown element type %d", type);
+    if (rows == 0 || cols == 0) return SO_OK;
+    SO_REQUIRE(dX && dCodes && dScales, "so_mxfp4_quantize: null array");
+    SO_REQUIRE(x_stride >= cols, "so_mxfp4_quantize: a stride is shorter than a row");
+    SO_REQUIRE(((uintptr_t)dCodes & 15) == 0, "so_mxfp4_quantize: codes are not 16-byte aligned");
+    SO_REQUIRE(cols <= 0xffffffe0u, "so_mxfp4_quantize: too many columns");
+    const so_on_device on(ctx->device);
+    SO_HIP(on.status);
+    so_for_type(type, [&](auto t) {
+        using T = decltype(t);
+        const Flat f = flat<T>(rows, cols);
+        mx_quantize_kernel<T><<<grid_of(f.total), kBlock, 0, ctx->stream>>>((const T *)dX, x_stride, cols, (uint32_t)f.groups, f.total, dCodes, dScales);
+    });
+    SO_LAUNCH_CHECK();
+    return SO_OK;
+}
+
+extern "C" so_status so_mxfp4_dequantize(so_ctx *ctx, const uint8_t *dCodes, const uint8_t *dScales, uint32_t rows, uint32_t cols, int type, void *dY, size_t y_stride)
+{
+    SO_REQUIRE(ctx != nullptr, "so_mxfp4_dequantize: ctx is null");
+    SO_REQUIRE(type >= SO_F32 && type <= SO_BF16, "so_mxfp4_dequantize: unknown element type %d", type);
+    if (rows == 0 || cols == 0) return SO_OK;
+    SO_REQUIRE(dY && dCodes && dScales, "so_mxfp4_dequantize: null array");
+    SO_REQUIRE(y_stride >= cols, "so_mxfp4_dequantize: a stride is shorter than a row");
+    SO_REQUIRE(((uintptr_t)dCodes & 15) == 0, "so_mxfp4_dequantize: codes are not 16-byte aligned");
+    SO_REQUIRE(cols <= 0xffffffe0u, "so_mxfp4_dequantize: too many columns");
+    const so_on_device on(ctx->device);
+    SO_HIP(on.status);
+    so_for_type(type, [&](auto t) {
+        using T = decltype(t);
+        const Flat f = flat<T>(rows, cols);
+        mx_dequantize_kernel<T><<<grid_of(f.total), kBlock, 0, ctx->stream>>>(dCodes, dScales, cols, (uint32_t)f.groups, f.total, (T *)dY, y_stride);
+    });
+    SO_LAUNCH_CHECK();
+    return SO_OK;
+}
+
+extern "C" so_status so_mxfp4_create(so_ctx *ctx, const uint8_t *dCodes, const uint8_t *dScales, uint32_t m, uint32_t n, so_mxfp4 **out)
+{
+    SO_REQUIRE(ctx != nullptr, "so_mxfp4_create: ctx is null");
+    SO_REQUIRE(out != nullptr, "so_mxfp4_create: out is null");
+    *out = nullptr;
+    SO_REQUIRE(m > 0 && n > 0, "so_mxfp4_create: an empty matrix");
+    SO_REQUIRE(dCodes && dScales, "so_mxfp4_create: null array");
+    SO_REQUIRE(((uintptr_t)dCodes & 15) == 0, "so_mxfp4_create: codes are not 16-byte aligned");
+    SO_REQUIRE(n <= 0xffffff00u && m <= 0xffffffe0u, "so_mxfp4_create: %u x %u is too large", m, n);
+    SO_REQUIRE(!ctx->capturing, "so_mxfp4_create: not allowed while a graph is being recorded");
+    const so_on_device on(ctx->device);
+    SO_HIP(on.status);
+    std::unique_ptr<so_mxfp4> W(new (std::nothrow) so_mxfp4());
+    if (!W) { so_set_error("host allocation failed"); return SO_ERR_OOM; }
+    W->m = m;
+    W->n = n;
+    W->blocks = so_mx_blocks(n);
+    W->tiles = so_ceil_div(m, kMxTile);
+    const uint64_t total = (uint64_t)W->tiles * W->blocks * kMxTile;                 // threads, and 16 bytes of codes each
+    SO_REQUIRE(total / kBlock < (1ull << 31), "so_mxfp4_create: %u x %u is too large for one launch", m, n);
+    SO_HIP(hipMalloc(&W->d_blob, total * 17));
+    W->d_codes = (so_u32x4 *)W->d_blob;
+    W->d_scales = (uint32_t *)(W->d_codes + total);
+    mx_tile_kernel<<<so_ceil_div(total, kBlock), kBlock, 0, ctx->stream>>>((const so_u32x4 *)dCodes, dScales, m, so_ceil_div(n, 32), W->blocks, total, W->d_codes, W->d_scales);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) {
+        (void)hipFree(W->d_blob);
+        so_set_error("kernel launch failed: %s (so_mxfp4_create)", hipGetErrorString(e));
+        return SO_ERR_HIP;
+    }
+    *out = W.release();
+    return SO_OK;
+}
+
+extern "C" so_status so_mxfp4_free(so_ctx *ctx, so_mxfp4 *W)
+{
+    if (!W) return SO_OK;
+    if (ctx && ctx->stream) (void)hipStreamSynchronize(ctx->stream);
+    (void)hipFree(W->d_blob);
+    delete W;
+    return SO_OK;
+}
+
+extern "C" so_status so_mxfp4_dims(const so_mxfp4 *W, uint32_t *m, uint32_t *n)
+{
+    SO_REQUIRE(W != nullptr, "so_mxfp4_dims: handle is null");
+    if (m) *m = W->m;
+    if (n) *n = W->n;
+    return SO_OK;
+}
+
+so_status so_mx_quantize_columns(so_ctx *ctx, int type, const void *dX, size_t x_stride, uint32_t n, uint32_t C, so_u32x4 *codes, uint32_t *scales)
+{
+    const uint32_t blocks = so_mx_blocks(n);
+    const uint64_t total = (uint64_t)(blocks / kMxUnit) * 2 * C;
+    so_for_type(type, [&](auto t) {
+        using T = decltype(t);
+        mx_columns_kernel<T><<<so_ceil_div(total, kBlock), kBlock, 0, ctx->stream>>>((const T *)dX, x_stride, n, C, blocks, total, codes, scales);
+    });
+    SO_LAUNCH_CHECK();
+    return SO_OK;
+}

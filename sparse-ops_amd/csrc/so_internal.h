@@ -201,6 +201,21 @@ struct so_graph {
 
 void so_set_error(const char *fmt, ...);
 
+// A context's device as the current one for as long as this lives; the caller's comes back with its end.
+struct so_on_device {
+    int before = -1;
+    hipError_t status = hipSuccess;
+    explicit so_on_device(int device)
+    {
+        status = hipGetDevice(&before);
+        if (status == hipSuccess && before != device) status = hipSetDevice(device);
+        else before = -1;
+    }
+    so_on_device(const so_on_device &) = delete;
+    so_on_device &operator=(const so_on_device &) = delete;
+    ~so_on_device() { if (before >= 0) (void)hipSetDevice(before); }
+};
+
 // csrc/matmul_tiled.hip: launches the LDS-staged kernel on E's TILED copy (the caller has checked that it applies).
 so_status so_matmul_tiled_launch(so_ctx *ctx, const so_ellpack *E, const float *dX, uint32_t C,
                                  const float *dBias, float *dY, int act);

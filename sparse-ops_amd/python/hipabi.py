@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(os.path.dirname(_HERE), "libsparseops_hip.so")
 
 SO_OK, SO_ERR_NO_DEVICE, SO_ERR_INVALID, SO_ERR_OOM, SO_ERR_HIP, SO_ERR_BOUNDS = range(6)
 ACT = {"none": 0, "relu": 1, "sigmoid": 2, "tanh": 3}
+TYPE = {"f32": 0, "f16": 1, "bf16": 2}
 LAYOUT_ROW, LAYOUT_SLOT, LAYOUT_BINS, LAYOUT_TILED, LAYOUT_RBM, LAYOUT_IDX16 = 1, 2, 4, 8, 16, 32
 
 # Every symbol include/sparseops_hip.h declares.
@@ -22,7 +23,9 @@ SYMBOLS = (
     "so_stage_in so_stage_out so_stage_in_transposed so_stage_out_transposed so_d2d so_fill_zero so_sync so_timer_begin so_timer_end so_ellpack_upload so_ellpack_free "
     "so_ellpack_dims so_ellpack_download so_ellpack_decode so_ellpack_encode so_ellpack_encode_noalloc so_matmul so_matmul_reserve so_last_kernel so_matvec so_matvec_to_host so_conv_plan_create so_conv_plan_free so_conv_plan_window so_conv_plan_tune so_conv2d_add so_conv2d_pair "
     "so_conv2d so_maxpool so_gap so_add so_act so_transpose so_reverse_axes3 so_copy_rows so_graph_begin so_graph_end "
-    "so_graph_launch so_graph_free so_rbm_upload so_rbm_free so_rbm_dims so_conv_plan_set_rbm so_conv_plan_rbm_info").split()
+    "so_graph_launch so_graph_free so_rbm_upload so_rbm_free so_rbm_dims so_conv_plan_set_rbm so_conv_plan_rbm_info "
+    "so_layer_norm so_layer_norm_grad so_layer_norm_reserve so_mxfp4_quantize so_mxfp4_dequantize so_mxfp4_create so_mxfp4_free so_mxfp4_dims so_mxfp4_matmul "
+    "so_mxfp4_matmul_reserve so_mxfp4_matvec").split()
 
 _vp = ct.c_void_p
 _u32 = ct.c_uint32
@@ -112,6 +115,17 @@ def load_library(path=None):
                         ct.POINTER(ct.c_uint64), ct.POINTER(ct.c_uint64)],
         "so_conv_plan_set_rbm": [_vp, _vp, _vp],
         "so_conv_plan_rbm_info": [_vp, ct.POINTER(ct.c_uint64)],
+        "so_layer_norm": [_vp, ct.c_int, _u32, _u32, _vp, ct.c_size_t, _vp, _vp, ct.c_float, _vp, ct.c_size_t, _vp, _vp],
+        "so_layer_norm_grad": [_vp, ct.c_int, _u32, _u32, _vp, ct.c_size_t, _vp, ct.c_size_t, _vp, _vp, _vp, _vp, ct.c_size_t, _vp, _vp],
+        "so_layer_norm_reserve": [_vp, ct.c_int, _u32, _u32],
+        "so_mxfp4_quantize": [_vp, ct.c_int, _vp, ct.c_size_t, _u32, _u32, _vp, _vp],
+        "so_mxfp4_dequantize": [_vp, _vp, _vp, _u32, _u32, ct.c_int, _vp, ct.c_size_t],
+        "so_mxfp4_create": [_vp, _vp, _vp, _u32, _u32, ct.POINTER(_vp)],
+        "so_mxfp4_free": [_vp, _vp],
+        "so_mxfp4_dims": [_vp, ct.POINTER(_u32), ct.POINTER(_u32)],
+        "so_mxfp4_matmul": [_vp, _vp, ct.c_int, _vp, ct.c_size_t, _u32, _vp, _vp, ct.c_size_t, ct.c_int],
+        "so_mxfp4_matmul_reserve": [_vp, _vp, _u32],
+        "so_mxfp4_matvec": [_vp, _vp, _vp, _vp, _vp],
     }
     for name, argtypes in sig.items():
         fn = getattr(lib, name)
@@ -193,6 +207,22 @@ class DeviceEllpack:
         if self.h:
             self.ctx.lib.so_ellpack_free(self.ctx.h, self.h)
             self.h = None
+
+
+class DeviceMxfp4:
+    """A matrix in microscaled 4-bit floating point, laid out for products (so_mxfp4)."""
+
+    def __init__(self, ctx, handle, m, n):
+        self.ctx, self.h, self.m, self.n = ctx, handle, m, n
+
+    def free(self):
+        if self.h:
+            self.ctx.lib.so_mxfp4_free(self.ctx.h, self.h)
+            self.h = None
+
+
+def _at(array):
+    return None if array is None else array.ptr
 
 
 class Context:
@@ -301,6 +331,42 @@ class Context:
 
     def matvec(self, E, dx, dBias, dy, layout=0):
         self._ck(self.lib.so_matvec(self.h, E.h, dx.ptr, dBias.ptr if dBias else None, dy.ptr, layout))
+
+    # Activations of the next calls are [features, batch] of `type` ("f32", "f16", "bf16"), their rows `*_stride` elements apart (None: no gap).
+
+    def layer_norm(self, dX, F, B, dGamma, dBeta, eps, dY, dMean=None, dRstd=None, type="f32", x_stride=None, y_stride=None):
+        self._ck(self.lib.so_layer_norm(self.h, TYPE[type], F, B, _at(dX), B if x_stride is None else x_stride, _at(dGamma), _at(dBeta), eps,
+                                        _at(dY), B if y_stride is None else y_stride, _at(dMean), _at(dRstd)))
+
+    def layer_norm_grad(self, dX, dDy, F, B, dGamma, dMean, dRstd, dDx, dDgamma, dDbeta, type="f32", x_stride=None, dy_stride=None, dx_stride=None):
+        self._ck(self.lib.so_layer_norm_grad(self.h, TYPE[type], F, B, _at(dX), B if x_stride is None else x_stride, _at(dDy), B if dy_stride is None else dy_stride,
+                                             _at(dGamma), _at(dMean), _at(dRstd), _at(dDx), B if dx_stride is None else dx_stride, _at(dDgamma), _at(dDbeta)))
+
+    def layer_norm_reserve(self, F, B, type="f32"):
+        self._ck(self.lib.so_layer_norm_reserve(self.h, TYPE[type], F, B))
+
+    def mxfp4_quantize(self, dX, rows, cols, dCodes, dScales, type="f32", x_stride=None):
+        """Row-major (rows, cols) to codes (rows, ceil(cols / 32), 16) and scales (rows, ceil(cols / 32)), bytes."""
+        self._ck(self.lib.so_mxfp4_quantize(self.h, TYPE[type], _at(dX), cols if x_stride is None else x_stride, rows, cols, _at(dCodes), _at(dScales)))
+
+    def mxfp4_dequantize(self, dCodes, dScales, rows, cols, dY, type="f32", y_stride=None):
+        self._ck(self.lib.so_mxfp4_dequantize(self.h, _at(dCodes), _at(dScales), rows, cols, TYPE[type], _at(dY), cols if y_stride is None else y_stride))
+
+    def mxfp4(self, dCodes, dScales, m, n):
+        """The matrix laid out for products -> DeviceMxfp4."""
+        h = _vp()
+        self._ck(self.lib.so_mxfp4_create(self.h, _at(dCodes), _at(dScales), m, n, ct.byref(h)))
+        return DeviceMxfp4(self, h.value, m, n)
+
+    def mxfp4_matmul(self, W, dX, C, dBias, dY, act="none", type="f32", x_stride=None, y_stride=None):
+        self._ck(self.lib.so_mxfp4_matmul(self.h, W.h, TYPE[type], _at(dX), C if x_stride is None else x_stride, C, _at(dBias), _at(dY),
+                                          C if y_stride is None else y_stride, ACT[act]))
+
+    def mxfp4_matmul_reserve(self, W, C):
+        self._ck(self.lib.so_mxfp4_matmul_reserve(self.h, W.h, C))
+
+    def mxfp4_matvec(self, W, dx, dBias, dy):
+        self._ck(self.lib.so_mxfp4_matvec(self.h, W.h, _at(dx), _at(dBias), _at(dy)))
 
     def conv_plan(self, E, geom):
         h = _vp()
