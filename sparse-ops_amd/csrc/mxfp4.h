@@ -2,8 +2,9 @@
 // block's scale 2^(s - 127) in a byte s (255: not a number).
 //
 // Outside, row-major: 16 bytes of codes a block, the even entry of two in the low half of a byte; scales beside.
-// Inside, as the scaled matrix instruction (32 x 32 x 64) takes an operand, lane l holding row l % 32 and block l / 32 of two: tiles of 32 rows, in a tile block by block
-// 32 rows x 16 bytes; the scales of 8 blocks as one word a lane, byte j of lane l for block 2 j + l / 32.  Blocks are padded to a multiple of 8 with zeros.
+// Inside, as the scaled matrix instruction (16 x 16 x 128) takes an operand, lane l holding row l % 16 and block l / 16 of four: tiles of 32 rows, in a tile unit by unit of 8
+// blocks, of a unit four operands of 64 lanes x 16 bytes: the first four blocks of rows 0..15, of rows 16..31, the last four of both.  A unit's scales are one word a lane, a byte
+// for each operand: lane l, byte 2 * (row / 16) + (block / 4) for row % 16 = l % 16, block % 4 = l / 16.  Blocks are padded to whole units with zeros.
 #pragma once
 #include "elements.h"
 #include "so_internal.h"
@@ -19,9 +20,19 @@ struct so_mxfp4 {
     uint32_t blocks = 0;                // of a row as stored, a multiple of kMxUnit
     uint32_t tiles = 0;
     void *d_blob = nullptr;             // one allocation for the two
-    so_u32x4 *d_codes = nullptr;        // [tiles][blocks][32]
-    uint32_t *d_scales = nullptr;       // [tiles][blocks / 8][64]
+    so_u32x4 *d_codes = nullptr;        // [tiles][units][4][64]
+    uint32_t *d_scales = nullptr;       // [tiles][units][64]
 };
+
+// Where the codes (by 16 bytes) and the scale (by bytes) of block b of a row lie.
+__host__ __device__ inline uint64_t so_mx_code_at(uint64_t row, uint32_t b, uint32_t units)
+{
+    return ((row / kMxTile * units + b / kMxUnit) * 4u + b % kMxUnit / 4u * 2u + row % kMxTile / 16u) * 64u + b % 4u * 16u + row % 16u;
+}
+__host__ __device__ inline uint64_t so_mx_scale_at(uint64_t row, uint32_t b, uint32_t units)
+{
+    return ((row / kMxTile * units + b / kMxUnit) * 64u + b % 4u * 16u + row % 16u) * 4u + row % kMxTile / 16u * 2u + b % kMxUnit / 4u;
+}
 
 static inline uint32_t so_mx_blocks(uint32_t n) { return so_ceil_div(n, 32 * kMxUnit) * kMxUnit; }
 

@@ -69,68 +69,93 @@ void mx_dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__re
     }
 }
 
-// Row-major codes and scales into tiles; a thread takes a block of a row, and for every eighth a word of scales.
+// Row-major codes and scales into tiles; a thread takes 16 bytes of the result.
 __global__ __launch_bounds__(kBlock)
-void mx_tile_kernel(const so_u32x4 *__restrict__ src, const uint8_t *__restrict__ src_scales, uint32_t m, uint32_t real, uint32_t blocks, uint64_t total, so_u32x4 *__restrict__ codes,
-                    uint32_t *__restrict__ scales)
+void mx_tile_kernel(const so_u32x4 *__restrict__ src, const uint8_t *__restrict__ src_scales, uint32_t m, uint32_t real, uint32_t units, uint64_t total, so_u32x4 *__restrict__ codes,
+                    uint8_t *__restrict__ scales)
 {
-    const uint64_t u = (uint64_t)blockIdx.x * kBlock + threadIdx.x;            // [tile][block][row]
-    if (u >= total) return;
-    const uint32_t r = (uint32_t)(u % kMxTile);
-    const uint64_t tb = u / kMxTile, tile = tb / blocks;
-    const uint32_t b = (uint32_t)(tb - tile * blocks);
-    const uint64_t row = tile * kMxTile + r;
+    const uint64_t at = (uint64_t)blockIdx.x * kBlock + threadIdx.x;           // [tile][unit][operand][lane]
+    if (at >= total) return;
+    const uint32_t lane = (uint32_t)(at % 64u), operand = (uint32_t)(at / 64u % 4u);
+    const uint64_t tu = at / 256u, tile = tu / units;
+    const uint32_t b = (uint32_t)(tu - tile * units) * kMxUnit + operand / 2u * 4u + lane / 16u;
+    const uint64_t row = tile * kMxTile + operand % 2u * 16u + lane % 16u;
     const bool in = row < m && b < real;
     so_u32x4 v = {0u, 0u, 0u, 0u};
     if (in) v = src[row * real + b];
-    codes[u] = v;
-    if (b % kMxUnit >= 2) return;                                              // blocks 0 and 1 of a unit: the words of lanes r and 32 + r
-    uint32_t w = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) w |= (uint32_t)(row < m && b + 2 * j < real ? src_scales[row * real + b + 2 * j] : kMxZero) << (8 * j);
-    scales[(tile * (blocks / kMxUnit) + b / kMxUnit) * 64 + b % kMxUnit * 32 + r] = w;
+    codes[at] = v;
+    scales[so_mx_scale_at(row, b, units)] = in ? src_scales[row * real + b] : kMxZero;
 }
 
-// X [n x C] into tiles of columns: a thread takes one column and four blocks of a unit, all even or all odd ones, whose scales share a word.
+// The word of the lane whose number differs in bit 3, 4 or 5, joined with this one's by max.
+__device__ __forceinline__ uint32_t max_over_rows(uint32_t v)
+{
+    v = max(v, so_lanes::word_across<8>(v));
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(b[0], b[1]);
+}
+
+// X [n x C] into tiles of columns.  A wave takes one block of 32 rows and 8 lanes of columns, 128 bytes a row: a lane 4 rows of 16 bytes, the largest magnitude of a column
+// meets across its 8 lanes.  (One lane a column with its 32 rows, four blocks one after the other, left most of the chip idle: 2777 x 101 fp16 38.5 us.)
 template <class T>
 __global__ __launch_bounds__(kBlock)
-void mx_columns_kernel(const T *__restrict__ X, size_t ldx, uint32_t n, uint32_t C, uint32_t blocks, uint64_t total, so_u32x4 *__restrict__ codes, uint32_t *__restrict__ scales)
+void mx_columns_kernel(const T *__restrict__ X, size_t ldx, uint32_t n, uint32_t C, uint32_t units, uint32_t quads, so_u32x4 *__restrict__ codes, uint8_t *__restrict__ scales)
 {
-    const uint64_t u = (uint64_t)blockIdx.x * kBlock + threadIdx.x;            // [unit][odd][column]
-    if (u >= total) return;
-    const uint64_t q = u / C;
-    const uint32_t c = (uint32_t)(u - q * C), odd = (uint32_t)(q & 1), unit = (uint32_t)(q >> 1);
-    const uint64_t tile = c / kMxTile;
-    const uint32_t r = c % kMxTile;
-    uint32_t word = 0;
-    for (uint32_t j = 0; j < 4; ++j) {
-        const uint32_t b = unit * kMxUnit + 2 * j + odd;
-        const uint64_t k0 = (uint64_t)b * 32;
-        so_u32x4 v = {0u, 0u, 0u, 0u};
-        uint32_t s = kMxZero;
-        if (k0 < n) {
-            const T *p = X + k0 * ldx + c;
-            float f[32];
-            uint32_t top = 0;
+    constexpr int V = so_elements<T>::V;
+    const uint32_t group = blockIdx.x / quads, b = (blockIdx.x - group * quads) * 4u + threadIdx.x / 64u;
+    const uint32_t lane = threadIdx.x % 64u, r = lane / 8u;
+    const uint64_t c = ((uint64_t)group * 8u + lane % 8u) * V, k0 = (uint64_t)b * 32u + r * 4u;
+    const uint32_t left = c >= C ? 0u : (uint32_t)min((uint64_t)V, C - c);
+    const T *p = X + k0 * ldx + c;
+    typename so_elements<T>::plain x[4];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                f[i] = k0 + i < n ? (float)p[(size_t)i * ldx] : 0.0f;
-                top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-            }
-            s = so_mx_scale(top);
-            if (s != 255u) {
-                const float scale = so_mx_power(s);
+    for (int i = 0; i < 4; ++i)
+        if (k0 + i < n && left) x[i] = so_group_load(p + (size_t)i * ldx, left);
+        else x[i] = typename so_elements<T>::plain{};
+    float f[4][V];
+    uint32_t top[V] = {};
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const float e[8] = {f[8 * g], f[8 * g + 1], f[8 * g + 2], f[8 * g + 3], f[8 * g + 4], f[8 * g + 5], f[8 * g + 6], f[8 * g + 7]};
-                    v[g] = so_mx_codes(e, scale);
-                }
-            }
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            f[i][e] = (float)x[i][e];
+            top[e] = max(top[e], __float_as_uint(f[i][e]) & 0x7fffffffu);
         }
-        codes[(tile * blocks + b) * kMxTile + r] = v;
-        word |= s << (8 * j);
+    const bool padding = (uint64_t)b * 32u >= n;
+    uint32_t w[V], own = 0;                                      // 4 codes of every column; the scale of column r % V
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const uint32_t s = so_mx_scale(max_over_rows(top[e]));
+        const float scale = so_mx_power(s);
+        w[e] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, f[0][e], f[1][e], scale, 0);
+        w[e] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[e], f[2][e], f[3][e], scale, 1);
+        if (s == 255u) w[e] = 0;
+        own = r % V == (uint32_t)e ? s : own;
     }
-    scales[(tile * (blocks / kMxUnit) + unit) * 64 + odd * 32 + r] = word;
+    // Columns against lanes, a bit of both at a time: in the end a lane has column r % V, its 32 codes (16-bit types) or the 16 of its half of the lanes.
+    uint32_t two[V / 2];
+#pragma unroll
+    for (int p = 0; p < V / 2; ++p) {
+        const uint32_t keep = r % 2u ? w[2 * p + 1] : w[2 * p], other = so_lanes::word_across<8>(r % 2u ? w[2 * p] : w[2 * p + 1]);
+        two[p] = r % 2u ? other | keep << 16 : keep | other << 16;
+    }
+    const uint64_t col = c + r % V;
+    const bool mine = r % V < left;
+    const auto a0 = __builtin_amdgcn_permlane16_swap(two[0], two[1], false, false);
+    if constexpr (V == 4) {
+        if (mine) reinterpret_cast<uint2 *>(codes)[so_mx_code_at(col, b, units) * 2u + r / 4u] = make_uint2(a0[0], a0[1]);
+        if (mine && r < 4u) scales[so_mx_scale_at(col, b, units)] = padding ? kMxZero : own;
+    } else {
+        const auto a1 = __builtin_amdgcn_permlane16_swap(two[2], two[3], false, false);
+        const auto lo = __builtin_amdgcn_permlane32_swap(a0[0], a1[0], false, false), hi = __builtin_amdgcn_permlane32_swap(a0[1], a1[1], false, false);
+        const so_u32x4 v = {lo[0], hi[0], lo[1], hi[1]};
+        if (mine) {
+            codes[so_mx_code_at(col, b, units)] = v;
+            scales[so_mx_scale_at(col, b, units)] = padding ? kMxZero : own;
+        }
+    }
 }
 
 // Rows that lie without a gap and end with a block are one long row.
@@ -209,7 +234,7 @@ extern "C" so_status so_mxfp4_create(so_ctx *ctx, const uint8_t *dCodes, const u
     SO_HIP(hipMalloc(&W->d_blob, total * 17));
     W->d_codes = (so_u32x4 *)W->d_blob;
     W->d_scales = (uint32_t *)(W->d_codes + total);
-    mx_tile_kernel<<<so_ceil_div(total, kBlock), kBlock, 0, ctx->stream>>>((const so_u32x4 *)dCodes, dScales, m, so_ceil_div(n, 32), W->blocks, total, W->d_codes, W->d_scales);
+    mx_tile_kernel<<<so_ceil_div(total, kBlock), kBlock, 0, ctx->stream>>>((const so_u32x4 *)dCodes, dScales, m, so_ceil_div(n, 32), W->blocks / kMxUnit, total, W->d_codes, (uint8_t *)W->d_scales);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) {
         (void)hipFree(W->d_blob);
         so_set_error("kernel launch failed: %s (so_mxfp4_create)", hipGetErrorString(e));
@@ -238,12 +263,19 @@ extern "C" so_status so_mxfp4_dims(const so_mxfp4 *W, uint32_t *m, uint32_t *n)
 
 so_status so_mx_quantize_columns(so_ctx *ctx, int type, const void *dX, size_t x_stride, uint32_t n, uint32_t C, so_u32x4 *codes, uint32_t *scales)
 {
-    const uint32_t blocks = so_mx_blocks(n);
-    const uint64_t total = (uint64_t)(blocks / kMxUnit) * 2 * C;
+    const uint32_t blocks = so_mx_blocks(n), quads = blocks / 4;
+    so_status status = SO_OK;
     so_for_type(type, [&](auto t) {
         using T = decltype(t);
-        mx_columns_kernel<T><<<so_ceil_div(total, kBlock), kBlock, 0, ctx->stream>>>((const T *)dX, x_stride, n, C, blocks, total, codes, scales);
+        const uint64_t groups = (uint64_t)so_ceil_div(C, 8 * so_elements<T>::V) * quads;
+        if (groups >= (1ull << 31)) {
+            so_set_error("so_mxfp4_matmul: %u x %u input is too large for one launch", n, C);
+            status = SO_ERR_INVALID;
+            return;
+        }
+        mx_columns_kernel<T><<<(uint32_t)groups, kBlock, 0, ctx->stream>>>((const T *)dX, x_stride, n, C, blocks / kMxUnit, quads, codes, (uint8_t *)scales);
     });
+    if (status != SO_OK) return status;
     SO_LAUNCH_CHECK();
     return SO_OK;
 }

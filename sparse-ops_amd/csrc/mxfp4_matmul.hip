@@ -6,99 +6,271 @@
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-template <int J>
-__device__ __forceinline__ f32x16 mx_mfma(so_u32x4 x, uint32_t sx, so_u32x4 w, uint32_t sw, f32x16 acc)
+// 16 x 16 x 128 with both operands in 4 bits; X's columns are the first operand, so that a lane holds row l % 16 of W and the neighbouring columns 4 (l / 16) .. + 3 of Y.  On values as
+// they come this instruction reaches 7.35 PFLOP/s, 32 x 32 x 64 6.6: the chip's power is what bounds both (zeros: 9.8 for the latter).
+template <int JX, int JW>
+__device__ __forceinline__ f32x4 mx_mfma(so_u32x4 x, uint32_t sx, so_u32x4 w, uint32_t sw, f32x4 acc)
 {
     const i32x8 a = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0}, b = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc, 4, 4, J, (int)sx, J, (int)sw);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, JX, (int)sx, JW, (int)sw);
 }
 
-// Y tile of MT x CT tiles of 32 x 32, WK waves that share the blocks between them, a unit of 8 each in turn; their sums meet in LDS.  X's columns are the instruction's
-// first operand, so that a lane holds one row of W and four neighbouring columns of Y in each four registers.
-template <class T, int MT, int CT, int WK, int ACT>
+// f(0), f(1), ... as compile-time numbers.
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void each(F &&f)
+{
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>());
+        each<N, I + 1>(f);
+    }
+}
+
+// Which tile of the output a workgroup takes.  Workgroups go round-robin to the 8 XCDs; each XCD gets neighbouring tiles of a strip four tiles of columns wide, so that its L2 is
+// asked for few rows of W and few columns of X.
+struct MxTile { uint32_t m, c; bool none; };
+__device__ __forceinline__ MxTile mx_tile_of(uint32_t mgroups, uint32_t cgroups, uint32_t per_xcd)
+{
+    const uint32_t id = (blockIdx.x % 8u) * per_xcd + blockIdx.x / 8u;
+    if (id >= mgroups * cgroups) return {0, 0, true};
+    const uint32_t strip = id / (4u * mgroups), wide = min(4u, cgroups - strip * 4u), in = id - strip * 4u * mgroups;
+    return {in / wide, strip * 4u + in % wide, false};
+}
+
+// A tile of Y of 16 MH x 16 CH, WK waves that share the blocks between them, a unit of 8 each in turn, straight from memory to registers; their sums meet in LDS.
+template <class T, int MH, int CH, int WK, int ACT>
 __global__ __launch_bounds__(64 * WK)
 void mx_matmul_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restrict__ Ws, const so_u32x4 *__restrict__ Xc, const uint32_t *__restrict__ Xs, uint32_t m, uint32_t C,
-                      uint32_t units, uint32_t wtiles, uint32_t xtiles, uint32_t mgroups, uint32_t per_xcd, uint32_t groups, const float *__restrict__ bias, T *__restrict__ Y, size_t ldy)
+                      uint32_t units, uint32_t wtiles, uint32_t xtiles, uint32_t mgroups, uint32_t cgroups, uint32_t per_xcd, const float *__restrict__ bias, T *__restrict__ Y,
+                      size_t ldy)
 {
-    constexpr int V = so_elements<T>::V, PITCH = CT * 32 + 4;
-    extern __shared__ float lds[];                                   // [WK][MT * 32][PITCH]
-    // Workgroups go round-robin to the 8 XCDs: each gets neighbouring tiles, rows of W first, whose columns of X then stay in one L2.
-    const uint32_t id = (blockIdx.x % 8u) * per_xcd + blockIdx.x / 8u;
-    if (id >= groups) return;
-    const uint32_t mg = id % mgroups, cg = id / mgroups;
+    constexpr int V = so_elements<T>::V, PITCH = CH * 16 + 4, MW = (MH + 1) / 2, CW = (CH + 1) / 2;
+    static_assert((MH == 1 || MH % 2 == 0) && (CH == 1 || CH % 2 == 0), "half a tile of 32, or whole ones");
+    extern __shared__ float lds[];                                   // [WK][MH * 16][PITCH]
+    const MxTile tile = mx_tile_of(mgroups, cgroups, per_xcd);
+    if (tile.none) return;
     const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x % 64u;
-    const so_u32x4 *wc[MT], *xc[CT];
-    const uint32_t *ws[MT], *xs[CT];
+    // half a tile: its operands begin 64 lanes further, and its scales are the upper half of the words
+    const uint32_t mhalf = MH == 1 ? tile.m % 2u : 0u, chalf = CH == 1 ? tile.c % 2u : 0u;
+    const so_u32x4 *wc[MW], *xc[CW];
+    const uint32_t *ws[MW], *xs[CW];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const size_t t = min(mg * MT + i, wtiles - 1u);              // a tile that is not there: the last one again, not stored
-        wc[i] = Wc + t * units * 256 + lane;
+    for (int i = 0; i < MW; ++i) {
+        const size_t t = min(MH == 1 ? tile.m / 2u : tile.m * MW + i, wtiles - 1u);              // a tile that is not there: the last one again, not stored
+        wc[i] = Wc + t * units * 256 + mhalf * 64u + lane;
         ws[i] = Ws + t * units * 64 + lane;
     }
 #pragma unroll
-    for (int i = 0; i < CT; ++i) {
-        const size_t t = min(cg * CT + i, xtiles - 1u);
-        xc[i] = Xc + t * units * 256 + lane;
+    for (int i = 0; i < CW; ++i) {
+        const size_t t = min(CH == 1 ? tile.c / 2u : tile.c * CW + i, xtiles - 1u);
+        xc[i] = Xc + t * units * 256 + chalf * 64u + lane;
         xs[i] = Xs + t * units * 64 + lane;
     }
-    f32x16 acc[MT][CT] = {};
-    for (uint32_t u = wave; u < units; u += WK) {
-        so_u32x4 w[MT][4], x[CT][4];
-        uint32_t sw[MT], sx[CT];
+    struct Unit {
+        so_u32x4 w[2][MH], x[2][CH];
+        uint32_t sw[MW], sx[CW];
+    };
+    const auto load = [&](Unit &t, uint32_t u) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            sw[i] = ws[i][(size_t)u * 64];
+        for (int i = 0; i < MW; ++i) t.sw[i] = ws[i][(size_t)u * 64] >> mhalf * 16u;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[i][j] = wc[i][(size_t)u * 256 + j * 64];
+        for (int i = 0; i < CW; ++i) t.sx[i] = xs[i][(size_t)u * 64] >> chalf * 16u;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+            for (int i = 0; i < MH; ++i) t.w[q][i] = wc[i / 2][(size_t)u * 256 + q * 128 + i % 2 * 64];
+#pragma unroll
+            for (int i = 0; i < CH; ++i) t.x[q][i] = xc[i / 2][(size_t)u * 256 + q * 128 + i % 2 * 64];
         }
-#pragma unroll
-        for (int i = 0; i < CT; ++i) {
-            sx[i] = xs[i][(size_t)u * 64];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[i][j] = xc[i][(size_t)u * 256 + j * 64];
+    };
+    f32x4 acc[MH][CH] = {};
+    const auto multiply = [&](const Unit &t) {
+        each<2>([&](auto q) {
+            each<CH>([&](auto k) {
+                each<MH>([&](auto i) {
+                    constexpr int Q = decltype(q)::value, K = decltype(k)::value, I = decltype(i)::value;
+                    acc[I][K] = mx_mfma<K % 2 * 2 + Q, I % 2 * 2 + Q>(t.x[Q][K], t.sx[K / 2], t.w[Q][I], t.sw[I / 2], acc[I][K]);
+                });
+            });
+        });
+    };
+    // two units at a time, the next on its way while one is multiplied; behind the last one that one again
+    const uint32_t turns = wave < units ? (units - wave + WK - 1u) / WK : 0u;
+    if (turns) {
+        const uint32_t last = wave + (turns - 1u) * WK;
+        Unit a, b;
+        load(a, wave);
+        for (uint32_t t = 0; t + 1u < turns; t += 2u) {
+            load(b, wave + (t + 1u) * WK);
+            multiply(a);
+            load(a, min(wave + (t + 2u) * WK, last));
+            multiply(b);
         }
-        const auto step = [&](auto byte) {
-            constexpr int J = decltype(byte)::value;
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int k = 0; k < CT; ++k) acc[i][k] = mx_mfma<J>(x[k][J], sx[k], w[i][J], sw[i], acc[i][k]);
-        };
-        step(std::integral_constant<int, 0>());
-        step(std::integral_constant<int, 1>());
-        step(std::integral_constant<int, 2>());
-        step(std::integral_constant<int, 3>());
+        if (turns % 2u) multiply(a);
     }
-    float *mine = lds + (size_t)wave * MT * 32 * PITCH;
+    float *mine = lds + (size_t)wave * MH * 16 * PITCH;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MH; ++i)
 #pragma unroll
-        for (int k = 0; k < CT; ++k)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f32x4 v = {acc[i][k][4 * q], acc[i][k][4 * q + 1], acc[i][k][4 * q + 2], acc[i][k][4 * q + 3]};
-                *reinterpret_cast<f32x4 *>(mine + (i * 32 + lane % 32u) * PITCH + k * 32 + 8 * q + 4 * (lane / 32u)) = v;
-            }
+        for (int k = 0; k < CH; ++k) *reinterpret_cast<f32x4 *>(mine + (i * 16 + lane % 16u) * PITCH + k * 16 + 4 * (lane / 16u)) = acc[i][k];
     __syncthreads();
-    constexpr int GR = CT * 32 / V;                                  // groups of 16 bytes in a row of the tile
-    for (uint32_t g = threadIdx.x; g < MT * 32 * GR; g += 64 * WK) {
+    constexpr int GR = CH * 16 / V;                                  // groups of 16 bytes in a row of the tile
+    for (uint32_t g = threadIdx.x; g < MH * 16 * GR; g += 64 * WK) {
         const uint32_t r = g / GR, c = g % GR * V;
-        const uint64_t row = (uint64_t)mg * (MT * 32) + r, col = (uint64_t)cg * (CT * 32) + c;
+        const uint64_t row = (uint64_t)tile.m * (MH * 16) + r, col = (uint64_t)tile.c * (CH * 16) + c;
         if (row >= m || col >= C) continue;
-        const float b = bias ? bias[row] : 0.0f;
+        const float add = bias ? bias[row] : 0.0f;
         float y[V];
 #pragma unroll
         for (int e = 0; e < V; e += 4) {
             f32x4 s = *reinterpret_cast<const f32x4 *>(lds + r * PITCH + c + e);
 #pragma unroll
-            for (int w = 1; w < WK; ++w) s += *reinterpret_cast<const f32x4 *>(lds + ((size_t)w * MT * 32 + r) * PITCH + c + e);
+            for (int w = 1; w < WK; ++w) s += *reinterpret_cast<const f32x4 *>(lds + ((size_t)w * MH * 16 + r) * PITCH + c + e);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[e + i] = so_epilogue<ACT>(s[i] + b);
+            for (int i = 0; i < 4; ++i) y[e + i] = so_epilogue<ACT>(s[i] + add);
         }
         so_group_store(Y + row * ldy + col, (uint32_t)min((uint64_t)V, C - col), y);
+    }
+}
+
+// The same for large products: a tile of (16 MH WM) x (16 CH WC), its waves WM x WC, each MH x CH operands.  Half a unit (128 entries a row) of W and of X at a time goes to LDS as it
+// lies in memory, in a ring of four, each wave bringing as many tiles of 32 rows as the others.
+template <class T, int MH, int CH, int WM, int WC, int ACT>
+__global__ __launch_bounds__(64 * WM * WC)
+void mx_matmul_staged_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restrict__ Ws, const so_u32x4 *__restrict__ Xc, const uint32_t *__restrict__ Xs, uint32_t m, uint32_t C,
+                             uint32_t units, uint32_t wtiles, uint32_t xtiles, uint32_t mgroups, uint32_t cgroups, uint32_t per_xcd, const float *__restrict__ bias, T *__restrict__ Y,
+                             size_t ldy)
+{
+    constexpr int V = so_elements<T>::V, WT = MH * WM / 2, XT = CH * WC / 2, WAVES = WM * WC, EACH = WT / WAVES;
+    static_assert(WT == XT && WT % WAVES == 0, "a wave brings as many tiles of W and of X as every other");
+    constexpr uint32_t RING = 4, X0 = WT * 2048, STAGE = (WT + XT) * 2048, S0 = RING * STAGE, SCALES = (WT + XT) * 256;
+    extern __shared__ char stage[];
+    const MxTile tile = mx_tile_of(mgroups, cgroups, per_xcd);
+    if (tile.none) return;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), lane = threadIdx.x % 64u;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)stage;
+    // Request P of this wave for half h, of W's codes, X's codes and, in the even halves, their scales for each of its tiles.
+    const auto request = [&](uint32_t h, auto piece) {
+        constexpr int P = decltype(piece)::value, I = P % EACH, KIND = P / EACH;                 // kinds 0, 1: W; 2, 3: X; 4, 5: scales
+        const uint32_t t = I * WAVES + wave;
+        const size_t at = (KIND < 2 || KIND == 4 ? (size_t)min(tile.m * WT + t, wtiles - 1u) : (size_t)min(tile.c * XT + t, xtiles - 1u)) * units;   // not there: the last one again, not stored
+        if constexpr (KIND < 4) {
+            const uint32_t to = lds0 + h % RING * STAGE + (KIND < 2 ? 0u : X0) + t * 2048u + KIND % 2 * 1024u;
+            const char *src = reinterpret_cast<const char *>(KIND < 2 ? Wc : Xc) + at * 4096 + (size_t)h * 2048 + KIND % 2 * 1024;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(lane * 16u), "s"(src) : "memory", "m0");
+        } else {
+            const uint32_t to = lds0 + S0 + h / 2u % RING * SCALES + ((KIND == 4 ? 0u : WT) + t) * 256u;
+            const char *src = reinterpret_cast<const char *>(KIND == 4 ? Ws : Xs) + (at + h / 2u) * 256;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(to), "v"(lane * 4u), "s"(src) : "memory", "m0");
+        }
+    };
+    const auto bring = [&](uint32_t h, auto odd) { each<(decltype(odd)::value ? 4 : 6) * EACH>([&](auto piece) { request(h, piece); }); };
+    constexpr int ASKS = 10 * EACH;                                  // requests of two halves, one of them with scales
+    // All but the last ASKS (or 0) requests have come in LDS, and all waves are done with what they read before.
+    const auto meet = [&](auto more) {
+        if constexpr (decltype(more)::value) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(ASKS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+    };
+    const uint32_t wm = wave / WC, wc = wave % WC;
+    struct Scales { uint32_t w[MH / 2], x[CH / 2]; };
+    const auto scales = [&](Scales &s, uint32_t u) {
+        const char *from = stage + S0 + u % RING * SCALES + lane * 4;
+#pragma unroll
+        for (int i = 0; i < MH / 2; ++i) s.w[i] = *reinterpret_cast<const uint32_t *>(from + (wm * (MH / 2) + i) * 256);
+#pragma unroll
+        for (int k = 0; k < CH / 2; ++k) s.x[k] = *reinterpret_cast<const uint32_t *>(from + (WT + wc * (CH / 2) + k) * 256);
+    };
+    const auto wat = [&](uint32_t h, int i) { return *reinterpret_cast<const so_u32x4 *>(stage + h % RING * STAGE + (wm * MH + i) * 1024 + lane * 16); };
+    const auto xat = [&](uint32_t h, int k) { return *reinterpret_cast<const so_u32x4 *>(stage + h % RING * STAGE + X0 + (wc * CH + k) * 1024 + lane * 16); };
+    f32x4 acc[MH][CH] = {};
+    so_u32x4 w[2][MH], x[CH];
+    Scales e, next;
+    const uint32_t halves = 2u * units;
+    const std::integral_constant<int, 0> even;
+    const std::integral_constant<int, 1> odd;
+    bring(0, even);
+    bring(1, odd);
+    if (halves > 2u) {
+        bring(2, even);
+        bring(3, odd);
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"(ASKS + 4 * EACH) : "memory");
+    } else {
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" : : : "memory");
+    }
+    scales(e, 0);
+#pragma unroll
+    for (int i = 0; i < MH; ++i) w[0][i] = wat(0, i);
+#pragma unroll
+    for (int k = 0; k < CH; ++k) x[k] = xat(0, k);
+    // Half h's products; the operands of half h + 1 take the places of those that have been multiplied for the last time.  Behind the last half they are read from a place of the
+    // ring that holds an older one, and not used.
+    const auto half = [&](uint32_t h, auto q, auto wait, auto more) {
+        constexpr int Q = decltype(q)::value;
+        meet(wait);                                                  // half h + 1 is there, the two after it may be on their way; half h is in registers
+        if constexpr (Q == 1) scales(next, (h + 1u) / 2u);
+#pragma unroll
+        for (int i = 0; i < MH; ++i) w[1 - Q][i] = wat(h + 1u, i);
+        __builtin_amdgcn_sched_barrier(0);
+        each<CH>([&](auto k) {
+            constexpr int K = decltype(k)::value;
+            each<MH>([&](auto i) {
+                constexpr int I = decltype(i)::value;
+                acc[I][K] = mx_mfma<K % 2 * 2 + Q, I % 2 * 2 + Q>(x[K], e.x[K / 2], w[Q][I], e.w[I / 2], acc[I][K]);
+            });
+            x[K] = xat(h + 1u, K);
+            // The requests for half h + 4, into the place of half h, one after each group of products: all at once they hold up every wave of the workgroup at the same time.
+            constexpr int PIECES = (Q == 1 ? 4 : 6) * EACH, FROM = K * PIECES / CH, TO = (K + 1) * PIECES / CH;
+            if constexpr (decltype(more)::value && TO > FROM)
+                each<TO - FROM>([&](auto i) { request(h + 4u, std::integral_constant<int, FROM + decltype(i)::value>()); });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (Q == 1) e = next;
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    uint32_t h = 0;
+    for (; h + 4u < halves; h += 2u) {
+        half(h, even, yes, yes);
+        half(h + 1u, odd, yes, yes);
+    }
+    if (h + 2u < halves) {                                           // the last unit but one: nothing left to ask for
+        half(h, even, yes, no);
+        half(h + 1u, odd, no, no);
+        h += 2u;
+    }
+    half(h, even, no, no);
+    half(h + 1u, odd, no, no);
+    __syncthreads();
+    // Out through LDS, each wave in a part of its own, 32 rows at a time: a lane's four columns of one row become 16 bytes of a row that 8 or 16 lanes store together.
+    constexpr int COLS = CH * 16, PITCH = COLS + 4, LANES = COLS / V, ROWS = 64 / LANES;
+    float *mine = reinterpret_cast<float *>(stage) + wave * 32 * PITCH;
+    const uint64_t col = (uint64_t)tile.c * (XT * 32) + wc * COLS + lane % LANES * V;
+#pragma unroll
+    for (int i = 0; i < MH; i += 2) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int k = 0; k < CH; ++k) *reinterpret_cast<f32x4 *>(mine + (j * 16 + lane % 16u) * PITCH + k * 16 + 4 * (lane / 16u)) = acc[i + j][k];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += ROWS) {
+            const uint32_t r = r0 + lane / LANES;
+            const uint64_t row = (uint64_t)tile.m * (WT * 32) + (wm * MH + i) * 16 + r;
+            float y[V];
+#pragma unroll
+            for (int f = 0; f < V; f += 4) {
+                const f32x4 s = *reinterpret_cast<const f32x4 *>(mine + r * PITCH + lane % LANES * V + f);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[f + k] = s[k];
+            }
+            if (row >= m || col >= C) continue;
+            const float add = bias ? bias[row] : 0.0f;
+#pragma unroll
+            for (int f = 0; f < V; ++f) y[f] = so_epilogue<ACT>(y[f] + add);
+            so_group_store(Y + row * ldy + col, (uint32_t)min((uint64_t)V, C - col), y);
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -118,27 +290,74 @@ so_status reserve(so_ctx *ctx, const char *who, const so_mxfp4 *W, uint32_t C)
     return so_matmul_workspace(ctx, s.codes + s.scales, 4);
 }
 
-template <class T, int MT, int CT, int WK, int ACT>
+struct Groups { uint32_t m, c, per_xcd; };
+so_status groups_of(const so_mxfp4 *W, uint32_t C, uint32_t rows, uint32_t cols, Groups *g)
+{
+    g->m = so_ceil_div(W->m, rows);
+    g->c = so_ceil_div(C, cols);
+    SO_REQUIRE((uint64_t)g->m * g->c < (1ull << 30), "so_mxfp4_matmul: %u x %u output is too large for one launch", W->m, C);
+    g->per_xcd = so_ceil_div((uint64_t)g->m * g->c, 8);
+    return SO_OK;
+}
+
+template <class T, int MH, int CH, int WK, int ACT>
 so_status launch(so_ctx *ctx, const so_mxfp4 *W, const so_u32x4 *codes, const uint32_t *scales, uint32_t C, const float *bias, T *Y, size_t ldy)
 {
-    const uint32_t xtiles = so_ceil_div(C, kMxTile), mgroups = so_ceil_div(W->tiles, MT);
-    const uint64_t groups = (uint64_t)mgroups * so_ceil_div(xtiles, CT);
-    SO_REQUIRE(groups < (1ull << 30), "so_mxfp4_matmul: %u x %u output is too large for one launch", W->m, C);
-    const uint32_t per_xcd = so_ceil_div(groups, 8);
-    constexpr uint32_t bytes = WK * MT * 32 * (CT * 32 + 4) * sizeof(float);
-    const auto kernel = mx_matmul_kernel<T, MT, CT, WK, ACT>;
+    Groups g;
+    if (const so_status s = groups_of(W, C, MH * 16, CH * 16, &g); s != SO_OK) return s;
+    constexpr uint32_t bytes = WK * MH * 16 * (CH * 16 + 4) * sizeof(float);
+    const auto kernel = mx_matmul_kernel<T, MH, CH, WK, ACT>;
     if (bytes > 48 * 1024) SO_HIP(so_allow_big_lds(ctx, (const void *)kernel));
-    kernel<<<per_xcd * 8, 64 * WK, bytes, ctx->stream>>>(W->d_codes, W->d_scales, codes, scales, W->m, C, W->blocks / kMxUnit, W->tiles, xtiles, mgroups, per_xcd, (uint32_t)groups,
-                                                        bias, Y, ldy);
+    kernel<<<g.per_xcd * 8, 64 * WK, bytes, ctx->stream>>>(W->d_codes, W->d_scales, codes, scales, W->m, C, W->blocks / kMxUnit, W->tiles, so_ceil_div(C, kMxTile), g.m, g.c, g.per_xcd,
+                                                          bias, Y, ldy);
     SO_LAUNCH_CHECK();
     return SO_OK;
+}
+
+template <class T, int MH, int CH, int WM, int WC, int ACT>
+so_status launch_staged(so_ctx *ctx, const so_mxfp4 *W, const so_u32x4 *codes, const uint32_t *scales, uint32_t C, const float *bias, T *Y, size_t ldy)
+{
+    Groups g;
+    if (const so_status s = groups_of(W, C, MH * WM * 16, CH * WC * 16, &g); s != SO_OK) return s;
+    constexpr uint32_t bytes = std::max<uint32_t>(4 * (MH * WM + CH * WC) / 2 * (2048 + 256), WM * WC * 32 * (CH * 16 + 4) * sizeof(float));
+    const auto kernel = mx_matmul_staged_kernel<T, MH, CH, WM, WC, ACT>;
+    SO_HIP(so_allow_big_lds(ctx, (const void *)kernel));
+    kernel<<<g.per_xcd * 8, 64 * WM * WC, bytes, ctx->stream>>>(W->d_codes, W->d_scales, codes, scales, W->m, C, W->blocks / kMxUnit, W->tiles, so_ceil_div(C, kMxTile), g.m, g.c, g.per_xcd,
+                                                               bias, Y, ldy);
+    SO_LAUNCH_CHECK();
+    return SO_OK;
+}
+
+// The forms, by tile: rows and columns of Y.  Up to 64 x 64 the waves of a workgroup share the blocks.
+struct Form { uint32_t rows, cols; const char *name; };
+constexpr Form kForms[] = {{16, 16, "mx-16x16"}, {32, 16, "mx-32x16"}, {32, 32, "mx-32x32"}, {64, 32, "mx-64x32"}, {64, 64, "mx-64x64"}, {64, 64, "mx-64x64-four"}, {128, 128, "mx-128x128"},
+                           {256, 256, "mx-256x256"}};
+constexpr int kFormCount = 8;
+
+// The largest tile that gives every compute unit a workgroup: a larger one asks the caches for less, a smaller one leaves none idle.  From a sweep over m of 64 .. 8192, n of 512 .. 8192
+// and C of 1 .. 2048 (fp32, with the quantisation; us), this form / the next smaller: 8192 x 8192 x 2048 256 x 256 76.3 / 96.3, 4096 x 8192 x 1024 128 x 128 38.0 / 39.7, 4096 x 8192 x 512
+// 64 x 64 on four waves 23.5 / 27.9 on eight, 4096 x 8192 x 256 64 x 64 16.3 / 18.7, 2048 x 8192 x 256 64 x 32 13.2 / 14.1, 1024 x 8192 x 256 32 x 32 9.9 / 12.4, 2048 x 8192 x 64 32 x 16
+// 8.2 / 9.0; with half as many workgroups as compute units the larger loses by as much (4096 x 8192 x 2048: 256 x 256 61.5, 128 x 128 56.3).
+int choose_form(const so_ctx *ctx, uint32_t m, uint32_t C)
+{
+    const uint64_t cus = (uint64_t)ctx->compute_units;
+    const auto tiles = [&](int f) { return (uint64_t)so_ceil_div(m, kForms[f].rows) * so_ceil_div(C, kForms[f].cols); };
+    const auto rounds = [](uint64_t tiles, uint64_t at_once) { return (tiles + at_once - 1) / at_once; };
+    if (tiles(6) >= cus) {
+        // one tile of 256 x 256 a compute unit at a time takes 0.78 of what its four quarters take, two of those at a time
+        return 4.0 * (double)rounds(tiles(7), cus) <= 1.28 * 2.0 * (double)rounds(tiles(6), 2 * cus) ? 7 : 6;
+    }
+    if (tiles(5) >= 2 * cus) return 5;
+    for (int f = 4; f > 0; --f)
+        if (tiles(f) >= cus) return f;
+    return 0;
 }
 
 constexpr int kVecThreads = 512, kVecWaves = kVecThreads / 64;
 constexpr uint32_t kVecChunk = 8192;         // entries of x in LDS at a time
 
 // y = W x + bias with x in fp32: a workgroup takes RT tiles of 32 rows, its waves a unit of 8 blocks each in turn.  A lane multiplies one block of a row with x from LDS, which
-// the rows share, as whole numbers of halves, and the block's sum with its scale.
+// the rows share, and the block's sum with its scale.
 template <int RT>
 __global__ __launch_bounds__(kVecThreads)
 void mx_matvec_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restrict__ Ws, const float *__restrict__ x, uint32_t m, uint32_t n, uint32_t units, uint32_t tiles,
@@ -155,7 +374,7 @@ void mx_matvec_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restric
         wc[i] = Wc + t * units * 256 + lane;
         ws[i] = Ws + t * units * 64 + lane;
     }
-    float acc[RT] = {};
+    float acc[RT][2] = {};
     constexpr uint32_t CU = kVecChunk / 256;                         // units of a chunk
     for (uint32_t u0 = 0; u0 < units; u0 += CU) {
         const uint32_t here = min(units - u0, CU);
@@ -175,40 +394,49 @@ void mx_matvec_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restric
                 for (int j = 0; j < 4; ++j) w[i][j] = wc[i][(size_t)(u0 + u) * 256 + j * 64];
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f32x4 *xp = xs + (u * 8 + 2 * j + lane / 32u) * 8;
-                float sum[RT] = {};
+            for (int q = 0; q < 2; ++q) {
+                const f32x4 *xp = xs + (u * 8 + 4 * q + lane / 16u) * 8;
+                float sum[RT][2] = {};
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const f32x4 a = xp[2 * g], b = xp[2 * g + 1];
 #pragma unroll
-                    for (int i = 0; i < RT; ++i) {
-                        const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i][j][g], 1.0f, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i][j][g], 1.0f, 1);
-                        const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i][j][g], 1.0f, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i][j][g], 1.0f, 3);
-                        sum[i] = fmaf(p0[0], a[0], sum[i]);
-                        sum[i] = fmaf(p0[1], a[1], sum[i]);
-                        sum[i] = fmaf(p1[0], a[2], sum[i]);
-                        sum[i] = fmaf(p1[1], a[3], sum[i]);
-                        sum[i] = fmaf(p2[0], b[0], sum[i]);
-                        sum[i] = fmaf(p2[1], b[1], sum[i]);
-                        sum[i] = fmaf(p3[0], b[2], sum[i]);
-                        sum[i] = fmaf(p3[1], b[3], sum[i]);
-                    }
+                    for (int i = 0; i < RT; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t c = w[i][2 * q + h][g];
+                            float &s = sum[i][h];
+                            const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
+                            const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
+                            s = fmaf(p0[0], a[0], s);
+                            s = fmaf(p0[1], a[1], s);
+                            s = fmaf(p1[0], a[2], s);
+                            s = fmaf(p1[1], a[3], s);
+                            s = fmaf(p2[0], b[0], s);
+                            s = fmaf(p2[1], b[1], s);
+                            s = fmaf(p3[0], b[2], s);
+                            s = fmaf(p3[1], b[3], s);
+                        }
                 }
 #pragma unroll
-                for (int i = 0; i < RT; ++i) {
-                    const uint32_t s = sc[i] >> (8 * j) & 255u;
-                    acc[i] = fmaf(sum[i], s == 255u ? __builtin_nanf("") : so_mx_power(s), acc[i]);
-                }
+                for (int i = 0; i < RT; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t s = sc[i] >> (16 * h + 8 * q) & 255u;
+                        acc[i][h] = fmaf(sum[i][h], s == 255u ? __builtin_nanf("") : so_mx_power(s), acc[i][h]);
+                    }
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i]), __float_as_uint(acc[i]), false, false);
-        const float s = __uint_as_float(h[0]) + __uint_as_float(h[1]);
-        if (lane < 32u) part[wave][i * 32 + lane] = s;
-    }
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {                                // the four blocks of a row lie 16 lanes apart
+            const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i][h]), __float_as_uint(acc[i][h]), false, false);
+            const float s = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+            const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+            if (lane < 16u) part[wave][i * 32 + h * 16 + lane] = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+        }
     __syncthreads();
     const uint64_t row = (uint64_t)blockIdx.x * (RT * 32) + threadIdx.x;
     if (threadIdx.x < RT * 32 && row < m) {
@@ -246,13 +474,25 @@ extern "C" so_status so_mxfp4_matmul(so_ctx *ctx, const so_mxfp4 *W, int type, c
     so_u32x4 *codes = (so_u32x4 *)ctx->mm_part->p;
     uint32_t *scales = (uint32_t *)((char *)codes + workspace_of(W, C).codes);
     if (const so_status s = so_mx_quantize_columns(ctx, type, dX, x_stride, W->n, C, codes, scales); s != SO_OK) return s;
-    const bool large = (uint64_t)so_ceil_div(W->tiles, 2) * so_ceil_div(C, 64) >= (uint64_t)ctx->compute_units;
+    const Form &form = kForms[ctx->tune.mxfp4_form >= 1 && ctx->tune.mxfp4_form <= kFormCount ? ctx->tune.mxfp4_form - 1 : choose_form(ctx, W->m, C)];
+    ctx->last_kernel = form.name;
     so_status status = SO_OK;
     so_for_type(type, [&](auto t) {
         using T = decltype(t);
         const auto with = [&](auto a) {
             constexpr int ACT = decltype(a)::value;
-            status = large ? launch<T, 2, 2, 4, ACT>(ctx, W, codes, scales, C, dBias, (T *)dY, y_stride) : launch<T, 1, 1, 8, ACT>(ctx, W, codes, scales, C, dBias, (T *)dY, y_stride);
+            T *y = (T *)dY;
+            const auto run = [&](auto kernel) { status = kernel(ctx, W, codes, scales, C, dBias, y, y_stride); };
+            switch (&form - kForms) {
+            case 0: run(launch<T, 1, 1, 8, ACT>); break;
+            case 1: run(launch<T, 2, 1, 8, ACT>); break;
+            case 2: run(launch<T, 2, 2, 8, ACT>); break;
+            case 3: run(launch<T, 4, 2, 8, ACT>); break;
+            case 4: run(launch<T, 4, 4, 8, ACT>); break;
+            case 5: run(launch<T, 4, 4, 4, ACT>); break;
+            case 6: run(launch_staged<T, 4, 4, 2, 2, ACT>); break;
+            default: run(launch_staged<T, 4, 8, 4, 2, ACT>); break;
+            }
         };
         if (act == SO_ACT_RELU) with(std::integral_constant<int, SO_ACT_RELU>());
         else if (act == SO_ACT_SIGMOID) with(std::integral_constant<int, SO_ACT_SIGMOID>());

@@ -115,6 +115,33 @@ def test_matmul(ctx, m, n, C, type_, act):
     handle.free()
 
 
+FORMS = ["mx-16x16", "mx-32x16", "mx-32x32", "mx-64x32", "mx-64x64", "mx-64x64-four", "mx-128x128", "mx-256x256"]
+
+
+@pytest.mark.parametrize("form", range(1, len(FORMS) + 1))
+@pytest.mark.parametrize("m,n,C", [(1, 40, 1), (70, 256, 33), (300, 257, 300), (257, 600, 17), (40, 1300, 530), (530, 2500, 65)])
+def test_matmul_on_every_tile(ctx, m, n, C, form):
+    """Each kernel form where another would be chosen: tiles that end inside the matrix, one to ten units of the contraction."""
+    rng = np.random.default_rng(m + 7 * n + 13 * C)
+    handle, W = weights(ctx, rng, m, n)
+    for type_ in ("f32", "bf16"):
+        X = values(stored(rng.standard_normal((n, C)), type_), type_)
+        Xq = mx.dequantize(*mx.quantize(np.ascontiguousarray(X.T)), n).T
+        bias = rng.standard_normal(m).astype(np.float32)
+        want = activated(W @ Xq + bias.astype(np.float64)[:, None], "relu")
+        whole, dX = place(ctx, X, type_, 1, 0)
+        out, dY = place(ctx, np.zeros((m, C)), type_, 2, 1, fill=-5.0)
+        with ctx.tuning(SPARSEOPS_MXFP4_MATMUL=form):
+            ctx.mxfp4_matmul(handle, dX, C, ctx.array(bias), dY, "relu", type=type_, x_stride=C + 1, y_stride=C + 2)
+        assert ctx.last_kernel() == FORMS[form - 1]
+        Y, rest = fetch(out, m, C, type_, 2, 1)
+        assert np.all(np.abs(Y - want) <= product_tolerance(W, Xq, bias, want, "relu", type_))
+        assert np.all(rest == -5.0), "places that are not the result's were written"
+        whole.free()
+        out.free()
+    handle.free()
+
+
 @pytest.mark.parametrize("m,n", [(1, 1), (5, 31), (32, 32), (33, 1000), (1024, 1024), (1000, 8193), (70, 20000), (17000, 300), (40000, 40)])
 def test_matvec(ctx, m, n):
     """x is fp32 and stays so: a block is a chain of 32 additions, its waves' and chunks' sums a few dozen more."""
