@@ -87,6 +87,7 @@ static void read_tuning(so_tuning &t)
     t.conv_vec = env_int("SPARSEOPS_CONV_VEC", 0);
     t.conv_columns = env_int("SPARSEOPS_CONV_COLUMNS", -1);
     t.conv_rbm = env_int("SPARSEOPS_CONV_RBM", -1);
+    t.norm_lanes = env_int("SPARSEOPS_NORM_LANES", -1);
     t.mxfp4_form = env_int("SPARSEOPS_MXFP4_MATMUL", 0);
     t.wait_spins = env_int("SPARSEOPS_WAIT_SPINS", -1);
 }

@@ -11,7 +11,7 @@ from elements import HALF_STEP, SMALLEST, TYPES, U, fetch, place, stored, values
 pytestmark = pytest.mark.gpu
 
 EPS = 1e-5
-SHAPES = [(1, 1), (1, 6), (7, 1), (64, 3), (97, 13), (257, 9), (1000, 33), (2049, 65), (4096, 1), (5000, 2), (301, 700), (8200, 17), (784, 64), (4099, 40), (128, 2500)]
+SHAPES = [(1, 1), (1, 6), (7, 1), (64, 3), (97, 13), (257, 9), (1000, 33), (2049, 65), (4096, 1), (5000, 2), (301, 700), (8200, 17), (784, 64), (4099, 40), (128, 2500), (16384, 5), (16385, 3), (20000, 12)]
 
 
 def problem(F, B, type_, seed=0, mean=0.5):
@@ -57,6 +57,23 @@ def test_forward(ctx, F, B, type_):
         assert np.all(rest == -5.0), "places that are not the result's were written"
         for a in (whole, out, dG, dB, dM, dR):
             a.free()
+
+
+@pytest.mark.parametrize("lanes", [0, 1, 2, 4, 8])
+@pytest.mark.parametrize("F,B", [(1, 1), (70, 9), (600, 40), (2049, 65), (4000, 130), (9000, 20)])
+def test_forward_however_it_is_cut(ctx, F, B, lanes):
+    """Every number of lanes a row of the kernel that holds all features, and the two kernels that share them out."""
+    for type_ in ("f32", "bf16"):
+        _, X, gamma, beta = problem(F, B, type_, seed=2)
+        whole, dX = place(ctx, X, type_, 3, 1)
+        out, dY = place(ctx, np.zeros((F, B)), type_, 2, 1, fill=-5.0)
+        dM, dR = ctx.empty((B,)), ctx.empty((B,))
+        with ctx.tuning(SPARSEOPS_NORM_LANES=lanes):
+            ctx.layer_norm(dX, F, B, ctx.array(gamma), ctx.array(beta), EPS, dY, dM, dR, type=type_, x_stride=B + 3, y_stride=B + 2)
+        Y, rest = fetch(out, F, B, type_, 2, 1)
+        check_forward(Y, X, gamma, beta, type_)
+        check_statistics(dM.download(), dR.download(), X)
+        assert np.all(rest == -5.0), "places that are not the result's were written"
 
 
 def check_grad(dx, dgamma, dbeta, X, dY, gamma, mean, rstd, type_):
@@ -207,10 +224,10 @@ def test_recorded_and_replayed(ctx):
     fresh = hipabi.Context()
     try:
         with pytest.raises(hipabi.SoError, match="so_layer_norm_reserve"):
-            a = fresh.empty((64, 64))
+            a = fresh.empty((20000, 8))
             fresh.graph_begin()
             try:
-                fresh.layer_norm(a, 64, 64, None, None, EPS, a)
+                fresh.layer_norm(a, 20000, 8, None, None, EPS, a)
             finally:
                 fresh.graph_free(fresh.graph_end())
         for F, B, type_ in shapes:
