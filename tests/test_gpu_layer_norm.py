@@ -111,6 +111,27 @@ def test_gradient(ctx, F, B, type_):
             a.free()
 
 
+@pytest.mark.parametrize("lanes", [0, 1, 2, 4, 8])
+@pytest.mark.parametrize("F,B", [(1, 1), (70, 9), (600, 40), (2049, 65), (4000, 130), (8100, 20), (9000, 3), (300, 9001), (1100, 5003)])
+def test_gradient_however_it_is_cut(ctx, F, B, lanes):
+    """Every number of lanes a row of the kernel that holds all features, with one tile or several for a workgroup, and the two kernels that share the features out."""
+    for type_ in ("f32", "bf16"):
+        rng, X, gamma, _ = problem(F, B, type_, seed=9)
+        dY = values(stored(0.1 * rng.standard_normal((F, B)), type_), type_)
+        mean, rstd = (s.astype(np.float32) for s in statistics(X))
+        whole, dX = place(ctx, X, type_, 3, 1)
+        whole2, dDy = place(ctx, dY, type_, 1, 0)
+        out, dDx = place(ctx, np.zeros((F, B)), type_, 2, 1, fill=-5.0)
+        dDg, dDb = ctx.empty((F,)), ctx.empty((F,))
+        with ctx.tuning(SPARSEOPS_NORM_LANES=lanes):
+            ctx.layer_norm_grad(dX, dDy, F, B, ctx.array(gamma), ctx.array(mean), ctx.array(rstd), dDx, dDg, dDb, type=type_, x_stride=B + 3, dy_stride=B + 1, dx_stride=B + 2)
+        dx, rest = fetch(out, F, B, type_, 2, 1)
+        check_grad(dx, dDg.download(), dDb.download(), X, dY, gamma, mean, rstd, type_)
+        assert np.all(rest == -5.0), "places that are not the result's were written"
+        for a in (whole, whole2, out):
+            a.free()
+
+
 def test_gradient_is_that_of_the_forward_pass(ctx):
     """Central differences of sum(Y * dY) along X, gamma and beta, from the kernel's own forward pass in fp32: with steps of 2^-6 the third derivative and the roundings of the
     sum are below the bound of one part in a hundred of the gradient's largest entry."""
