@@ -101,10 +101,10 @@ __device__ __forceinline__ uint32_t max_over_rows(uint32_t v)
 // meets across its 8 lanes.  (One lane a column with its 32 rows, four blocks one after the other, left most of the chip idle: 2777 x 101 fp16 38.5 us.)
 template <class T>
 __global__ __launch_bounds__(kBlock)
-void mx_columns_kernel(const T *__restrict__ X, size_t ldx, uint32_t n, uint32_t C, uint32_t units, uint32_t quads, so_u32x4 *__restrict__ codes, uint8_t *__restrict__ scales)
+void mx_columns_kernel(const T *__restrict__ X, size_t ldx, uint32_t n, uint32_t C, uint32_t units, uint32_t across, so_u32x4 *__restrict__ codes, uint8_t *__restrict__ scales)
 {
     constexpr int V = so_elements<T>::V;
-    const uint32_t group = blockIdx.x / quads, b = (blockIdx.x - group * quads) * 4u + threadIdx.x / 64u;
+    const uint32_t quad = blockIdx.x / across, group = blockIdx.x - quad * across, b = quad * 4u + threadIdx.x / 64u;     // as X lies in memory
     const uint32_t lane = threadIdx.x % 64u, r = lane / 8u;
     const uint64_t c = ((uint64_t)group * 8u + lane % 8u) * V, k0 = (uint64_t)b * 32u + r * 4u;
     const uint32_t left = c >= C ? 0u : (uint32_t)min((uint64_t)V, C - c);
@@ -267,13 +267,14 @@ so_status so_mx_quantize_columns(so_ctx *ctx, int type, const void *dX, size_t x
     so_status status = SO_OK;
     so_for_type(type, [&](auto t) {
         using T = decltype(t);
-        const uint64_t groups = (uint64_t)so_ceil_div(C, 8 * so_elements<T>::V) * quads;
+        const uint32_t across = so_ceil_div(C, 8 * so_elements<T>::V);
+        const uint64_t groups = (uint64_t)across * quads;
         if (groups >= (1ull << 31)) {
             so_set_error("so_mxfp4_matmul: %u x %u input is too large for one launch", n, C);
             status = SO_ERR_INVALID;
             return;
         }
-        mx_columns_kernel<T><<<(uint32_t)groups, kBlock, 0, ctx->stream>>>((const T *)dX, x_stride, n, C, blocks / kMxUnit, quads, codes, (uint8_t *)scales);
+        mx_columns_kernel<T><<<(uint32_t)groups, kBlock, 0, ctx->stream>>>((const T *)dX, x_stride, n, C, blocks / kMxUnit, across, codes, (uint8_t *)scales);
     });
     if (status != SO_OK) return status;
     SO_LAUNCH_CHECK();

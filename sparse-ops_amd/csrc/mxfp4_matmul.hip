@@ -353,98 +353,133 @@ int choose_form(const so_ctx *ctx, uint32_t m, uint32_t C)
     return 0;
 }
 
-constexpr int kVecThreads = 512, kVecWaves = kVecThreads / 64;
-constexpr uint32_t kVecChunk = 8192;         // entries of x in LDS at a time
+constexpr uint32_t kVecChunk = 16384;        // entries of x in LDS at a time
+constexpr uint32_t kVecThreads = 512;
 
-// y = W x + bias with x in fp32: a workgroup takes RT tiles of 32 rows, its waves a unit of 8 blocks each in turn.  A lane multiplies one block of a row with x from LDS, which
-// the rows share, and the block's sum with its scale.
-template <int RT>
+// y = W x + bias with x in fp32: a workgroup takes H halves of a tile, 16 rows each, its waves a unit of 8 blocks each in turn.  A lane multiplies one block of a row with x from LDS, which
+// the rows share, and the block's sum with its scale.  Bound by the vector instructions, a conversion for two products, where few workgroups run (64 x 8192 5.3 us), and by the reading of
+// the codes where many do (16384 x 16384, 143 MB: 31.7 us, 4.5 TB/s).
+template <int H>
 __global__ __launch_bounds__(kVecThreads)
 void mx_matvec_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restrict__ Ws, const float *__restrict__ x, uint32_t m, uint32_t n, uint32_t units, uint32_t tiles,
                       const float *__restrict__ bias, float *__restrict__ y)
 {
-    __shared__ f32x4 xs[kVecChunk / 4];
-    __shared__ float part[kVecWaves][RT * 32];
-    const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x % 64u;
-    const so_u32x4 *wc[RT];
-    const uint32_t *ws[RT];
+    constexpr uint32_t NT = kVecThreads, WAVES = NT / 64, CU = kVecChunk / 256;        // units of a chunk
+    constexpr int S = H > 1 ? H / 2 : 1;                             // words of scales, one for two halves
+    extern __shared__ f32x4 xs[];                                    // a chunk of x, behind it the waves' sums
+    float *part = reinterpret_cast<float *>(xs) + min(units, CU) * 256;      // [WAVES][H * 16]
+    const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x % 64u, odd = H == 1 ? blockIdx.x % 2u : 0u;
+    const so_u32x4 *wc[S];
+    const uint32_t *ws[S];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const size_t t = min(blockIdx.x * RT + i, tiles - 1u);
-        wc[i] = Wc + t * units * 256 + lane;
+    for (int i = 0; i < S; ++i) {
+        const size_t t = min(H == 1 ? blockIdx.x / 2u : blockIdx.x * S + i, tiles - 1u);
+        wc[i] = Wc + t * units * 256 + odd * 64 + lane;
         ws[i] = Ws + t * units * 64 + lane;
     }
-    float acc[RT][2] = {};
-    constexpr uint32_t CU = kVecChunk / 256;                         // units of a chunk
+    struct Unit {
+        so_u32x4 w[H][2];
+        uint32_t s[S];
+    };
+    const auto load = [&](Unit &t, uint32_t u) {
+#pragma unroll
+        for (int i = 0; i < S; ++i) t.s[i] = ws[i][(size_t)u * 64];
+#pragma unroll
+        for (int i = 0; i < H; ++i)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) t.w[i][q] = wc[i / 2][(size_t)u * 256 + q * 128 + i % 2 * 64];
+    };
+    float acc[H] = {};
+    const auto multiply = [&](const Unit &t, uint32_t u) {           // u: of the chunk
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const f32x4 *xp = xs + (u * 8 + 4 * q + lane / 16u) * 8;
+            float sum[H] = {};
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 a = xp[2 * g], b = xp[2 * g + 1];
+#pragma unroll
+                for (int i = 0; i < H; ++i) {
+                    const uint32_t c = t.w[i][q][g];
+                    float &s = sum[i];
+                    const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
+                    const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
+                    s = fmaf(p0[0], a[0], s);
+                    s = fmaf(p0[1], a[1], s);
+                    s = fmaf(p1[0], a[2], s);
+                    s = fmaf(p1[1], a[3], s);
+                    s = fmaf(p2[0], b[0], s);
+                    s = fmaf(p2[1], b[1], s);
+                    s = fmaf(p3[0], b[2], s);
+                    s = fmaf(p3[1], b[3], s);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                const uint32_t s = t.s[i / 2] >> (16 * (i % 2 + odd) + 8 * q) & 255u;
+                acc[i] = fmaf(sum[i], s == 255u ? __builtin_nanf("") : so_mx_power(s), acc[i]);
+            }
+        }
+    };
     for (uint32_t u0 = 0; u0 < units; u0 += CU) {
-        const uint32_t here = min(units - u0, CU);
+        const uint32_t here = min(units - u0, CU), turns = wave < here ? (here - wave + WAVES - 1u) / WAVES : 0u;
+        // two units at a time, the next on its way while one is multiplied, the first ones also while x is; behind the last one that one again
+        const uint32_t last = wave + (turns ? turns - 1u : 0u) * WAVES;
+        Unit a, b;
+        if (turns) {
+            load(a, u0 + wave);
+            load(b, u0 + min(wave + WAVES, last));
+        }
         if (u0) __syncthreads();
-        for (uint32_t k = threadIdx.x; k < here * 256; k += kVecThreads) {
-            const uint64_t at = (uint64_t)u0 * 256 + k;
-            reinterpret_cast<float *>(xs)[k] = at < n ? x[at] : 0.0f;
+        for (uint32_t k0 = threadIdx.x; k0 < here * 256; k0 += 8 * NT) {     // eight requests on their way, what lies behind x as zeros
+            float v[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) v[i] = x[min((uint64_t)u0 * 256 + k0 + i * NT, (uint64_t)n - 1u)];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                if (k0 + i * NT < here * 256) reinterpret_cast<float *>(xs)[k0 + i * NT] = (uint64_t)u0 * 256 + k0 + i * NT < n ? v[i] : 0.0f;
         }
         __syncthreads();
-        for (uint32_t u = wave; u < here; u += kVecWaves) {
-            so_u32x4 w[RT][4];
-            uint32_t sc[RT];
-#pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                sc[i] = ws[i][(size_t)(u0 + u) * 64];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[i][j] = wc[i][(size_t)(u0 + u) * 256 + j * 64];
-            }
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const f32x4 *xp = xs + (u * 8 + 4 * q + lane / 16u) * 8;
-                float sum[RT][2] = {};
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 a = xp[2 * g], b = xp[2 * g + 1];
-#pragma unroll
-                    for (int i = 0; i < RT; ++i)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint32_t c = w[i][2 * q + h][g];
-                            float &s = sum[i][h];
-                            const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
-                            const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
-                            s = fmaf(p0[0], a[0], s);
-                            s = fmaf(p0[1], a[1], s);
-                            s = fmaf(p1[0], a[2], s);
-                            s = fmaf(p1[1], a[3], s);
-                            s = fmaf(p2[0], b[0], s);
-                            s = fmaf(p2[1], b[1], s);
-                            s = fmaf(p3[0], b[2], s);
-                            s = fmaf(p3[1], b[3], s);
-                        }
-                }
-#pragma unroll
-                for (int i = 0; i < RT; ++i)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t s = sc[i] >> (16 * h + 8 * q) & 255u;
-                        acc[i][h] = fmaf(sum[i][h], s == 255u ? __builtin_nanf("") : so_mx_power(s), acc[i][h]);
-                    }
-            }
+        for (uint32_t t = 0; t + 1u < turns; t += 2u) {
+            multiply(a, wave + t * WAVES);
+            load(a, u0 + min(wave + (t + 2u) * WAVES, last));
+            multiply(b, wave + (t + 1u) * WAVES);
+            load(b, u0 + min(wave + (t + 3u) * WAVES, last));
         }
+        if (turns % 2u) multiply(a, last);
     }
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {                                // the four blocks of a row lie 16 lanes apart
-            const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i][h]), __float_as_uint(acc[i][h]), false, false);
-            const float s = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-            const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
-            if (lane < 16u) part[wave][i * 32 + h * 16 + lane] = __uint_as_float(b[0]) + __uint_as_float(b[1]);
-        }
+    for (int i = 0; i < H; ++i) {                                    // the four blocks of a row lie 16 lanes apart
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[i]), __float_as_uint(acc[i]), false, false);
+        const float s = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+        const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+        if (lane < 16u) part[wave * (H * 16) + i * 16 + lane] = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+    }
     __syncthreads();
-    const uint64_t row = (uint64_t)blockIdx.x * (RT * 32) + threadIdx.x;
-    if (threadIdx.x < RT * 32 && row < m) {
-        float s = part[0][threadIdx.x];
+    const uint64_t row = (uint64_t)blockIdx.x * (H * 16) + threadIdx.x;
+    if (threadIdx.x < H * 16 && row < m) {
+        float s[WAVES];
 #pragma unroll
-        for (int w = 1; w < kVecWaves; ++w) s += part[w][threadIdx.x];
-        y[row] = bias ? s + bias[row] : s;
+        for (uint32_t w = 0; w < WAVES; ++w) s[w] = part[w * (H * 16) + threadIdx.x];
+#pragma unroll
+        for (uint32_t step = WAVES / 2; step; step /= 2)
+#pragma unroll
+            for (uint32_t w = 0; w < step; ++w) s[w] += s[w + step];
+        y[row] = bias ? s[0] + bias[row] : s[0];
     }
+}
+
+// 16 rows a workgroup below one tile a compute unit, which leaves fewer of them idle, else 32, which share what is read of x (us, 16 / 32): 1024 x 4096 3.9 / 5.0, 2048 x 8192 6.1 / 7.8,
+// 8192 x 4096 7.7 / 7.5, 8192 x 8192 10.9 / 11.3, 16384 x 8192 19.0 / 16.1, 16384 x 16384 35.6 / 31.7, there with 64 rows 33.4 and with 1024 threads 41.2 / 35.1.
+template <int H>
+so_status launch_matvec(so_ctx *ctx, const so_mxfp4 *W, const float *dx, const float *dBias, float *dy)
+{
+    const uint32_t units = W->blocks / kMxUnit, lds = (std::min(units * 256u, kVecChunk) + kVecThreads / 64 * H * 16) * (uint32_t)sizeof(float);
+    const auto kernel = mx_matvec_kernel<H>;
+    if (lds > 48 * 1024) SO_HIP(so_allow_big_lds(ctx, (const void *)kernel));
+    kernel<<<so_ceil_div(W->m, H * 16), kVecThreads, lds, ctx->stream>>>(W->d_codes, W->d_scales, dx, W->m, W->n, units, W->tiles, dBias, dy);
+    SO_LAUNCH_CHECK();
+    return SO_OK;
 }
 
 } // namespace
@@ -508,11 +543,5 @@ extern "C" so_status so_mxfp4_matvec(so_ctx *ctx, const so_mxfp4 *W, const float
     SO_REQUIRE(dx && dy && dx != dy, "so_mxfp4_matvec: null or aliased vector");
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
-    const uint32_t units = W->blocks / kMxUnit;
-    if (W->tiles >= 2 * (uint32_t)ctx->compute_units)
-        mx_matvec_kernel<2><<<so_ceil_div(W->tiles, 2), kVecThreads, 0, ctx->stream>>>(W->d_codes, W->d_scales, dx, W->m, W->n, units, W->tiles, dBias, dy);
-    else
-        mx_matvec_kernel<1><<<W->tiles, kVecThreads, 0, ctx->stream>>>(W->d_codes, W->d_scales, dx, W->m, W->n, units, W->tiles, dBias, dy);
-    SO_LAUNCH_CHECK();
-    return SO_OK;
+    return W->tiles < (uint32_t)ctx->compute_units ? launch_matvec<1>(ctx, W, dx, dBias, dy) : launch_matvec<2>(ctx, W, dx, dBias, dy);
 }

@@ -114,7 +114,7 @@ def test_gradient(ctx, F, B, type_):
 @pytest.mark.parametrize("lanes", [0, 1, 2, 4, 8])
 @pytest.mark.parametrize("F,B", [(1, 1), (70, 9), (600, 40), (2049, 65), (4000, 130), (8100, 20), (9000, 3), (300, 9001), (1100, 5003)])
 def test_gradient_however_it_is_cut(ctx, F, B, lanes):
-    """Every number of lanes a row of the kernel that holds all features, with one tile or several for a workgroup, and the two kernels that share the features out."""
+    """Every number of lanes a row of the kernel that holds all features for a batch of one tile, and the two kernels that share the features out."""
     for type_ in ("f32", "bf16"):
         rng, X, gamma, _ = problem(F, B, type_, seed=9)
         dY = values(stored(0.1 * rng.standard_normal((F, B)), type_), type_)
