@@ -12,7 +12,8 @@
 // layout, src/sparse_onnx.cpp:17-39).
 //
 // Supported ops (src/sparse_onnx.cpp:176-538): MatMul, Gemm, Conv (group 1), Relu,
-// Sigmoid, Tanh, Add, MaxPool, GlobalAveragePool, Flatten (axis 1), Identity.
+// Sigmoid, Tanh, Add, MaxPool, GlobalAveragePool, Flatten (axis 1), Identity; beyond those LayerNormalization over all
+// axes but the batch.
 // Anything else throws std::runtime_error("Unsupported ONNX op: <op>").
 // An activation that directly follows a MatMul/Gemm/Conv whose result has no other
 // consumer is fused into that kernel's epilogue (the reference fuses Relu only,

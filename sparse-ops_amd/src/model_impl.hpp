@@ -13,7 +13,7 @@
 
 namespace sparseops {
 
-enum class Op { MatMul, Conv, Act, Add, MaxPool, GlobalAveragePool };
+enum class Op { MatMul, Conv, Act, Add, MaxPool, GlobalAveragePool, LayerNorm };
 
 struct LayerPlan {
     Op op = Op::Act;
@@ -34,6 +34,11 @@ struct LayerPlan {
     bool has_bias = false;
     int act = SO_ACT_NONE;      // fused epilogue, or the activation of an Act layer
     bool residual = false;      // Conv: in1 is added to the convolution before the activation
+
+    // LayerNormalization: `bias` (and has_bias) is its B
+    std::vector<float> scale;   // host copy; device copy lives in Impl::bias_pool
+    std::size_t scale_offset = 0;
+    float epsilon = 0.0f;
 
     // pools
     so_pool_geom pg{};
@@ -62,7 +67,7 @@ struct SparseOnnxModel::Impl {
                                    // when the model has convolutions (their LDS-windowed kernel works on such batch tiles)
     bool has_conv = false;
 
-    sparseops::DeviceBuffer bias_pool;   // all biases, contiguous
+    sparseops::DeviceBuffer bias_pool;   // all biases and scales, contiguous
     sparseops::DeviceBuffer arena;       // all activation slots
     sparseops::DeviceBuffer stage_in, stage_out;  // staging for the caller's layouts (batch-major, or unpadded rows)
     sparseops::DeviceBuffer stage_mid;            // [features x batch] between a transpose and the padded arena rows

@@ -57,6 +57,7 @@ void SparseOnnxModel::resize_buffers(uint32_t batch)
         // whatever so_matmul would allocate at this batch is allocated now (run() allocates nothing, and a
         // launch graph cannot be recorded across an allocation)
         else if (L.op == Op::MatMul && L.dE) check(so_matmul_reserve(ctx, L.dE, pbatch), "so_matmul_reserve");
+        else if (L.op == Op::LayerNorm) check(so_layer_norm_reserve(ctx, SO_F32, uint32_t(L.out_features), pbatch), "so_layer_norm_reserve");
     }
     M.set_conv_rbm();
     if (!M.layers.empty() && M.record_pays()) {
@@ -136,6 +137,9 @@ void SparseOnnxModel::Impl::enqueue_layers(const float *in, float *out) const
             break;
         case Op::Add:
             check(so_add(ctx, src(L.in0), src(L.in1), L.out_features * B, dst(L.out)), "so_add");
+            break;
+        case Op::LayerNorm:
+            check(so_layer_norm(ctx, SO_F32, uint32_t(L.out_features), B, src(L.in0), B, bias_pool.f32() + L.scale_offset, bias, L.epsilon, dst(L.out), B, nullptr, nullptr), "so_layer_norm");
             break;
         case Op::MaxPool:
             check(so_maxpool(ctx, &L.pg, src(L.in0), B, dst(L.out)), "so_maxpool");

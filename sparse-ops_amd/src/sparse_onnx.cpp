@@ -292,6 +292,45 @@ SparseOnnxModel::SparseOnnxModel(const std::string &onnx_path) : impl_(new Impl(
             continue;
         }
 
+        if (op == "LayerNormalization") {
+            need_inputs(2);
+            const std::string x = resolve(node.input[0]);
+            const auto &xs = shape_of(x);
+            const std::size_t F = features_of(xs);
+            int64_t axis = -1, stash = 1;
+            if (const auto *a = node.find("axis")) axis = a->i;
+            if (const auto *a = node.find("stash_type")) stash = a->i;
+            if (axis != 1 && axis + int64_t(xs.size()) != 1)
+                throw std::runtime_error("LayerNormalization: only over all axes but the batch is supported");
+            if (stash != 1) throw std::runtime_error("LayerNormalization: stash_type must be 1 (float)");
+            for (std::size_t k = 1; k < node.output.size(); ++k)
+                if (!node.output[k].empty()) throw std::runtime_error("LayerNormalization: Mean and InvStdDev outputs are not supported");
+            const auto parameter = [&](const std::string &nm, const char *what) {
+                auto it = init.find(resolve(nm));
+                if (it == init.end()) throw std::runtime_error(std::string("LayerNormalization: ") + what + " initializer not found");
+                std::vector<float> v = it->second->floats();
+                if (v.size() != F) throw std::runtime_error(std::string("LayerNormalization: ") + what + " length must equal the features");
+                return v;
+            };
+            Pending p;
+            p.plan.op = Op::LayerNorm;
+            p.plan.name = op;
+            p.plan.epsilon = 1e-5f;
+            if (const auto *a = node.find("epsilon")) p.plan.epsilon = a->f;
+            if (!(p.plan.epsilon >= 0.0f)) throw std::runtime_error("LayerNormalization: epsilon is negative or not a number");
+            p.plan.scale = parameter(node.input[1], "Scale");
+            if (node.input.size() > 2 && !node.input[2].empty()) {
+                p.plan.bias = parameter(node.input[2], "B");
+                p.plan.has_bias = true;
+            }
+            p.plan.out_features = F;
+            p.inputs = {x};
+            p.output = out;
+            pend.push_back(std::move(p));
+            M.shape_map[out] = std::vector<int>(xs);
+            continue;
+        }
+
         if (op == "MaxPool" || op == "GlobalAveragePool") {
             need_inputs(1);
             const std::string x = resolve(node.input[0]);
@@ -494,19 +533,24 @@ SparseOnnxModel::SparseOnnxModel(const std::string &onnx_path) : impl_(new Impl(
     bool convs = false;
     for (const auto &p : pend) convs = convs || p.plan.op == Op::Conv;
     const bool fast_fc = !(rbm_env && rbm_env[0] == '0') && !(convs && B0 < 64);
+    const auto place = [&](const std::vector<float> &v) {
+        const std::size_t at = bias_total;
+        bias_total += (v.size() + 63) / 64 * 64;
+        return at;
+    };
     for (auto &p : pend) {
+        if (p.plan.has_bias) p.plan.bias_offset = place(p.plan.bias);
+        if (p.plan.op == Op::LayerNorm) p.plan.scale_offset = place(p.plan.scale);
         if (p.plan.op != Op::MatMul && p.plan.op != Op::Conv) continue;
         p.plan.dE = mirror(*p.plan.E, p.plan.op == Op::MatMul ? matmul_layouts(*p.plan.E, uint32_t(B0), fast_fc) : SO_LAYOUT_ROW);
         if (p.plan.op == Op::Conv) check(so_conv_plan_create(ctx, p.plan.dE, &p.plan.cg, &p.plan.conv), "so_conv_plan_create");
-        if (p.plan.has_bias) {
-            p.plan.bias_offset = bias_total;
-            bias_total += (p.plan.bias.size() + 63) / 64 * 64;
-        }
     }
     if (bias_total) {
         std::vector<float> packed(bias_total, 0.0f);
-        for (const auto &p : pend)
+        for (const auto &p : pend) {
             if (p.plan.has_bias) std::copy(p.plan.bias.begin(), p.plan.bias.end(), packed.begin() + long(p.plan.bias_offset));
+            std::copy(p.plan.scale.begin(), p.plan.scale.end(), packed.begin() + long(p.plan.scale_offset));
+        }
         M.bias_pool.reserve(bias_total * sizeof(float));
         check(so_h2d(ctx, M.bias_pool.get(), packed.data(), bias_total * sizeof(float)), "so_h2d(bias)");
     }
@@ -549,6 +593,8 @@ std::vector<std::string> SparseOnnxModel::describe() const
             if (L.rbm) s += " +rbm";
         } else if (L.op == Op::Act) {
             s += std::string(" act=") + act_name(L.act);
+        } else if (L.op == Op::LayerNorm) {
+            s += std::string(" bias=") + (L.has_bias ? "1" : "0");
         }
         s += " out_features=" + std::to_string(L.out_features);
         out.push_back(s);
