@@ -10,6 +10,7 @@ namespace {
 constexpr int kBlock = 256;
 
 // Row-major to codes and scales.  A lane takes 16 bytes of a row, a block is 8 lanes of fp32 or 4 of a 16-bit type; a block that the row ends in is filled with zeros.
+// Bound by the memory: 8192 x 8192 bf16, 170 MB, 39 us, and 27 us back, together 5.1 TB/s where a copy reaches 5.6; four groups a lane, asked for at once, 42 us, a short division for the row 39.
 template <class T>
 __global__ __launch_bounds__(kBlock)
 void mx_quantize_kernel(const T *__restrict__ X, size_t ldx, uint32_t cols, uint32_t groups, uint64_t total, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales)
@@ -99,6 +100,7 @@ __device__ __forceinline__ uint32_t max_over_rows(uint32_t v)
 
 // X [n x C] into tiles of columns.  A wave takes one block of 32 rows and 8 lanes of columns, 128 bytes a row: a lane 4 rows of 16 bytes, the largest magnitude of a column
 // meets across its 8 lanes.  (One lane a column with its 32 rows, four blocks one after the other, left most of the chip idle: 2777 x 101 fp16 38.5 us.)
+// Bound by the memory and the launch: 8192 x 2048 bf16, 42 MB, 12 us; 14 us with the workgroups of one column after the other.
 template <class T>
 __global__ __launch_bounds__(kBlock)
 void mx_columns_kernel(const T *__restrict__ X, size_t ldx, uint32_t n, uint32_t C, uint32_t units, uint32_t across, so_u32x4 *__restrict__ codes, uint8_t *__restrict__ scales)
@@ -158,7 +160,7 @@ void mx_columns_kernel(const T *__restrict__ X, size_t ldx, uint32_t n, uint32_t
     }
 }
 
-// Rows that lie without a gap and end with a block are one long row.
+// Groups of 16 bytes, of a row (whole blocks) and of all.
 struct Flat { uint64_t groups, total; };
 template <class T>
 Flat flat(uint32_t rows, uint32_t cols)
