@@ -357,8 +357,8 @@ constexpr uint32_t kVecChunk = 16384;        // entries of x in LDS at a time
 constexpr uint32_t kVecThreads = 512;
 
 // y = W x + bias with x in fp32: a workgroup takes H halves of a tile, 16 rows each, its waves a unit of 8 blocks each in turn.  A lane multiplies one block of a row with x from LDS, which
-// the rows share, and the block's sum with its scale.  Bound by the vector instructions, a conversion for two products, where few workgroups run (64 x 8192 5.3 us), and by the reading of
-// the codes where many do (16384 x 16384, 143 MB: 31.7 us, 4.5 TB/s).
+// the rows share, and the block's sum with its scale.  Bound by the vector instructions, a conversion for two products, where few workgroups run (64 x 8192 4.5 us), and by the reading of
+// the codes where many do (16384 x 16384, 143 MB: 29.2 us, 4.9 TB/s).
 template <int H>
 __global__ __launch_bounds__(kVecThreads)
 void mx_matvec_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restrict__ Ws, const float *__restrict__ x, uint32_t m, uint32_t n, uint32_t units, uint32_t tiles,
@@ -431,13 +431,18 @@ void mx_matvec_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restric
             load(b, u0 + min(wave + WAVES, last));
         }
         if (u0) __syncthreads();
-        for (uint32_t k0 = threadIdx.x; k0 < here * 256; k0 += 8 * NT) {     // eight requests on their way, what lies behind x as zeros
-            float v[8];
+        // x in groups of 16 bytes, four of them on their way (one float after the other took 37.5 us for 16384 x 16384, eight at once 31.7), what lies behind x as zeros
+        for (uint32_t k0 = threadIdx.x; k0 < here * 64; k0 += 4 * NT) {
+            f32x4 v[4];
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) v[i] = x[min((uint64_t)u0 * 256 + k0 + i * NT, (uint64_t)n - 1u)];
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint64_t at = (uint64_t)u0 * 256 + (k0 + i * NT) * 4u;
+                v[i] = f32x4{};
+                if (k0 + i * NT < here * 64 && at < n) v[i] = so_group_load(x + at, (uint32_t)min(n - at, (uint64_t)4));
+            }
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i)
-                if (k0 + i * NT < here * 256) reinterpret_cast<float *>(xs)[k0 + i * NT] = (uint64_t)u0 * 256 + k0 + i * NT < n ? v[i] : 0.0f;
+            for (uint32_t i = 0; i < 4; ++i)
+                if (k0 + i * NT < here * 64) xs[k0 + i * NT] = v[i];
         }
         __syncthreads();
         for (uint32_t t = 0; t + 1u < turns; t += 2u) {
@@ -469,7 +474,7 @@ void mx_matvec_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restric
     }
 }
 
-// 16 rows a workgroup below one tile a compute unit, which leaves fewer of them idle, else 32, which share what is read of x (us, 16 / 32): 1024 x 4096 3.9 / 5.0, 2048 x 8192 6.1 / 7.8,
+// 16 rows a workgroup below one tile a compute unit, which leaves fewer of them idle, else 32, which share what is read of x (us, 16 / 32, before x came in groups of 16 bytes): 1024 x 4096 3.9 / 5.0, 2048 x 8192 6.1 / 7.8,
 // 8192 x 4096 7.7 / 7.5, 8192 x 8192 10.9 / 11.3, 16384 x 8192 19.0 / 16.1, 16384 x 16384 35.6 / 31.7, there with 64 rows 33.4 and with 1024 threads 41.2 / 35.1.
 template <int H>
 so_status launch_matvec(so_ctx *ctx, const so_mxfp4 *W, const float *dx, const float *dBias, float *dy)
