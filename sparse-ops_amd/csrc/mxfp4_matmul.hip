@@ -474,8 +474,8 @@ void mx_matvec_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restric
     }
 }
 
-// 16 rows a workgroup below one tile a compute unit, which leaves fewer of them idle, else 32, which share what is read of x (us, 16 / 32, before x came in groups of 16 bytes): 1024 x 4096 3.9 / 5.0, 2048 x 8192 6.1 / 7.8,
-// 8192 x 4096 7.7 / 7.5, 8192 x 8192 10.9 / 11.3, 16384 x 8192 19.0 / 16.1, 16384 x 16384 35.6 / 31.7, there with 64 rows 33.4 and with 1024 threads 41.2 / 35.1.
+// 16 rows a workgroup up to one tile a compute unit, which leaves fewer of them idle, else 32, which share what is read of x (us, 16 / 32): 1024 x 1024 2.9 / 3.2, 1024 x 4096 3.7 / 4.7,
+// 1000 x 16384 7.6 / 10.8, 8192 x 8192 9.3 / 10.0, 12000 x 12000 19.1 / 19.4, 16384 x 8192 17.2 / 14.9, 16384 x 1000 5.3 / 4.4.  (64 rows, or 1024 threads, were faster nowhere by 3%.)
 template <int H>
 so_status launch_matvec(so_ctx *ctx, const so_mxfp4 *W, const float *dx, const float *dBias, float *dy)
 {
@@ -548,5 +548,5 @@ extern "C" so_status so_mxfp4_matvec(so_ctx *ctx, const so_mxfp4 *W, const float
     SO_REQUIRE(dx && dy && dx != dy, "so_mxfp4_matvec: null or aliased vector");
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
-    return W->tiles < (uint32_t)ctx->compute_units ? launch_matvec<1>(ctx, W, dx, dBias, dy) : launch_matvec<2>(ctx, W, dx, dBias, dy);
+    return W->tiles <= (uint32_t)ctx->compute_units ? launch_matvec<1>(ctx, W, dx, dBias, dy) : launch_matvec<2>(ctx, W, dx, dBias, dy);
 }
