@@ -48,6 +48,19 @@ def test_quantize_and_back(ctx, rows, cols, type_):
             a.free()
 
 
+@pytest.mark.parametrize("type_", ["f16", "bf16"])
+@pytest.mark.parametrize("apart", [1, 8, 64, 512, 2048])
+def test_quantize_every_16_bit_pattern(ctx, type_, apart):
+    """Blocks of 32 patterns `apart` from each other: infinities and NaN, subnormal numbers, every mantissa beside a largest one of its own binade and of others."""
+    bits = np.arange(65536, dtype=np.uint16).reshape(-1, 32, apart).transpose(0, 2, 1).reshape(2048, 32)
+    array = np.ascontiguousarray(bits).view(STORAGE[type_])
+    codes, scales = mx.quantize(values(array, type_))
+    dX, dC, dS = ctx.array(array, STORAGE[type_]), ctx.empty((2048, 1, 16), np.uint8), ctx.empty((2048, 1), np.uint8)
+    ctx.mxfp4_quantize(dX, 2048, 32, dC, dS, type=type_)
+    assert np.array_equal(dS.download(), scales)
+    assert np.array_equal(dC.download(), codes)
+
+
 def test_every_code_and_scale_and_blocks_that_are_not_numbers(ctx):
     codes = np.tile((np.arange(256, dtype=np.uint8)).reshape(1, 16, 16), (256, 1, 1))
     scales = np.repeat(np.arange(256, dtype=np.uint8)[:, None], 16, axis=1)
