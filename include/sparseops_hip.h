@@ -384,7 +384,7 @@ so_status so_mxfp4_dequantize(so_ctx *ctx, const uint8_t *dCodes, const uint8_t 
                               int type, void *dY, size_t y_stride);
 
 /* A matrix W [m x n] for products, laid out for the matrix cores from row-major codes and scales in device memory, which
- * are free for reuse once the stream has passed the call.  Takes 17 bytes for 32 entries, n rounded up to 256. */
+ * are free for reuse on return.  Takes 17 bytes for 32 entries, m rounded up to 32 and n to 256. */
 typedef struct so_mxfp4 so_mxfp4;
 so_status so_mxfp4_create(so_ctx *ctx, const uint8_t *dCodes, const uint8_t *dScales, uint32_t m, uint32_t n, so_mxfp4 **out);
 so_status so_mxfp4_free(so_ctx *ctx, so_mxfp4 *W);

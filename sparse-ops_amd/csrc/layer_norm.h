@@ -214,7 +214,8 @@ void for_lanes(uint32_t lanes, F &&f)
     else f(std::integral_constant<int, 8>());
 }
 
-static inline bool ranges_fit(const Cut &c, uint32_t F) { return c.groups + so_ceil_div(F, 16) < (1ull << 31); }
+// (The kernel that holds all features has no more threads: it takes 512 only where a tile has several parts.)
+static inline bool ranges_fit(const Cut &c, uint32_t joiners = 0) { return so_grid_fits(c.groups + joiners + 64, kThreads); }
 
 static inline so_status workspace(so_ctx *ctx, const char *who, size_t bytes)
 {

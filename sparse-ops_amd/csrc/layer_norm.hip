@@ -277,7 +277,7 @@ extern "C" so_status so_layer_norm_reserve(so_ctx *ctx, int type, uint32_t F, ui
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
     const Cut c = cut_of(type, F, B);
-    SO_REQUIRE(ranges_fit(c, F), "so_layer_norm_reserve: %u x %u is too large for one launch", F, B);
+    SO_REQUIRE(ranges_fit(c), "so_layer_norm_reserve: %u x %u is too large for one launch", F, B);
     return workspace(ctx, "so_layer_norm_reserve", std::max(c.cols_bytes, so_norm_grad_bytes(ctx, type, F, B)));
 }
 
@@ -295,7 +295,7 @@ extern "C" so_status so_layer_norm(so_ctx *ctx, int type, uint32_t F, uint32_t B
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
     const Cut c = cut_of(type, F, B);
-    SO_REQUIRE(ranges_fit(c, F), "so_layer_norm: %u x %u is too large for one launch", F, B);
+    SO_REQUIRE(ranges_fit(c), "so_layer_norm: %u x %u is too large for one launch", F, B);
     if (const Whole w = whole_of(ctx, type, F, B); w.lanes) {
         const uint32_t tiles = so_ceil_div(B, w.lanes * (16u / (uint32_t)so_type_bytes(type))), per_xcd = so_ceil_div(tiles, 8);
         hipError_t allowed = hipSuccess;

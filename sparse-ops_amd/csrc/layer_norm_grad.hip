@@ -274,7 +274,7 @@ extern "C" so_status so_layer_norm_grad(so_ctx *ctx, int type, uint32_t F, uint3
     const bool params = dDgamma || dDbeta;
     if (!dDx && !params) return SO_OK;
     const Cut c = cut_of(type, F, B);
-    SO_REQUIRE(ranges_fit(c, F), "so_layer_norm_grad: %u x %u is too large for one launch", F, B);
+    SO_REQUIRE(ranges_fit(c, so_ceil_div(F, 16)), "so_layer_norm_grad: %u x %u is too large for one launch", F, B);
     if (const One w = one_of(ctx, type, F, B); w.lanes) {
         so_for_type(type, [&](auto t) {
             using T = decltype(t);

@@ -19,6 +19,7 @@ struct so_mxfp4 {
     uint32_t m = 0, n = 0;
     uint32_t blocks = 0;                // of a row as stored, a multiple of kMxUnit
     uint32_t tiles = 0;
+    int device = 0;
     void *d_blob = nullptr;             // one allocation for the two
     so_u32x4 *d_codes = nullptr;        // [tiles][units][4][64]
     uint32_t *d_scales = nullptr;       // [tiles][units][64]
@@ -57,5 +58,5 @@ __device__ __forceinline__ uint32_t so_mx_codes(const float (&v)[8], float scale
     return w;
 }
 
-// csrc/mxfp4.hip: X [n x C] quantised in blocks of 32 of its rows, into tiles of 32 columns as above.
+// csrc/mxfp4.hip: X [n x C] quantised in blocks of 32 of its rows, into tiles of 32 columns as above.  Without `codes` only whether it is small enough for a launch.
 so_status so_mx_quantize_columns(so_ctx *ctx, int type, const void *dX, size_t x_stride, uint32_t n, uint32_t C, so_u32x4 *codes, uint32_t *scales);

@@ -233,14 +233,17 @@ extern "C" so_status so_mxfp4_create(so_ctx *ctx, const uint8_t *dCodes, const u
     W->blocks = so_mx_blocks(n);
     W->tiles = so_ceil_div(m, kMxTile);
     const uint64_t total = (uint64_t)W->tiles * W->blocks * kMxTile;                 // threads, and 16 bytes of codes each
-    SO_REQUIRE(total / kBlock < (1ull << 31), "so_mxfp4_create: %u x %u is too large for one launch", m, n);
+    SO_REQUIRE(so_grid_fits(total / kBlock, kBlock), "so_mxfp4_create: %u x %u is too large for one launch", m, n);
+    W->device = ctx->device;
     SO_HIP(hipMalloc(&W->d_blob, total * 17));
     W->d_codes = (so_u32x4 *)W->d_blob;
     W->d_scales = (uint32_t *)(W->d_codes + total);
     mx_tile_kernel<<<so_ceil_div(total, kBlock), kBlock, 0, ctx->stream>>>((const so_u32x4 *)dCodes, dScales, m, so_ceil_div(n, 32), W->blocks / kMxUnit, total, W->d_codes, (uint8_t *)W->d_scales);
-    if (const hipError_t e = hipGetLastError(); e != hipSuccess) {
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);                      // from here on other contexts may use it
+    if (e != hipSuccess) {
         (void)hipFree(W->d_blob);
-        so_set_error("kernel launch failed: %s (so_mxfp4_create)", hipGetErrorString(e));
+        so_set_error("so_mxfp4_create: %s", hipGetErrorString(e));
         return SO_ERR_HIP;
     }
     *out = W.release();
@@ -250,6 +253,7 @@ extern "C" so_status so_mxfp4_create(so_ctx *ctx, const uint8_t *dCodes, const u
 extern "C" so_status so_mxfp4_free(so_ctx *ctx, so_mxfp4 *W)
 {
     if (!W) return SO_OK;
+    SO_REQUIRE(!ctx || !ctx->capturing, "so_mxfp4_free: not allowed while a graph is being recorded");
     if (ctx && ctx->stream) (void)hipStreamSynchronize(ctx->stream);
     (void)hipFree(W->d_blob);
     delete W;
@@ -266,18 +270,18 @@ extern "C" so_status so_mxfp4_dims(const so_mxfp4 *W, uint32_t *m, uint32_t *n)
 
 so_status so_mx_quantize_columns(so_ctx *ctx, int type, const void *dX, size_t x_stride, uint32_t n, uint32_t C, so_u32x4 *codes, uint32_t *scales)
 {
-    const uint32_t blocks = so_mx_blocks(n), quads = blocks / 4;
+    const uint32_t blocks = so_mx_blocks(n);
     so_status status = SO_OK;
     so_for_type(type, [&](auto t) {
         using T = decltype(t);
         const uint32_t across = so_ceil_div(C, 8 * so_elements<T>::V);
-        const uint64_t groups = (uint64_t)across * quads;
-        if (groups >= (1ull << 31)) {
+        const uint64_t groups = (uint64_t)across * (blocks / 4);
+        if (!so_grid_fits(groups, kBlock)) {
             so_set_error("so_mxfp4_matmul: %u x %u input is too large for one launch", n, C);
             status = SO_ERR_INVALID;
-            return;
+        } else if (codes) {
+            mx_columns_kernel<T><<<(uint32_t)groups, kBlock, 0, ctx->stream>>>((const T *)dX, x_stride, n, C, blocks / kMxUnit, across, codes, (uint8_t *)scales);
         }
-        mx_columns_kernel<T><<<(uint32_t)groups, kBlock, 0, ctx->stream>>>((const T *)dX, x_stride, n, C, blocks / kMxUnit, across, codes, (uint8_t *)scales);
     });
     if (status != SO_OK) return status;
     SO_LAUNCH_CHECK();

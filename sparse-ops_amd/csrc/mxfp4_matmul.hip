@@ -291,20 +291,16 @@ so_status reserve(so_ctx *ctx, const char *who, const so_mxfp4 *W, uint32_t C)
 }
 
 struct Groups { uint32_t m, c, per_xcd; };
-so_status groups_of(const so_mxfp4 *W, uint32_t C, uint32_t rows, uint32_t cols, Groups *g)
+Groups groups_of(const so_mxfp4 *W, uint32_t C, uint32_t rows, uint32_t cols)
 {
-    g->m = so_ceil_div(W->m, rows);
-    g->c = so_ceil_div(C, cols);
-    SO_REQUIRE((uint64_t)g->m * g->c < (1ull << 30), "so_mxfp4_matmul: %u x %u output is too large for one launch", W->m, C);
-    g->per_xcd = so_ceil_div((uint64_t)g->m * g->c, 8);
-    return SO_OK;
+    const uint32_t m = so_ceil_div(W->m, rows), c = so_ceil_div(C, cols);
+    return {m, c, so_ceil_div((uint64_t)m * c, 8)};
 }
 
 template <class T, int MH, int CH, int WK, int ACT>
 so_status launch(so_ctx *ctx, const so_mxfp4 *W, const so_u32x4 *codes, const uint32_t *scales, uint32_t C, const float *bias, T *Y, size_t ldy)
 {
-    Groups g;
-    if (const so_status s = groups_of(W, C, MH * 16, CH * 16, &g); s != SO_OK) return s;
+    const Groups g = groups_of(W, C, MH * 16, CH * 16);
     constexpr uint32_t bytes = WK * MH * 16 * (CH * 16 + 4) * sizeof(float);
     const auto kernel = mx_matmul_kernel<T, MH, CH, WK, ACT>;
     if (bytes > 48 * 1024) SO_HIP(so_allow_big_lds(ctx, (const void *)kernel));
@@ -317,8 +313,7 @@ so_status launch(so_ctx *ctx, const so_mxfp4 *W, const so_u32x4 *codes, const ui
 template <class T, int MH, int CH, int WM, int WC, int ACT>
 so_status launch_staged(so_ctx *ctx, const so_mxfp4 *W, const so_u32x4 *codes, const uint32_t *scales, uint32_t C, const float *bias, T *Y, size_t ldy)
 {
-    Groups g;
-    if (const so_status s = groups_of(W, C, MH * WM * 16, CH * WC * 16, &g); s != SO_OK) return s;
+    const Groups g = groups_of(W, C, MH * WM * 16, CH * WC * 16);
     constexpr uint32_t bytes = std::max<uint32_t>(4 * (MH * WM + CH * WC) / 2 * (2048 + 256), WM * WC * 32 * (CH * 16 + 4) * sizeof(float));
     const auto kernel = mx_matmul_staged_kernel<T, MH, CH, WM, WC, ACT>;
     SO_HIP(so_allow_big_lds(ctx, (const void *)kernel));
@@ -338,18 +333,20 @@ constexpr int kFormCount = 8;
 // and C of 1 .. 2048 (fp32, with the quantisation; us), this form / the next smaller: 8192 x 8192 x 2048 256 x 256 76.3 / 96.3, 4096 x 8192 x 1024 128 x 128 38.0 / 39.7, 4096 x 8192 x 512
 // 64 x 64 on four waves 23.5 / 27.9 on eight, 4096 x 8192 x 256 64 x 64 16.3 / 18.7, 2048 x 8192 x 256 64 x 32 13.2 / 14.1, 1024 x 8192 x 256 32 x 32 9.9 / 12.4, 2048 x 8192 x 64 32 x 16
 // 8.2 / 9.0; with half as many workgroups as compute units the larger loses by as much (4096 x 8192 x 2048: 256 x 256 61.5, 128 x 128 56.3).
+// None half of whose columns would do: 32768 x 4096 x 8 32 x 16 15.4, 64 x 64 on four waves 17.2, 128 x 128 20.0; 65536 x 4096 x 32 32 x 32 27.0, 128 x 128 29.9.
 int choose_form(const so_ctx *ctx, uint32_t m, uint32_t C)
 {
     const uint64_t cus = (uint64_t)ctx->compute_units;
     const auto tiles = [&](int f) { return (uint64_t)so_ceil_div(m, kForms[f].rows) * so_ceil_div(C, kForms[f].cols); };
     const auto rounds = [](uint64_t tiles, uint64_t at_once) { return (tiles + at_once - 1) / at_once; };
-    if (tiles(6) >= cus) {
+    const auto wide = [&](int f) { return C <= kForms[f].cols / 2; };
+    if (tiles(6) >= cus && !wide(6)) {
         // one tile of 256 x 256 a compute unit at a time takes 0.78 of what its four quarters take, two of those at a time
-        return 4.0 * (double)rounds(tiles(7), cus) <= 1.28 * 2.0 * (double)rounds(tiles(6), 2 * cus) ? 7 : 6;
+        return !wide(7) && 4.0 * (double)rounds(tiles(7), cus) <= 1.28 * 2.0 * (double)rounds(tiles(6), 2 * cus) ? 7 : 6;
     }
-    if (tiles(5) >= 2 * cus) return 5;
+    if (tiles(5) >= 2 * cus && !wide(5)) return 5;
     for (int f = 4; f > 0; --f)
-        if (tiles(f) >= cus) return f;
+        if (tiles(f) >= cus && !wide(f)) return f;
     return 0;
 }
 
@@ -494,6 +491,7 @@ extern "C" so_status so_mxfp4_matmul_reserve(so_ctx *ctx, const so_mxfp4 *W, uin
     SO_REQUIRE(ctx != nullptr && W != nullptr, "so_mxfp4_matmul_reserve: null handle");
     SO_REQUIRE(!ctx->capturing, "so_mxfp4_matmul_reserve: a graph is being recorded");
     if (C == 0) return SO_OK;
+    SO_REQUIRE(W->device == ctx->device, "so_mxfp4_matmul_reserve: the matrix lies on another device");
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
     return reserve(ctx, "so_mxfp4_matmul_reserve", W, C);
@@ -507,14 +505,16 @@ extern "C" so_status so_mxfp4_matmul(so_ctx *ctx, const so_mxfp4 *W, int type, c
     if (C == 0) return SO_OK;
     SO_REQUIRE(dX && dY && dX != dY, "so_mxfp4_matmul: null or aliased tensor");
     SO_REQUIRE(x_stride >= C && y_stride >= C, "so_mxfp4_matmul: a stride is shorter than a row");
-    SO_REQUIRE((uint64_t)W->blocks * C < (1ull << 38), "so_mxfp4_matmul: %u x %u input is too large for one launch", W->n, C);
+    SO_REQUIRE(W->device == ctx->device, "so_mxfp4_matmul: the matrix lies on another device");
+    const Form &form = kForms[ctx->tune.mxfp4_form >= 1 && ctx->tune.mxfp4_form <= kFormCount ? ctx->tune.mxfp4_form - 1 : choose_form(ctx, W->m, C)];
+    SO_REQUIRE(so_grid_fits((uint64_t)so_ceil_div(W->m, form.rows) * so_ceil_div(C, form.cols) + 8, 512), "so_mxfp4_matmul: %u x %u output is too large for one launch", W->m, C);
+    if (const so_status s = so_mx_quantize_columns(ctx, type, dX, x_stride, W->n, C, nullptr, nullptr); s != SO_OK) return s;      // whether it can be done
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
     if (const so_status s = reserve(ctx, "so_mxfp4_matmul", W, C); s != SO_OK) return s;
     so_u32x4 *codes = (so_u32x4 *)ctx->mm_part->p;
     uint32_t *scales = (uint32_t *)((char *)codes + workspace_of(W, C).codes);
     if (const so_status s = so_mx_quantize_columns(ctx, type, dX, x_stride, W->n, C, codes, scales); s != SO_OK) return s;
-    const Form &form = kForms[ctx->tune.mxfp4_form >= 1 && ctx->tune.mxfp4_form <= kFormCount ? ctx->tune.mxfp4_form - 1 : choose_form(ctx, W->m, C)];
     ctx->last_kernel = form.name;
     so_status status = SO_OK;
     so_for_type(type, [&](auto t) {
@@ -546,6 +546,8 @@ extern "C" so_status so_mxfp4_matvec(so_ctx *ctx, const so_mxfp4 *W, const float
 {
     SO_REQUIRE(ctx != nullptr && W != nullptr, "so_mxfp4_matvec: null handle");
     SO_REQUIRE(dx && dy && dx != dy, "so_mxfp4_matvec: null or aliased vector");
+    SO_REQUIRE(W->device == ctx->device, "so_mxfp4_matvec: the matrix lies on another device");
+    SO_REQUIRE(so_grid_fits(W->tiles, kVecThreads), "so_mxfp4_matvec: %u rows are too many for one launch", W->m);
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
     return W->tiles <= (uint32_t)ctx->compute_units ? launch_matvec<1>(ctx, W, dx, dBias, dy) : launch_matvec<2>(ctx, W, dx, dBias, dy);

@@ -352,6 +352,9 @@ hipError_t so_allow_big_lds(so_ctx *ctx, const void *kernel);
 
 static inline uint32_t so_ceil_div(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
+// A launch has fewer than 2^32 threads.
+static inline bool so_grid_fits(uint64_t groups, uint32_t threads) { return groups < (1ull << 32) / threads; }
+
 // Epilogue shared by the matmul and conv kernels.  expf/tanhf are the accurate
 // OCML routines (no fast-math), matching 1.0f/(1.0f+expf(-v)) and tanhf(v).
 template <int ACT>

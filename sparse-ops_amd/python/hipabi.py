@@ -217,7 +217,7 @@ class DeviceMxfp4:
 
     def free(self):
         if self.h:
-            self.ctx.lib.so_mxfp4_free(self.ctx.h, self.h)
+            self.ctx._ck(self.ctx.lib.so_mxfp4_free(self.ctx.h, self.h))
             self.h = None
 
 

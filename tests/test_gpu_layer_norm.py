@@ -228,6 +228,9 @@ def test_no_columns_and_refusals(ctx):
     refused("one stride", lambda: ctx.layer_norm(dX, F, B - 1, None, None, EPS, dX, y_stride=B))
     refused("eps", lambda: ctx.layer_norm(dX, F, B, None, None, -1.0, dY))
     refused("eps", lambda: ctx.layer_norm(dX, F, B, None, None, float("nan"), dY))
+    refused("too large for one launch", lambda: ctx.layer_norm(dX, 1, 0xffffffff, None, None, EPS, dY))
+    refused("too large for one launch", lambda: ctx.layer_norm_grad(dX, dY, 0x7fffffff, 100, None, st, st, dX, None, None))
+    refused("too large for one launch", lambda: ctx.layer_norm_reserve(1, 0xffffffff))
     refused("no features", lambda: ctx.layer_norm_grad(dX, dY, 0, B, None, st, st, dX, None, None))
     refused("null tensor", lambda: ctx.layer_norm_grad(dX, None, F, B, None, st, st, dX, None, None))
     refused("null tensor", lambda: ctx.layer_norm_grad(dX, dY, F, B, None, None, st, dX, None, None))

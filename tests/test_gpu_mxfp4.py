@@ -254,12 +254,20 @@ def test_empty_calls_and_refusals(ctx):
     refused("null or aliased", lambda: ctx.mxfp4_matmul(W, None, 4, None, a))
     refused("null or aliased", lambda: ctx.mxfp4_matmul(W, a, 4, None, a))
     refused("stride", lambda: ctx.mxfp4_matmul(W, a, 4, None, ctx.empty((64, 4)), x_stride=3))
+    refused("too large for one launch", lambda: ctx.mxfp4(b, c, 0xffffffe0, 1 << 20))
+    refused("too large for one launch", lambda: ctx.mxfp4_matmul(W, a, 0xffffffff, None, ctx.empty((64, 4))))
     refused("null or aliased", lambda: ctx.mxfp4_matvec(W, None, None, a))
     lib = ctx.lib
     assert lib.so_mxfp4_quantize(ctx.h, 7, a.ptr, 64, 64, 64, b.ptr, c.ptr) == hipabi.SO_ERR_INVALID
     assert lib.so_mxfp4_dequantize(ctx.h, b.ptr, c.ptr, 64, 64, 3, a.ptr, 64) == hipabi.SO_ERR_INVALID
     assert lib.so_mxfp4_matmul(ctx.h, W.h, 9, a.ptr, 64, 4, None, b.ptr, 64, 0) == hipabi.SO_ERR_INVALID
     assert lib.so_mxfp4_matmul(ctx.h, W.h, 0, a.ptr, 64, 4, None, b.ptr, 64, 4) == hipabi.SO_ERR_INVALID
+    ctx.graph_begin()
+    try:
+        refused("recorded", W.free)
+        refused("recorded", lambda: ctx.mxfp4(b, c, 64, 64))
+    finally:
+        ctx.graph_free(ctx.graph_end())
     W.free()
 
 
