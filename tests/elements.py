@@ -40,3 +40,20 @@ def fetch(whole, rows, cols, type_, pad=0, shift=0):
     flat = values(whole.download(), type_)
     body = flat[shift:].reshape(rows, cols + pad)
     return body[:, :cols], np.concatenate([flat[:shift], body[:, cols:].ravel()])
+
+
+def place_apart(ctx, matrix, type_, stride):
+    """A device array whose rows lie `stride` elements apart, nothing written between them."""
+    rows, cols = matrix.shape
+    whole = ctx.empty(((rows - 1) * stride + cols,), STORAGE[type_])
+    for r in range(rows):
+        line = np.ascontiguousarray(stored(matrix[r], type_))
+        ctx._ck(ctx.lib.so_h2d(ctx.h, whole.offset(r * stride).ptr, line.ctypes.data, line.nbytes))
+    return whole
+
+
+def fetch_apart(ctx, whole, rows, cols, type_, stride):
+    out = np.empty((rows, cols), STORAGE[type_])
+    for r in range(rows):
+        ctx._ck(ctx.lib.so_d2h(ctx.h, out[r].ctypes.data, whole.offset(r * stride).ptr, out[r].nbytes))
+    return values(out, type_)

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import hipabi
-from elements import HALF_STEP, SMALLEST, TYPES, U, fetch, place, stored, values
+from elements import HALF_STEP, SMALLEST, TYPES, U, fetch, fetch_apart, place, place_apart, stored, values
 
 pytestmark = pytest.mark.gpu
 
@@ -205,6 +205,29 @@ def test_columns_far_from_zero_constant_and_not_finite(ctx):
     check_forward(Y[:, rest], X[:, rest], gamma, beta, "f32")
     check_statistics(dM.download()[rest], rstd[rest], X[:, rest])
     assert np.array_equal(Y[:, 6], beta.astype(np.float64)) and np.array_equal(Y[:, 7], beta.astype(np.float64))
+
+
+@pytest.mark.parametrize("lanes", [-1, 0])
+def test_offsets_beyond_32_bits(ctx, lanes):
+    """Rows 2^30 + 5 elements apart: the last ones begin beyond 2^32 elements."""
+    F, B, apart = 6, 70, 2 ** 30 + 5
+    _, X, gamma, beta = problem(F, B, "f16", seed=4)
+    dX, dY, dM, dR = place_apart(ctx, X, "f16", apart), ctx.empty(((F - 1) * apart + B,), np.float16), ctx.empty((B,)), ctx.empty((B,))
+    dG, dB, dg, db = ctx.array(gamma), ctx.array(beta), ctx.empty((F,)), ctx.empty((F,))
+    with ctx.tuning(SPARSEOPS_NORM_LANES=lanes):
+        ctx.layer_norm(dX, F, B, dG, dB, EPS, dY, dM, dR, type="f16", x_stride=apart, y_stride=apart)
+        check_forward(fetch_apart(ctx, dY, F, B, "f16", apart), X, gamma, beta, "f16")
+        # the gradient of the sum of all results: none for X, the normalised rows' sums for gamma, B for beta
+        ones = place_apart(ctx, np.ones((F, B)), "f16", apart)
+        ctx.layer_norm_grad(dX, ones, F, B, None, dM, dR, dY, dg, db, type="f16", x_stride=apart, dy_stride=apart, dx_stride=apart)
+    mean, rstd = statistics(X)
+    h = (X - mean) * rstd
+    bound = U * 64 * (np.abs(X).max(axis=0) * rstd)                    # of h; g and its mean are exact here
+    assert np.all(np.abs(fetch_apart(ctx, dY, F, B, "f16", apart)) <= rstd * (1 + np.abs(h)) * bound + SMALLEST["f16"])
+    assert np.all(np.abs(dg.download() - h.sum(axis=1)) <= bound.sum() + U * 16 * np.abs(h).sum(axis=1))
+    assert np.array_equal(db.download(), np.full(F, B, np.float32))
+    for a in (dX, dY, ones):
+        a.free()
 
 
 def test_no_columns_and_refusals(ctx):

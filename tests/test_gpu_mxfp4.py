@@ -4,7 +4,7 @@ import pytest
 
 import hipabi
 import mx_reference as mx
-from elements import HALF_STEP, SMALLEST, STORAGE, TYPES, U, fetch, place, stored, values
+from elements import HALF_STEP, SMALLEST, STORAGE, TYPES, U, fetch, fetch_apart, place, place_apart, stored, values
 
 pytestmark = pytest.mark.gpu
 
@@ -54,7 +54,8 @@ def test_quantize_every_16_bit_pattern(ctx, type_, apart):
     """Blocks of 32 patterns `apart` from each other: infinities and NaN, subnormal numbers, every mantissa beside a largest one of its own binade and of others."""
     bits = np.arange(65536, dtype=np.uint16).reshape(-1, 32, apart).transpose(0, 2, 1).reshape(2048, 32)
     array = np.ascontiguousarray(bits).view(STORAGE[type_])
-    codes, scales = mx.quantize(values(array, type_))
+    with np.errstate(invalid="ignore"):
+        codes, scales = mx.quantize(values(array, type_))
     dX, dC, dS = ctx.array(array, STORAGE[type_]), ctx.empty((2048, 1, 16), np.uint8), ctx.empty((2048, 1), np.uint8)
     ctx.mxfp4_quantize(dX, 2048, 32, dC, dS, type=type_)
     assert np.array_equal(dS.download(), scales)
@@ -223,6 +224,27 @@ def test_the_same_bits_every_time_and_across_states(ctx):
     assert np.array_equal(dY.download().view(np.uint32), dZ.download().view(np.uint32))
     first.free()
     second.free()
+
+
+def test_offsets_beyond_32_bits(ctx):
+    """Rows 2^30 + 5 elements apart, the last ones beyond 2^32 elements: quantisation, its way back, the input and the output of a product."""
+    rng = np.random.default_rng(15)
+    rows, cols, apart = 6, 70, 2 ** 30 + 5
+    X = values(stored(rng.standard_normal((rows, cols)), "f16"), "f16")
+    dX, dY = place_apart(ctx, X, "f16", apart), ctx.empty(((rows - 1) * apart + cols,), np.float16)
+    codes, scales = mx.quantize(X)
+    dC, dS = ctx.empty(codes.shape, np.uint8), ctx.empty(scales.shape, np.uint8)
+    ctx.mxfp4_quantize(dX, rows, cols, dC, dS, type="f16", x_stride=apart)
+    assert np.array_equal(dC.download(), codes) and np.array_equal(dS.download(), scales)
+    ctx.mxfp4_dequantize(dC, dS, rows, cols, dY, type="f16", y_stride=apart)
+    assert np.array_equal(fetch_apart(ctx, dY, rows, cols, "f16", apart), mx.dequantize(codes, scales, cols))
+    handle, W = weights(ctx, rng, rows, rows)
+    ctx.mxfp4_matmul(handle, dX, cols, None, dY, type="f16", x_stride=apart, y_stride=apart)
+    Xq = mx.dequantize(*mx.quantize(np.ascontiguousarray(X.T)), rows).T
+    want = W @ Xq
+    assert np.all(np.abs(fetch_apart(ctx, dY, rows, cols, "f16", apart) - want) <= product_tolerance(W, Xq, None, want, "none", "f16"))
+    for a in (handle, dX, dY):
+        a.free()
 
 
 def test_empty_calls_and_refusals(ctx):
