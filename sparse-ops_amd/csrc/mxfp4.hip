@@ -112,10 +112,11 @@ void mx_columns_kernel(const T *__restrict__ X, size_t ldx, uint32_t n, uint32_t
     const uint64_t c = ((uint64_t)group * 8u + lane % 8u) * V, k0 = (uint64_t)b * 32u + r * 4u;
     const uint32_t left = c >= C ? 0u : (uint32_t)min((uint64_t)V, C - c);
     const T *p = X + k0 * ldx + c;
+    const uint32_t wide = so_group_wide_rows<T>(left, n, ldx);     // what stands behind a row's end goes into columns that are not stored
     typename so_elements<T>::plain x[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (k0 + i < n && left) x[i] = so_group_load(p + (size_t)i * ldx, left);
+        if (k0 + i < n && left) x[i] = so_group_load(p + (size_t)i * ldx, left, k0 + i < wide);
         else x[i] = typename so_elements<T>::plain{};
     float f[4][V];
     uint32_t top[V] = {};
