@@ -47,7 +47,7 @@ void mx_matmul_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restric
 {
     constexpr int V = so_elements<T>::V, PITCH = CH * 16 + 4, MW = (MH + 1) / 2, CW = (CH + 1) / 2;
     static_assert((MH == 1 || MH % 2 == 0) && (CH == 1 || CH % 2 == 0), "half a tile of 32, or whole ones");
-    extern __shared__ float lds[];                                   // [WK][MH * 16][PITCH]
+    extern __shared__ f32x4 sums[];                                  // [WK][MH * 16][PITCH / 4]
     const MxTile tile = mx_tile_of(mgroups, cgroups, per_xcd);
     if (tile.none) return;
     const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x % 64u;
@@ -109,11 +109,11 @@ void mx_matmul_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restric
         }
         if (turns % 2u) multiply(a);
     }
-    float *mine = lds + (size_t)wave * MH * 16 * PITCH;
+    f32x4 *mine = sums + wave * MH * 16 * (PITCH / 4);
 #pragma unroll
     for (int i = 0; i < MH; ++i)
 #pragma unroll
-        for (int k = 0; k < CH; ++k) *reinterpret_cast<f32x4 *>(mine + (i * 16 + lane % 16u) * PITCH + k * 16 + 4 * (lane / 16u)) = acc[i][k];
+        for (int k = 0; k < CH; ++k) mine[(i * 16 + lane % 16u) * (PITCH / 4) + k * 4 + lane / 16u] = acc[i][k];
     __syncthreads();
     constexpr int GR = CH * 16 / V;                                  // groups of 16 bytes in a row of the tile
     for (uint32_t g = threadIdx.x; g < MH * 16 * GR; g += 64 * WK) {
@@ -124,9 +124,9 @@ void mx_matmul_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restric
         float y[V];
 #pragma unroll
         for (int e = 0; e < V; e += 4) {
-            f32x4 s = *reinterpret_cast<const f32x4 *>(lds + r * PITCH + c + e);
+            f32x4 s = sums[r * (PITCH / 4) + (c + e) / 4];
 #pragma unroll
-            for (int w = 1; w < WK; ++w) s += *reinterpret_cast<const f32x4 *>(lds + ((size_t)w * MH * 16 + r) * PITCH + c + e);
+            for (int w = 1; w < WK; ++w) s += sums[(w * MH * 16 + r) * (PITCH / 4) + (c + e) / 4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[e + i] = so_epilogue<ACT>(s[i] + add);
         }
@@ -330,9 +330,9 @@ constexpr Form kForms[] = {{16, 16, "mx-16x16"}, {32, 16, "mx-32x16"}, {32, 32, 
 constexpr int kFormCount = 8;
 
 // The largest tile that gives every compute unit a workgroup: a larger one asks the caches for less, a smaller one leaves none idle.  From a sweep over m of 64 .. 8192, n of 512 .. 8192
-// and C of 1 .. 2048 (fp32, with the quantisation; us), this form / the next smaller: 8192 x 8192 x 2048 256 x 256 76.3 / 96.3, 4096 x 8192 x 1024 128 x 128 38.0 / 39.7, 4096 x 8192 x 512
-// 64 x 64 on four waves 23.5 / 27.9 on eight, 4096 x 8192 x 256 64 x 64 16.3 / 18.7, 2048 x 8192 x 256 64 x 32 13.2 / 14.1, 1024 x 8192 x 256 32 x 32 9.9 / 12.4, 2048 x 8192 x 64 32 x 16
-// 8.2 / 9.0; with half as many workgroups as compute units the larger loses by as much (4096 x 8192 x 2048: 256 x 256 61.5, 128 x 128 56.3).
+// and C of 1 .. 2048 (fp32, with the quantisation; us), this form / the next smaller: 8192 x 8192 x 2048 256 x 256 76.3 / 96.3, 4096 x 8192 x 1024 128 x 128 36.9 / 37.6, 4096 x 8192 x 512
+// 64 x 64 on four waves 22.4 / 25.3 on eight, 4096 x 8192 x 256 64 x 64 15.0 / 19.1, 2048 x 8192 x 256 64 x 32 11.6 / 12.6, 1024 x 8192 x 256 32 x 32 9.3 / 10.6, 2048 x 8192 x 64 32 x 16
+// 8.0 / 8.7; with half as many workgroups as compute units the larger loses by as much (4096 x 8192 x 2048: 256 x 256 61.5, 128 x 128 56.3).
 // None half of whose columns would do: 32768 x 4096 x 8 32 x 16 15.4, 64 x 64 on four waves 17.2, 128 x 128 20.0; 65536 x 4096 x 32 32 x 32 27.0, 128 x 128 29.9.
 int choose_form(const so_ctx *ctx, uint32_t m, uint32_t C)
 {

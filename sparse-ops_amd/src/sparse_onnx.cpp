@@ -300,7 +300,7 @@ SparseOnnxModel::SparseOnnxModel(const std::string &onnx_path) : impl_(new Impl(
             int64_t axis = -1, stash = 1;
             if (const auto *a = node.find("axis")) axis = a->i;
             if (const auto *a = node.find("stash_type")) stash = a->i;
-            if (axis != 1 && axis + int64_t(xs.size()) != 1)
+            if (axis != 1 && axis != 1 - int64_t(xs.size()))
                 throw std::runtime_error("LayerNormalization: only over all axes but the batch is supported");
             if (stash != 1) throw std::runtime_error("LayerNormalization: stash_type must be 1 (float)");
             for (std::size_t k = 1; k < node.output.size(); ++k)

@@ -226,6 +226,30 @@ def test_the_same_bits_every_time_and_across_states(ctx):
     second.free()
 
 
+def test_one_matrix_from_two_contexts(ctx):
+    """A matrix made by one context is ready for another's stream at once; the two multiply without waiting for each other, each in its own workspace."""
+    rng = np.random.default_rng(21)
+    other = hipabi.Context()
+    try:
+        handle, W = weights(ctx, rng, 1500, 2000)
+        X = rng.standard_normal((2, 2000, 300)).astype(np.float32)
+        ins, outs = [c.array(x) for c, x in zip((ctx, other), X)], [c.empty((1500, 300)) for c in (ctx, other)]
+        for _ in range(3):
+            for c, dX, dY in zip((ctx, other), ins, outs):
+                c.mxfp4_matmul(handle, dX, 300, None, dY)
+        for x, dY in zip(X, outs):
+            Xq = mx.dequantize(*mx.quantize(np.ascontiguousarray(x.T.astype(np.float64))), 2000).T
+            want = W @ Xq
+            assert np.all(np.abs(dY.download() - want) <= product_tolerance(W, Xq, None, want, "none", "f32"))
+        ctx.sync()
+        other.sync()
+        handle.free()
+        for a in ins + outs:
+            a.free()
+    finally:
+        other.close()
+
+
 def test_offsets_beyond_32_bits(ctx):
     """Rows 2^30 + 5 elements apart, the last ones beyond 2^32 elements: quantisation, its way back, the input and the output of a product."""
     rng = np.random.default_rng(15)

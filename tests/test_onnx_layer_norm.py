@@ -14,6 +14,8 @@ def norm_model(shape=(2, 6), scale=(6,), bias=(6,), inputs=None, outputs=("y",),
     (norm_model(axis=0), "over all axes but the batch"),
     (norm_model(axis=-2), "over all axes but the batch"),
     (norm_model(axis=2), "over all axes but the batch"),
+    (norm_model(axis=2 ** 63 - 1), "over all axes but the batch"),
+    (norm_model(axis=-3), "over all axes but the batch"),
     (norm_model((2, 3, 2, 1), axis=-1), "over all axes but the batch"),
     (norm_model((2, 3, 2, 1)), "over all axes but the batch"),                 # the default is the last axis
     (norm_model((2, 3, 2, 1), axis=2), "over all axes but the batch"),
