@@ -113,6 +113,8 @@ __device__ __forceinline__ void write_rows(const Place<T, LC, RPT, NT, FULL> &at
 }
 
 // All features of a tile of columns in one workgroup's registers: X is read once.  The tiles go to the XCDs in runs of neighbours, which share cache lines where LC is less than 8.
+// Bound by the memory where there are tiles enough, in three phases that do not overlap, since a compute unit holds one large tile: 4096 x 8192 bf16 34.5 us, 3.9 TB/s (a copy 24); by latencies
+// where not: 4096 x 1 fp32 5.2 us.
 template <class T, int LC, int RPT, int NT>
 __global__ __launch_bounds__(NT)
 void norm_whole_kernel(uint32_t F, uint32_t B, uint32_t tiles, uint32_t per_xcd, const T *X, size_t ldx, const float *__restrict__ gamma, const float *__restrict__ beta, float eps, T *Y,
@@ -161,7 +163,7 @@ void norm_whole_kernel(uint32_t F, uint32_t B, uint32_t tiles, uint32_t per_xcd,
     });
 }
 
-// Mean and sum of squared deviations of every column of a part.
+// Mean and sum of squared deviations of every column of a part; then the parts joined and the result.  4096 x 256 fp32 3.0 + 4.2 us, one workgroup a compute unit.
 template <class T, int LC, int RPT>
 __global__ __launch_bounds__(kThreads)
 void norm_parts_kernel(uint32_t F, uint32_t B, uint32_t tiles, const T *X, size_t ldx, float2 *__restrict__ cols)
