@@ -69,7 +69,8 @@ __device__ __forceinline__ uint32_t so_group_wide_rows(uint32_t left, uint32_t r
     return rows > below ? rows - below : 0u;
 }
 
-// The first `left` elements of a group, whole or in pieces of 4, 2 and 1; fp32 values are rounded to nearest even.
+// The first `left` elements of a group, whole or in pieces of 4, 2 and 1; fp32 values are rounded to nearest even.  Stored for the next reader: past the caches (nontemporal) a layer norm of
+// 4096 x 8192 bf16 on data from memory takes 29 us instead of 34.5, but a second one that reads its result 71 instead of 50 for the two.
 template <class T>
 __device__ __forceinline__ void so_group_store(T *p, uint32_t left, const float (&f)[so_elements<T>::V])
 {
