@@ -361,7 +361,7 @@ so_status so_layer_norm(so_ctx *ctx, int type, uint32_t F, uint32_t B, const voi
                         float *dMean, float *dRstd);
 /* Its gradient: with g = dY * gamma and h = (X - mean) * rstd, dX = rstd * (g - sum_f g / F - h * sum_f (g h) / F),
  * dgamma_f = sum_b dY h, dbeta_f = sum_b dY, written, not added to.  Any of the three may be NULL.  dDx may be dX or dDy
- * with the same stride.  With B = 0 dgamma and dbeta are zeros.  Sums are taken in the same order on every call. */
+ * with the same stride; other overlaps are not allowed.  With B = 0 dgamma and dbeta are zeros.  Sums are taken in the same order on every call. */
 so_status so_layer_norm_grad(so_ctx *ctx, int type, uint32_t F, uint32_t B, const void *dX, size_t x_stride,
                              const void *dDy, size_t dy_stride, const float *dGamma, const float *dMean,
                              const float *dRstd, void *dDx, size_t dx_stride, float *dDgamma, float *dDbeta);

@@ -294,6 +294,7 @@ extern "C" so_status so_layer_norm(so_ctx *ctx, int type, uint32_t F, uint32_t B
     SO_REQUIRE(dX && dY, "so_layer_norm: null tensor");
     SO_REQUIRE(x_stride >= B && y_stride >= B, "so_layer_norm: a stride is shorter than a row");
     SO_REQUIRE(dX != dY || x_stride == y_stride, "so_layer_norm: in place needs one stride");
+    SO_REQUIRE(!dMean || dMean != dRstd, "so_layer_norm: one array for both statistics");
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
     const Cut c = cut_of(type, F, B);

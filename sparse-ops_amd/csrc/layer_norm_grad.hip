@@ -271,6 +271,8 @@ extern "C" so_status so_layer_norm_grad(so_ctx *ctx, int type, uint32_t F, uint3
     SO_REQUIRE(dX && dDy && dMean && dRstd, "so_layer_norm_grad: null tensor");
     SO_REQUIRE(x_stride >= B && dy_stride >= B && (!dDx || dx_stride >= B), "so_layer_norm_grad: a stride is shorter than a row");
     SO_REQUIRE((dDx != dX || dx_stride == x_stride) && (dDx != dDy || dx_stride == dy_stride), "so_layer_norm_grad: in place needs one stride");
+    SO_REQUIRE(!dDgamma || (dDgamma != dDbeta && dDgamma != dGamma), "so_layer_norm_grad: aliased parameter gradients");
+    SO_REQUIRE(!dDbeta || dDbeta != dGamma, "so_layer_norm_grad: aliased parameter gradients");
     const bool params = dDgamma || dDbeta;
     if (!dDx && !params) return SO_OK;
     const Cut c = cut_of(type, F, B);

@@ -255,6 +255,10 @@ def test_no_columns_and_refusals(ctx):
     refused("too large for one launch", lambda: ctx.layer_norm_grad(dX, dY, 0x7fffffff, 100, None, st, st, dX, None, None))
     refused("too large for one launch", lambda: ctx.layer_norm_reserve(1, 0xffffffff))
     refused("no features", lambda: ctx.layer_norm_grad(dX, dY, 0, B, None, st, st, dX, None, None))
+    refused("both statistics", lambda: ctx.layer_norm(dX, F, B, None, None, EPS, dY, st, st))
+    wide, other = ctx.empty((F,)), ctx.empty((F,))
+    for args in ((wide, wide, other), (wide, other, wide), (wide, other, other)):
+        refused("aliased", lambda: ctx.layer_norm_grad(dX, dY, F, B, args[0], st, st, dX, args[1], args[2]))
     refused("null tensor", lambda: ctx.layer_norm_grad(dX, None, F, B, None, st, st, dX, None, None))
     refused("null tensor", lambda: ctx.layer_norm_grad(dX, dY, F, B, None, None, st, dX, None, None))
     refused("stride", lambda: ctx.layer_norm_grad(dX, dY, F, B, None, st, st, dX, None, None, dy_stride=1))
