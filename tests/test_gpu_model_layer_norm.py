@@ -81,3 +81,31 @@ def test_between_products(backend, ctx, tmp_path, B):
     rel = off_s.max(axis=1, keepdims=True) / np.abs(s).max(axis=1, keepdims=True)
     bound = tol + 3 * np.abs(g2) * rel * top * (1 + np.abs(y - c2) / np.abs(g2))
     assert np.all(np.abs(results[0] - y) <= bound), np.max(np.abs(results[0] - y) / bound)
+
+
+@pytest.mark.parametrize("B", [1, 3, 5, 7, 20, 33])
+def test_after_a_convolution(backend, ctx, tmp_path, B):
+    """With convolutions the batch is carried in longer rows: what stands behind it (zeros, which without an epsilon become NaN) reaches no sample.  A sample's result is within the
+    normalisation's tolerance of that of its own convolution, taken from a model that ends there."""
+    rng = np.random.default_rng(40 + B)
+    Wc = datagen.magnitude_prune(rng.standard_normal((8, 27)).astype(np.float32), .5).reshape(8, 3, 3, 3)
+    bc, g, b = (rng.standard_normal(n).astype(np.float32) for n in (8, 8 * 36, 8 * 36))
+    Wf = datagen.magnitude_prune(rng.standard_normal((10, 8 * 36)).astype(np.float32), .5)
+    conv = ow.node("Conv", ["x", "Wc", "bc"], ["c"], kernel_shape=[3, 3], pads=[1, 1, 1, 1], strides=[1, 1], dilations=[1, 1], group=1)
+    norm_node = ow.node("LayerNormalization", ["c", "g", "b"], ["n"], axis=1, epsilon=0.0)
+    inits = [("Wc", Wc), ("bc", bc), ("g", g.reshape(8, 6, 6)), ("b", b.reshape(8, 6, 6)), ("Wf", Wf)]
+    tail = [ow.node("Flatten", ["n"], ["f"], axis=1), ow.node("Gemm", ["f", "Wf"], ["y"], alpha=1.0, beta=1.0, transB=1)]
+    image = [("x", (B, 3, 6, 6))]
+    X = rng.standard_normal((B, 3, 6, 6)).astype(np.float32)
+    make = lambda name, nodes, out: backend.SparseOnnxModel(ow.save(str(tmp_path / name), ow.model(nodes, image, [out], inits, opset=17)))
+    c = make("c.onnx", [conv], ("c", (B, 8, 6, 6))).run(X).reshape(B, -1).astype(np.float64)
+    want, tol, _ = norm(c, g, b, 0.0)
+    model = make("n.onnx", [conv, norm_node], ("n", (B, 8, 6, 6)))
+    for Y in (model.run(X), _run_device(model, ctx, X)):
+        assert np.all(np.abs(Y.reshape(B, -1) - want) <= tol)
+    whole = make("y.onnx", [conv, norm_node] + tail, ("y", (B, 10)))
+    W = np.abs(Wf.T.astype(np.float64))
+    # the product adds at most 288 entries of a row, each with two roundings
+    bound = tol @ W + U * 2 * 288 * (np.abs(want) @ W)
+    for Y in (whole.run(X), whole.run(X), _run_device(whole, ctx, X)):
+        assert np.all(np.abs(Y - want @ Wf.T.astype(np.float64)) <= bound)
