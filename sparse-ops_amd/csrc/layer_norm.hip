@@ -13,9 +13,10 @@ namespace {
 // Mean m and sum of squared deviations q of two sets of na and nb values from those of each: with t = mb - ma, m = ma + t nb / (na + nb), q = qa + qb + t^2 na nb / (na + nb).  No
 // difference of large sums is taken, so a column far from zero keeps its variance.
 struct Share { float to, sq; };      // nb / (na + nb), na nb / (na + nb)
+// The first of two is 1 where a is empty, which the hardware's reciprocal times nb need not be: a column of one value keeps it as its mean.
 __device__ __forceinline__ Share share_of(float na, float nb)
 {
-    const float sum = na + nb, to = sum > 0.0f ? nb * __builtin_amdgcn_rcpf(sum) : 0.0f;
+    const float to = na > 0.0f ? nb * __builtin_amdgcn_rcpf(na + nb) : nb > 0.0f ? 1.0f : 0.0f;
     return {to, na * to};
 }
 __device__ __forceinline__ void join(float2 &a, float2 b, Share s)
