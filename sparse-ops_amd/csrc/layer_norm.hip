@@ -11,7 +11,8 @@ using namespace so_norm;
 namespace {
 
 // Mean m and sum of squared deviations q of two sets of na and nb values from those of each: with t = mb - ma, m = ma + t nb / (na + nb), q = qa + qb + t^2 na nb / (na + nb).  No
-// difference of large sums is taken, so a column far from zero keeps its variance.
+// difference of large sums is taken, so a column far from zero keeps its variance.  The share is taken before the square: beside an empty set (mean 0) t is the column's own size, whose
+// square fp32 need not hold.
 struct Share { float to, sq; };      // nb / (na + nb), na nb / (na + nb)
 // The first of two is 1 where a is empty, which the hardware's reciprocal times nb need not be: a column of one value keeps it as its mean.
 __device__ __forceinline__ Share share_of(float na, float nb)
@@ -23,7 +24,7 @@ __device__ __forceinline__ void join(float2 &a, float2 b, Share s)
 {
     const float t = b.x - a.x;
     a.x = fmaf(t, s.to, a.x);
-    a.y = fmaf(t * t, s.sq, a.y + b.y);
+    a.y = fmaf(t * s.sq, t, a.y + b.y);
 }
 
 // done(column of the tile, its mean and sum of squared deviations over the rows of the workgroup), in one thread for each column: a thread's own rows first, in one pass as

@@ -1,11 +1,11 @@
-"""so_layer_norm on columns at the ends of the element types: columns without variance.
+"""so_layer_norm on columns at the ends of the element types: values whose squares fp32 does not hold, columns without variance.
 
 Statistics and results are those of test_gpu_layer_norm.py, with its tolerances; a column of one value has that value as its mean and no deviation in any order of its sums, so its results are exact."""
 import numpy as np
 import pytest
 
-from elements import fetch, place
-from test_gpu_layer_norm import EPS
+from elements import U, fetch, place, stored, values
+from test_gpu_layer_norm import EPS, check_forward, check_grad, check_statistics, problem, statistics
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,47 @@ def test_columns_of_one_value_in_parts(ctx, B):
         Y, mean, _ = forward(ctx, X, np.ones(F, np.float32), beta, "f32", -1)
         assert np.array_equal(mean, X[0]), (rows, mean)
         assert np.array_equal(Y, np.tile(beta.astype(np.float64)[:, None], (1, B))), rows
+
+
+@pytest.mark.parametrize("lanes", LANES)
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("F", [1, 3, 70, 1000, 9000])
+def test_values_whose_squares_fp32_does_not_hold(ctx, F, type_, lanes):
+    """Columns of one value of 2^64 .. 2^120 have no variance: the results are beta, the statistics the value and 1 / sqrt(eps)."""
+    B = 13
+    _, _, gamma, beta = problem(F, B, type_)
+    value = np.exp2(np.linspace(64, 120, B).round()) * np.where(np.arange(B) % 2, -1.0, 1.0)
+    X = np.tile(value, (F, 1))
+    Y, mean, rstd = forward(ctx, X, gamma, beta, type_, lanes)
+    assert np.array_equal(Y, np.tile(values(stored(beta, type_), type_)[:, None], (1, B)))
+    assert np.array_equal(mean.astype(np.float64), value)
+    want = 1.0 / np.sqrt(np.float64(np.float32(EPS)))
+    assert np.all(np.abs(rstd - want) <= want * 4 * U)          # a root and a quotient
+
+
+@pytest.mark.parametrize("lanes", LANES)
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("F", [1, 3, 33, 70])
+def test_large_values_that_differ(ctx, F, type_, lanes):
+    """A mean of 2^66, whose square fp32 does not hold, and deviations of 2^59, the sum of whose squares it does."""
+    rng, _, gamma, beta = problem(F, 11, type_)
+    X = values(stored(2.0 ** 66 + 2.0 ** 59 * rng.uniform(-2, 2, (F, 11)), type_), type_)
+    Y, mean, rstd = forward(ctx, X, gamma, beta, type_, lanes)
+    check_forward(Y, X, gamma, beta, type_)
+    check_statistics(mean, rstd, X)
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("F,B", [(3, 5), (70, 11), (1100, 40)])
+def test_gradient_of_large_values(ctx, F, B, type_):
+    """The gradient at such columns: one workgroup's, and in parts."""
+    rng, _, gamma, _ = problem(F, B, type_)
+    X = values(stored(2.0 ** 66 + 2.0 ** 58 * rng.uniform(-2, 2, (F, B)), type_), type_)
+    dY = values(stored(rng.standard_normal((F, B)), type_), type_)
+    mean, rstd = (s.astype(np.float32) for s in statistics(X))
+    dX, dDy, dDx = (place(ctx, M, type_)[0] for M in (X, dY, np.zeros((F, B))))
+    dG, dM, dR, dDg, dDb = ctx.array(gamma), ctx.array(mean), ctx.array(rstd), ctx.empty((F,)), ctx.empty((F,))
+    ctx.layer_norm_grad(dX, dDy, F, B, dG, dM, dR, dDx, dDg, dDb, type=type_)
+    check_grad(fetch(dDx, F, B, type_)[0], dDg.download(), dDb.download(), X, dY, gamma, mean, rstd, type_)
+    for a in (dX, dDy, dDx, dG, dM, dR, dDg, dDb):
+        a.free()
