@@ -355,7 +355,7 @@ enum { SO_F32 = 0, SO_F16 = 1, SO_BF16 = 2 };
 /* For every column b: mean_b = sum_f X / F, rstd_b = 1 / sqrt(sum_f (X - mean)^2 / F + eps),
  * Y = (X - mean) * rstd * gamma_f + beta_f.  dGamma NULL: ones, dBeta NULL: zeros.  dMean, dRstd [B]: what
  * so_layer_norm_grad takes, or NULL.  dY may be dX with the same stride; other overlaps are not allowed.  B may be 0, F may not.  A column
- * with an infinity or NaN gives NaN throughout, the others are not touched by it. */
+ * with an infinity or NaN gives NaN throughout, its statistics too; the others are not touched by it. */
 so_status so_layer_norm(so_ctx *ctx, int type, uint32_t F, uint32_t B, const void *dX, size_t x_stride,
                         const float *dGamma, const float *dBeta, float eps, void *dY, size_t y_stride,
                         float *dMean, float *dRstd);

@@ -27,6 +27,14 @@ __device__ __forceinline__ void join(float2 &a, float2 b, Share s)
     a.y = fmaf(t * s.sq, t, a.y + b.y);
 }
 
+// What a column's mean and sum of squared deviations give: its mean and 1 / deviation.  An infinity or NaN in it leaves the mean no finite number in any order of the joins, and where it
+// is an infinity (one row a thread) the squares may still be 0: x - x makes both results NaN then, and adds zero otherwise.
+__device__ __forceinline__ float2 results_of(float2 all, uint32_t F, float eps)
+{
+    const float none = all.x - all.x;
+    return make_float2(all.x + none, 1.0f / sqrtf(all.y / (float)F + eps) + none);
+}
+
 // done(column of the tile, its mean and sum of squared deviations over the rows of the workgroup), in one thread for each column: a thread's own rows first, in one pass as
 // they come, as differences from the first of them, then the rows of a wave pair by pair, then the waves.  A thread holds 32 rows at most, and the value that it counts from is one
 // of them: the squares that cancel are at most as many times what is left, so the sum keeps all but 5 of its bits wherever the column lies and whatever sticks out of it.  `lds` holds NT / 64 * LC * V values.
@@ -147,12 +155,11 @@ void norm_whole_kernel(uint32_t F, uint32_t B, uint32_t tiles, uint32_t per_xcd,
         }
         at.load(x, X, ldx);
         tile_moments(at, x, lds, [&](uint32_t col, float2 all) {
-            const float rstd = 1.0f / sqrtf(all.y / (float)F + eps);
-            st[col] = make_float2(all.x, rstd);
+            const float2 of = st[col] = results_of(all, F, eps);
             const uint64_t c = (uint64_t)id * (LC * V) + col;
             if (c < B) {
-                if (mean_out) mean_out[c] = all.x;
-                if (rstd_out) rstd_out[c] = rstd;
+                if (mean_out) mean_out[c] = of.x;
+                if (rstd_out) rstd_out[c] = of.y;
             }
         });
         if constexpr (!OWN)
@@ -209,12 +216,11 @@ void norm_apply_kernel(uint32_t F, uint32_t B, uint32_t parts, uint32_t tiles, c
                                                  at.load(x, X, ldx);
                                              });
         if (threadIdx.x < COLS) {
-            const float rstd = 1.0f / sqrtf(all.s.y / (float)F + eps);
-            st[threadIdx.x] = make_float2(all.s.x, rstd);
+            const float2 of = st[threadIdx.x] = results_of(all.s, F, eps);
             const uint64_t c = (uint64_t)first + threadIdx.x;
             if (at.part == 0 && c < B) {
-                if (mean_out) mean_out[c] = all.s.x;
-                if (rstd_out) rstd_out[c] = rstd;
+                if (mean_out) mean_out[c] = of.x;
+                if (rstd_out) rstd_out[c] = of.y;
             }
         }
         __syncthreads();

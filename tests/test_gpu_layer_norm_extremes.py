@@ -1,10 +1,10 @@
-"""so_layer_norm on columns at the ends of the element types: values whose squares fp32 does not hold, columns without variance.
+"""so_layer_norm on columns at the ends of the element types: infinities wherever they stand, values whose squares fp32 does not hold, columns without variance.
 
 Statistics and results are those of test_gpu_layer_norm.py, with its tolerances; a column of one value has that value as its mean and no deviation in any order of its sums, so its results are exact."""
 import numpy as np
 import pytest
 
-from elements import U, fetch, place, stored, values
+from elements import TYPES, U, fetch, place, stored, values
 from test_gpu_layer_norm import EPS, check_forward, check_grad, check_statistics, problem, statistics
 
 pytestmark = pytest.mark.gpu
@@ -93,3 +93,27 @@ def test_gradient_of_large_values(ctx, F, B, type_):
     check_grad(fetch(dDx, F, B, type_)[0], dDg.download(), dDb.download(), X, dY, gamma, mean, rstd, type_)
     for a in (dX, dDy, dDx, dG, dM, dR, dDg, dDb):
         a.free()
+
+
+@pytest.mark.parametrize("lanes", LANES)
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("F", [1, 2, 3, 65, 200, 2000, 9000])
+def test_not_finite_wherever_it_stands(ctx, F, type_, lanes):
+    """One infinity or NaN in a column, in its first, its second, its last or some other row, or several: results and statistics of that column are NaN, the others keep theirs."""
+    B = 23
+    rng, X, gamma, beta = problem(F, B, type_, seed=11)
+    bad = list(range(1, B, 2))
+    for i, b in enumerate(bad):
+        row = (0, min(1, F - 1), F - 1, int(rng.integers(F)))[i % 4]
+        X[row, b] = (np.inf, -np.inf, np.nan)[i % 3]
+        if i == len(bad) - 1:
+            X[:, b] = np.inf
+        if i == len(bad) - 2:
+            X[:, b] = np.where(np.arange(F) % 2, np.inf, -np.inf)
+    good = [b for b in range(B) if b not in bad]
+    Y, mean, rstd = forward(ctx, X, gamma, beta, type_, lanes)
+    assert np.isnan(Y[:, bad]).all()
+    assert np.isnan(mean[bad]).all(), mean[bad]
+    assert np.isnan(rstd[bad]).all(), rstd[bad]
+    check_forward(Y[:, good], X[:, good], gamma, beta, type_)
+    check_statistics(mean[good], rstd[good], X[:, good])
