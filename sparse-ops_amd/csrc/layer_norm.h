@@ -214,7 +214,7 @@ void for_lanes(uint32_t lanes, F &&f)
     else f(std::integral_constant<int, 8>());
 }
 
-// (The kernel that holds all features has no more threads: it takes 512 only where a tile has several parts.)
+// Of the kernels that take parts, and of the one that holds all features with as many lanes a row as it chooses.
 static inline bool ranges_fit(const Cut &c, uint32_t joiners = 0) { return so_grid_fits(c.groups + joiners + 64, kThreads); }
 
 static inline so_status workspace(so_ctx *ctx, const char *who, size_t bytes)

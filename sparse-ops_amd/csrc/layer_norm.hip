@@ -309,6 +309,7 @@ extern "C" so_status so_layer_norm(so_ctx *ctx, int type, uint32_t F, uint32_t B
     SO_REQUIRE(ranges_fit(c), "so_layer_norm: %u x %u is too large for one launch", F, B);
     if (const Whole w = whole_of(ctx, type, F, B); w.lanes) {
         const uint32_t tiles = so_ceil_div(B, w.lanes * (16u / (uint32_t)so_type_bytes(type))), per_xcd = so_ceil_div(tiles, 8);
+        SO_REQUIRE(so_grid_fits((uint64_t)per_xcd * 8, w.threads), "so_layer_norm: %u x %u is too large for one launch", F, B);      // fewer lanes forced, more tiles
         hipError_t allowed = hipSuccess;
         so_for_type(type, [&](auto t) {
             using T = decltype(t);

@@ -4,6 +4,7 @@ Statistics and results are those of test_gpu_layer_norm.py, with its tolerances;
 import numpy as np
 import pytest
 
+import hipabi
 from elements import TYPES, U, fetch, place, stored, values
 from test_gpu_layer_norm import EPS, check_forward, check_grad, check_statistics, problem, statistics
 
@@ -117,3 +118,13 @@ def test_not_finite_wherever_it_stands(ctx, F, type_, lanes):
     assert np.isnan(rstd[bad]).all(), rstd[bad]
     check_forward(Y[:, good], X[:, good], gamma, beta, type_)
     check_statistics(mean[good], rstd[good], X[:, good])
+
+
+def test_forced_tiles_that_a_launch_does_not_hold(ctx):
+    """2^28 columns are 2^26 workgroups at one lane a row, more threads than a launch has: refused ahead of any work."""
+    a = ctx.empty((64,))
+    with ctx.tuning(SPARSEOPS_NORM_LANES=1):
+        with pytest.raises(hipabi.SoError, match="too large for one launch") as e:
+            ctx.layer_norm(a, 1, 1 << 28, None, None, EPS, a)
+    assert e.value.status == hipabi.SO_ERR_INVALID
+    a.free()
