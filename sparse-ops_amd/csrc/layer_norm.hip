@@ -247,33 +247,54 @@ Whole whole_of(const so_ctx *ctx, int type, uint32_t F, uint32_t B)
     // One launch and one reading against two: it is the slower one only where long columns leave most compute units without a tile or give them 16 bytes of a row each (a cache line a
     // row and workgroup, in and out).  Whole / in parts, us: fp32 1024 x 1024 6.0 / 6.4, 8192 x 1 6.7 / 7.2, 4096 x 256 9.8 / 6.6, 4096 x 1024 17 / 11, 4096 x 4096 23 / 34; bf16 512 x 1024
     // 4.7 / 6.4, 1024 x 1024 7.6 / 6.6, 2048 x 16 6.8 / 6.6, 4096 x 1 8.3 / 7.5, 2048 x 16384 25 / 39, 8192 x 4096 34 / 40.
-    if (asked < 0 && (few || lanes == 1) && F * V > 4096 && ((uint64_t)F * B > 65536 || F * V * V > 131072)) return {0, 0, 0};
-    uint32_t threads = per <= 512 ? 256 : few && per <= 8192 ? 1024 : per <= 4096 ? 256 : 512, rows = 1;
+    if (lanes == 1 && F * V * V > 131072) return {0, 0, 0};
+    if (asked < 0 && (few || lanes == 1) && F * V > 4096 && (uint64_t)F * B > 65536) return {0, 0, 0};
+    // 1024 threads where only latency counts, which with more lanes a row is in parts
+    const uint32_t threads = per <= 512 ? 256 : lanes == 1 && (few || per > 4096 / V) ? 1024 : per <= 4096 ? 256 : 512;
+    uint32_t rows = 1;
     while (rows * threads < per) rows *= 2;
     return {lanes, rows, threads};
 }
 
-template <class F>
+// f(lanes, rows, threads) as compile-time numbers, for those that whole_of chooses with 16 / V bytes an element.
+template <int V, class F>
 void for_whole(const Whole &w, F &&f)
 {
-    const auto rows = [&](auto lanes, auto threads) {
-        constexpr int NT = decltype(threads)::value;
-        if constexpr (NT == 512) {
-            if (w.rows == 16) f(lanes, std::integral_constant<int, 16>(), threads);
-            else f(lanes, std::integral_constant<int, 32>(), threads);
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    const std::integral_constant<int, 4> four;
+    const std::integral_constant<int, 8> eight;
+    const std::integral_constant<int, 16> sixteen;
+    const std::integral_constant<int, 256> few;
+    const std::integral_constant<int, 512> more;
+    const std::integral_constant<int, 1024> most;
+    const auto more_lanes = [&](auto lanes) {
+        if (w.threads == 512) {
+            if (w.rows == 16) f(lanes, sixteen, more);
+            else f(lanes, std::integral_constant<int, 32>(), more);
         } else {
-            if (w.rows == 1) f(lanes, std::integral_constant<int, 1>(), threads);
-            else if (w.rows == 2) f(lanes, std::integral_constant<int, 2>(), threads);
-            else if (w.rows == 4) f(lanes, std::integral_constant<int, 4>(), threads);
-            else if (NT == 1024 || w.rows == 8) f(lanes, std::integral_constant<int, 8>(), threads);
-            else if constexpr (NT == 256) f(lanes, std::integral_constant<int, 16>(), threads);
+            if (w.rows == 1) f(lanes, one, few);
+            else if (w.rows == 2) f(lanes, two, few);
+            else if (w.rows == 4) f(lanes, four, few);
+            else if (w.rows == 8) f(lanes, eight, few);
+            else f(lanes, sixteen, few);
         }
     };
-    for_lanes(w.lanes, [&](auto lanes) {
-        if (w.threads == 256) rows(lanes, std::integral_constant<int, 256>());
-        else if (w.threads == 512) rows(lanes, std::integral_constant<int, 512>());
-        else rows(lanes, std::integral_constant<int, 1024>());
-    });
+    if (w.lanes == 2) more_lanes(two);
+    else if (w.lanes == 4) more_lanes(four);
+    else if (w.lanes == 8) more_lanes(eight);
+    else if (w.threads == 256) {
+        if (w.rows == 1) f(one, one, few);
+        else if (V == 8 || w.rows == 2) f(one, two, few);
+        else if constexpr (V == 4) f(one, four, few);
+    } else {
+        if (w.rows == 1) f(one, one, most);
+        else if (V == 8 || w.rows == 2) f(one, two, most);
+        else if constexpr (V == 4) {
+            if (w.rows == 4) f(one, four, most);
+            else f(one, eight, most);
+        }
+    }
 }
 
 } // namespace
@@ -313,7 +334,7 @@ extern "C" so_status so_layer_norm(so_ctx *ctx, int type, uint32_t F, uint32_t B
         hipError_t allowed = hipSuccess;
         so_for_type(type, [&](auto t) {
             using T = decltype(t);
-            for_whole(w, [&](auto lanes, auto rows, auto threads) {
+            for_whole<so_elements<T>::V>(w, [&](auto lanes, auto rows, auto threads) {
                 constexpr int LC = decltype(lanes)::value, RPT = decltype(rows)::value, NT = decltype(threads)::value;
                 const uint32_t lds = ((NT / 64 + 1) * LC * so_elements<T>::V + (RPT <= 8 ? 0u : F)) * (uint32_t)sizeof(float2);
                 const auto kernel = norm_whole_kernel<T, LC, RPT, NT>;

@@ -219,14 +219,13 @@ One one_of(const so_ctx *ctx, int type, uint32_t F, uint32_t B)
     const uint32_t V = 16u / (uint32_t)so_type_bytes(type);
     uint32_t lanes = 1;
     while (lanes < 8 && B > lanes * V) lanes *= 2;
-    const int asked = ctx->tune.norm_lanes;
-    if (asked == 0 || B > lanes * V) return {0, 0, 0};
-    if ((uint64_t)F * lanes * V > (asked > 0 ? 2048 * V : 8192)) return {0, 0, 0};
+    if (ctx->tune.norm_lanes == 0 || B > lanes * V || (uint64_t)F * lanes * V > 8192) return {0, 0, 0};
     const uint32_t per = F * lanes, threads = per <= 512 ? 256 : 1024;
     return {lanes, so_ceil_div(per, threads), threads};
 }
 
-template <class F>
+// As for_whole: 16-bit types have a row a thread of 1024 at most.
+template <int V, class F>
 void for_one(const One &w, F &&f)
 {
     for_lanes(w.lanes, [&](auto lanes) {
@@ -238,8 +237,8 @@ void for_one(const One &w, F &&f)
             if (w.rows == 1) f(lanes, one, few);
             else f(lanes, two, few);
         } else {
-            if (w.rows == 1) f(lanes, one, many);
-            else f(lanes, two, many);
+            if (V == 8 || w.rows == 1) f(lanes, one, many);
+            else if constexpr (V == 4) f(lanes, two, many);
         }
     });
 }
@@ -280,7 +279,7 @@ extern "C" so_status so_layer_norm_grad(so_ctx *ctx, int type, uint32_t F, uint3
     if (const One w = one_of(ctx, type, F, B); w.lanes) {
         so_for_type(type, [&](auto t) {
             using T = decltype(t);
-            for_one(w, [&](auto lanes, auto held, auto threads) {
+            for_one<so_elements<T>::V>(w, [&](auto lanes, auto held, auto threads) {
                 constexpr int LC = decltype(lanes)::value, RPT = decltype(held)::value, NT = decltype(threads)::value;
                 norm_grad_one_kernel<T, LC, RPT, NT><<<1, NT, 0, ctx->stream>>>(F, B, (const T *)dX, x_stride, (const T *)dDy, dy_stride, dGamma, dMean, dRstd, (T *)dDx, dx_stride,
                                                                                 dDgamma, dDbeta);

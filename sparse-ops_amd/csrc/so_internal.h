@@ -36,7 +36,7 @@ struct so_tuning {
     int conv_columns = -1;   // SPARSEOPS_CONV_COLUMNS: 0 forbids the column kernel, 1 forces it on plans tuned for the batch
     int conv_vec = 0;        // SPARSEOPS_CONV_VEC: most batch entries per lane in the gather kernel
     int wait_spins = -1;     // SPARSEOPS_WAIT_SPINS: most polls of a bounded wait on LDS progress counters (0: every wait gives up at once; tests)
-    int norm_lanes = -1;     // SPARSEOPS_NORM_LANES: lanes of a row (1, 2, 4, 8) of the layer norm that holds all features, 0 forbids it and the gradient in one workgroup
+    int norm_lanes = -1;     // SPARSEOPS_NORM_LANES: lanes of a row (1, 2, 4, 8) of the layer norm that holds all features, 0 forbids it and the gradient in one workgroup; more than whole_of has a kernel for: in parts
     int mxfp4_form = 0;      // SPARSEOPS_MXFP4_MATMUL: the tile of so_mxfp4_matmul, by its number in csrc/mxfp4_matmul.hip
     int conv_rbm = -1;       // SPARSEOPS_CONV_RBM: 0 forbids the row-block-merged kernel on plans that carry its streams, 1 asks for it against any other override
 };
