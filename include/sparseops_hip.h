@@ -392,7 +392,8 @@ so_status so_mxfp4_dims(const so_mxfp4 *W, uint32_t *m, uint32_t *n);
 /* Y [m x C] = act(W Q(X) + bias): so_matmul with both operands in 4 bits.  X [n x C] and Y are of `type`, rows x_stride
  * and y_stride elements apart; Q quantises X as above in blocks of 32 of its rows, within the call.  Products and the sums of a
  * block are exact, blocks are added in fp32, in the same order on every call; Y is rounded once.  dBias [m] may be NULL.
- * A block of X that is not a number makes its column of Y NaN, one of W its row. */
+ * A block of X that is not a number makes its column of Y NaN, one of W its row, through every activation (SO_ACT_RELU keeps
+ * NaN here; so_act and so_matmul, as the reference, make 0 of it). */
 so_status so_mxfp4_matmul(so_ctx *ctx, const so_mxfp4 *W, int type, const void *dX, size_t x_stride, uint32_t C,
                           const float *dBias, void *dY, size_t y_stride, int act);
 /* Grows the context's workspace to what C columns need: before recording a product into a graph, as so_matmul_reserve. */

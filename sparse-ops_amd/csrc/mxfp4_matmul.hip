@@ -27,6 +27,14 @@ __device__ __forceinline__ void each(F &&f)
     }
 }
 
+// The activation of a sum, as so_epilogue but that a ReLU keeps NaN: a block that is not a number marks all results that it goes into.
+template <int ACT>
+__device__ __forceinline__ float mx_epilogue(float v)
+{
+    if constexpr (ACT == SO_ACT_RELU) return v <= 0.0f ? 0.0f : v;
+    else return so_epilogue<ACT>(v);
+}
+
 // Which tile of the output a workgroup takes.  Workgroups go round-robin to the 8 XCDs; each XCD gets neighbouring tiles of a strip four tiles of columns wide, so that its L2 is
 // asked for few rows of W and few columns of X.
 struct MxTile { uint32_t m, c; bool none; };
@@ -130,7 +138,7 @@ void mx_matmul_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restric
 #pragma unroll
             for (int w = 1; w < WK; ++w) s += sums[(w * MH * 16 + r) * (PITCH / 4) + (c + e) / 4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[e + i] = so_epilogue<ACT>(s[i] + add);
+            for (int i = 0; i < 4; ++i) y[e + i] = mx_epilogue<ACT>(s[i] + add);
         }
         so_group_store(Y + row * ldy + col, (uint32_t)min((uint64_t)V, C - col), y);
     }
@@ -272,7 +280,7 @@ void mx_matmul_staged_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__
             if (row >= m || col >= C) continue;
             const float add = bias ? bias[row] : 0.0f;
 #pragma unroll
-            for (int f = 0; f < V; ++f) y[f] = so_epilogue<ACT>(y[f] + add);
+            for (int f = 0; f < V; ++f) y[f] = mx_epilogue<ACT>(y[f] + add);
             so_group_store(Y + row * ldy + col, (uint32_t)min((uint64_t)V, C - col), y);
         }
         __builtin_amdgcn_wave_barrier();
