@@ -19,11 +19,12 @@
  *     [features x B] with the batch contiguous (include/sparse_onnx.hpp:148-154),
  *     4-D tensors are [C][H][W][B] (src/layers/conv_kernels.cpp:342-347).
  *   - arrays are fp32 unless an operator takes an element type (SO_F32, SO_F16, SO_BF16).
- *   - all arithmetic is fp32; every output element is produced by the same
- *     rounding sequence as the reference (bias first, then one fused
- *     multiply-add per stored nonzero in ascending slot order), except so_matvec
- *     whose in-row summation order differs (wave reduction) and is accurate to
- *     fp32 round-off.
+ *   - all arithmetic is fp32, but for the products and the sums of a block in
+ *     so_mxfp4_matmul, which are exact; every output element of an operator that stands in for one of the
+ *     reference's is produced by the same rounding sequence as there (bias first, then
+ *     one fused multiply-add per stored nonzero in ascending slot order), except so_matvec
+ *     and so_matmul on SO_LAYOUT_RBM, whose in-row summation order differs and which are
+ *     accurate to fp32 round-off.
  */
 #ifndef SPARSEOPS_HIP_H
 #define SPARSEOPS_HIP_H
