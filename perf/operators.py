@@ -11,7 +11,11 @@ is how many places longer the input's rows are than the batch.  `kind` says whic
   matmul      so_mxfp4_matmul: Y = act(W X + b), W kept in 4 bits, X quantised in blocks of 32 features within the call.
   matvec      so_mxfp4_matvec: y = W x + b, W kept in 4 bits, x as it is.
 
-With `own` false the same passes are made of elementary torch operations in 32 bits."""
+With `own` false the same passes are made of elementary torch operations in 32 bits.
+
+With `own` true a pass is queued on the context's own stream, with which torch's streams are not ordered.  `prepare` waits for
+what torch has to do ahead of it; whoever reads a pass's results, or writes into what a state holds, calls `finish()` before that
+(or waits for the whole device).  A state that is dropped waits by itself before its memory goes back to torch."""
 import math
 import os
 import sys
@@ -88,6 +92,22 @@ def context():
         import hipabi
         _context = hipabi.Context(0)
     return _context
+
+
+def finish():
+    """Waits until all passes made so far are done: their results can be read, their memory used for something else."""
+    if _context is not None:
+        _context.sync()
+
+
+class InUse:
+    """Held by a state, ahead of its tensors: passes over them may still be queued when the state is dropped."""
+
+    def __init__(self):
+        self.wait = finish
+
+    def __del__(self):
+        self.wait()
 
 
 class OnGpu:
@@ -191,7 +211,8 @@ def _inputs(case, seed):
 
 
 def prepare(case, seed):
-    s = _inputs(case, seed)
+    s = {"in_use": InUse()} if own else {}          # the first to go
+    s.update(_inputs(case, seed))
     kind, new = case["kind"], lambda *shape, type=torch.float32: torch.zeros(*shape, dtype=type, device="cuda")
     if own:
         if kind == "norm":
