@@ -14,10 +14,9 @@ namespace {
 // difference of large sums is taken, so a column far from zero keeps its variance.  The share is taken before the square: beside an empty set (mean 0) t is the column's own size, whose
 // square fp32 need not hold.
 struct Share { float to, sq; };      // nb / (na + nb), na nb / (na + nb)
-// The first of two is 1 where a is empty, which the hardware's reciprocal times nb need not be: a column of one value keeps it as its mean.
 __device__ __forceinline__ Share share_of(float na, float nb)
 {
-    const float to = na > 0.0f ? nb * __builtin_amdgcn_rcpf(na + nb) : nb > 0.0f ? 1.0f : 0.0f;
+    const float sum = na + nb, to = sum > 0.0f ? nb * __builtin_amdgcn_rcpf(sum) : 0.0f;
     return {to, na * to};
 }
 __device__ __forceinline__ void join(float2 &a, float2 b, Share s)
@@ -209,7 +208,13 @@ void norm_apply_kernel(uint32_t F, uint32_t B, uint32_t parts, uint32_t tiles, c
         const uint32_t first = at.tile * COLS;
         const Moments all = join_parts<COLS>(lds, first, B, parts, Moments{make_float2(0.0f, 0.0f), 0.0f},
                                              [&](uint32_t p, uint32_t c) { return Moments{cols[(size_t)p * B + c], (float)min(F - p * At::RS, (uint32_t)At::RS)}; },
-                                             [](Moments &a, const Moments &b) { join(a.s, b.s, share_of(a.n, b.n)); a.n += b.n; },
+                                             // The first part is taken as it is: the hardware's reciprocal of its rows times its rows need not be 1, and a column of one value keeps it
+                                             // as its mean.  (Lanes and waves hold the first rows of a tile first: none of those joined there is empty but the second.)
+                                             [](Moments &a, const Moments &b) {
+                                                 if (a.n > 0.0f) join(a.s, b.s, share_of(a.n, b.n));
+                                                 else a.s = b.s;
+                                                 a.n += b.n;
+                                             },
                                              [&] {
                                                  load_rows(at, ga, gamma, 1.0f);
                                                  load_rows(at, be, beta, 0.0f);
