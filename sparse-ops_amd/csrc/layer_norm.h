@@ -154,7 +154,7 @@ __device__ __forceinline__ void by_fullness(uint32_t tile, uint32_t B, F &&f)
     else f(std::false_type());
 }
 
-// Every thread takes each kThreads / COLS-th part of a column of the tile, take(part, column of B), and add(s, value) adds it to s; the shares of a column are added in the threads below
+// Every thread takes each kThreads / COLS-th part of a column of the tile, take(part, column of B), the first one as it is (s where there is none), and add(s, value) adds the others to it; the shares of a column are added in the threads below
 // COLS, which get the sum.  meanwhile() asks for other things once the first values are on their way.  `lds` holds kThreads values.
 template <int COLS, class Value, class Take, class Add, class Meanwhile>
 __device__ __forceinline__ Value join_parts(Value *lds, uint32_t first, uint32_t B, uint32_t parts, Value s, Take &&take, Add &&add, Meanwhile &&meanwhile)
@@ -171,8 +171,12 @@ __device__ __forceinline__ Value join_parts(Value *lds, uint32_t first, uint32_t
     };
     ask(share);
     meanwhile();
-    for (uint32_t p = share; p < end; p += 4u * SHARES) {
-        if (p != share) ask(p);
+    if (share < end) s = v[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+        if (share + i * SHARES < end) add(s, v[i]);
+    for (uint32_t p = share + 4u * SHARES; p < end; p += 4u * SHARES) {
+        ask(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (p + i * SHARES < end) add(s, v[i]);

@@ -208,13 +208,9 @@ void norm_apply_kernel(uint32_t F, uint32_t B, uint32_t parts, uint32_t tiles, c
         const uint32_t first = at.tile * COLS;
         const Moments all = join_parts<COLS>(lds, first, B, parts, Moments{make_float2(0.0f, 0.0f), 0.0f},
                                              [&](uint32_t p, uint32_t c) { return Moments{cols[(size_t)p * B + c], (float)min(F - p * At::RS, (uint32_t)At::RS)}; },
-                                             // The first part is taken as it is: the hardware's reciprocal of its rows times its rows need not be 1, and a column of one value keeps it
-                                             // as its mean.  (Lanes and waves hold the first rows of a tile first: none of those joined there is empty but the second.)
-                                             [](Moments &a, const Moments &b) {
-                                                 if (a.n > 0.0f) join(a.s, b.s, share_of(a.n, b.n));
-                                                 else a.s = b.s;
-                                                 a.n += b.n;
-                                             },
+                                             // (Of two joined none is empty but the second: a thread's first part is taken as it is, lanes and waves hold the first rows of a tile first.  Beside an
+                                             // empty first one the share would be the hardware's reciprocal of nb times nb, which need not be 1, and a column of one value not keep it as its mean.)
+                                             [](Moments &a, const Moments &b) { join(a.s, b.s, share_of(a.n, b.n)); a.n += b.n; },
                                              [&] {
                                                  load_rows(at, ga, gamma, 1.0f);
                                                  load_rows(at, be, beta, 0.0f);
