@@ -190,23 +190,51 @@ __device__ __forceinline__ Value join_parts(Value *lds, uint32_t first, uint32_t
 
 constexpr int kRows = 4;      // rows a thread holds of a part
 
+// Every workgroup that writes results joins the parts of its columns, which grow with the features as the workgroups do: where a thread would have more than kJoin of them, groups of as many
+// are joined to one each first, until it has not.  At once / in groups, us: fp32 40960 x 32, 40 parts a thread, 12.5 / 14.4 (groups of 32); 65536 x 32, 64 parts, 16.3 / 16.8; 65536 x 256 57 / 42;
+// 802816 x 32, 784 parts, 579 / 53, three times the matrix at a copy's rate 49.
+constexpr uint32_t kJoin = 48;
+constexpr uint32_t group_of(uint32_t columns) { return kJoin * (kThreads / columns); }
+
 // How [F x B] is cut: lanes of a row, tiles of columns, parts of the features.
 struct Cut {
-    uint32_t lanes, tiles, parts;
+    uint32_t lanes, tiles, parts, columns;      // columns of a tile
     uint64_t groups;
-    size_t cols_bytes, rows_bytes;
+    size_t cols_bytes, rows_bytes;              // cols: of the parts, behind them their groups
 };
 static inline Cut cut_of(int type, uint32_t F, uint32_t B)
 {
     const uint32_t V = 16u / (uint32_t)so_type_bytes(type);
     Cut c;
     c.lanes = B <= V ? 1 : B <= 2 * V ? 2 : B <= 4 * V ? 4 : 8;
-    c.tiles = so_ceil_div(B, c.lanes * V);
+    c.columns = c.lanes * V;
+    c.tiles = so_ceil_div(B, c.columns);
     c.parts = so_ceil_div(F, kThreads / c.lanes * kRows);
     c.groups = (uint64_t)c.tiles * c.parts;
-    c.cols_bytes = (size_t)c.parts * B * sizeof(float2);
+    c.cols_bytes = ((size_t)c.parts + (c.parts > group_of(c.columns) ? so_ceil_div(c.parts, group_of(c.columns)) : 0u)) * B * sizeof(float2);
     c.rows_bytes = (size_t)c.tiles * F * sizeof(float2);
     return c;
+}
+
+// What the workgroups that write results join: arrays of B, each of so many rows of X.
+struct Parts {
+    float2 *at;
+    uint32_t count, rows;
+};
+// The parts of a cut in cols, group by group by launch(workgroups, parts, their groups), until they are few enough.
+template <class F>
+Parts few_parts(const Cut &c, uint32_t features, uint32_t B, float2 *cols, F &&launch)
+{
+    const uint32_t group = group_of(c.columns);
+    Parts p = {cols, c.parts, std::min(features, kThreads / c.lanes * kRows)};
+    float2 *to = cols + (size_t)c.parts * B;
+    while (p.count > group) {
+        const Parts next = {to, so_ceil_div(p.count, group), (uint32_t)std::min<uint64_t>(features, (uint64_t)p.rows * group)};
+        launch(c.tiles * next.count, p, next.at);
+        to = p.at;
+        p = next;
+    }
+    return p;
 }
 
 template <class F>

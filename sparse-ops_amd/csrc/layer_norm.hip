@@ -190,13 +190,39 @@ void norm_parts_kernel(uint32_t F, uint32_t B, uint32_t tiles, const T *X, size_
     });
 }
 
+struct Moments { float2 s; float n; };
+// Those of a column over parts of `per` rows each, the last one fewer, from part `first` on.
+template <int COLS, class Meanwhile>
+__device__ __forceinline__ Moments join_moments(Moments *lds, uint32_t column, uint32_t F, uint32_t B, uint32_t first, uint32_t parts, uint32_t per, const float2 *__restrict__ cols,
+                                                Meanwhile &&meanwhile)
+{
+    return join_parts<COLS>(lds, column, B, parts, Moments{make_float2(0.0f, 0.0f), 0.0f},
+                            [&](uint32_t p, uint32_t c) { return Moments{cols[(size_t)(first + p) * B + c], (float)min(F - (first + p) * per, per)}; },
+                            // (Of two joined none is empty but the second: a thread's first part is taken as it is, lanes and waves hold the first rows of a tile first.  Beside an
+                            // empty first one the share would be the hardware's reciprocal of nb times nb, which need not be 1, and a column of one value not keep it as its mean.)
+                            [](Moments &a, const Moments &b) { join(a.s, b.s, share_of(a.n, b.n)); a.n += b.n; },
+                            meanwhile);
+}
+
+// A group of parts to one.
+template <int COLS>
+__global__ __launch_bounds__(kThreads)
+void norm_group_kernel(uint32_t F, uint32_t B, uint32_t parts, uint32_t per, uint32_t tiles, const float2 *__restrict__ cols, float2 *__restrict__ out)
+{
+    __shared__ Moments lds[kThreads];
+    const uint2 which = tile_and_part(tiles);
+    const uint32_t first = which.y * group_of(COLS);
+    const Moments all = join_moments<COLS>(lds, which.x * COLS, F, B, first, min(parts - first, group_of(COLS)), per, cols, [] {});
+    const uint64_t c = (uint64_t)which.x * COLS + threadIdx.x;
+    if (threadIdx.x < COLS && c < B) out[(size_t)which.y * B + c] = all.s;
+}
+
 template <class T, int LC, int RPT>
 __global__ __launch_bounds__(kThreads)
-void norm_apply_kernel(uint32_t F, uint32_t B, uint32_t parts, uint32_t tiles, const T *X, size_t ldx, const float2 *__restrict__ cols, const float *__restrict__ gamma,
+void norm_apply_kernel(uint32_t F, uint32_t B, uint32_t parts, uint32_t per, uint32_t tiles, const T *X, size_t ldx, const float2 *__restrict__ cols, const float *__restrict__ gamma,
                        const float *__restrict__ beta, float eps, T *Y, size_t ldy, float *__restrict__ mean_out, float *__restrict__ rstd_out)
 {
     constexpr int COLS = LC * so_elements<T>::V;
-    struct Moments { float2 s; float n; };
     __shared__ Moments lds[kThreads];
     __shared__ float2 st[COLS];
     const uint2 which = tile_and_part(tiles);
@@ -206,16 +232,11 @@ void norm_apply_kernel(uint32_t F, uint32_t B, uint32_t parts, uint32_t tiles, c
         typename so_elements<T>::plain x[RPT];
         float ga[RPT], be[RPT];
         const uint32_t first = at.tile * COLS;
-        const Moments all = join_parts<COLS>(lds, first, B, parts, Moments{make_float2(0.0f, 0.0f), 0.0f},
-                                             [&](uint32_t p, uint32_t c) { return Moments{cols[(size_t)p * B + c], (float)min(F - p * At::RS, (uint32_t)At::RS)}; },
-                                             // (Of two joined none is empty but the second: a thread's first part is taken as it is, lanes and waves hold the first rows of a tile first.  Beside an
-                                             // empty first one the share would be the hardware's reciprocal of nb times nb, which need not be 1, and a column of one value not keep it as its mean.)
-                                             [](Moments &a, const Moments &b) { join(a.s, b.s, share_of(a.n, b.n)); a.n += b.n; },
-                                             [&] {
-                                                 load_rows(at, ga, gamma, 1.0f);
-                                                 load_rows(at, be, beta, 0.0f);
-                                                 at.load(x, X, ldx);
-                                             });
+        const Moments all = join_moments<COLS>(lds, first, F, B, 0, parts, per, cols, [&] {
+            load_rows(at, ga, gamma, 1.0f);
+            load_rows(at, be, beta, 0.0f);
+            at.load(x, X, ldx);
+        });
         if (threadIdx.x < COLS) {
             const float2 of = st[threadIdx.x] = results_of(all.s, F, eps);
             const uint64_t c = (uint64_t)first + threadIdx.x;
@@ -354,8 +375,11 @@ extern "C" so_status so_layer_norm(so_ctx *ctx, int type, uint32_t F, uint32_t B
         for_lanes(c.lanes, [&](auto lanes) {
             constexpr int LC = decltype(lanes)::value;
             norm_parts_kernel<T, LC, kRows><<<(uint32_t)c.groups, kThreads, 0, ctx->stream>>>(F, B, c.tiles, (const T *)dX, x_stride, cols);
-            norm_apply_kernel<T, LC, kRows><<<(uint32_t)c.groups, kThreads, 0, ctx->stream>>>(F, B, c.parts, c.tiles, (const T *)dX, x_stride, cols, dGamma, dBeta, eps, (T *)dY, y_stride,
-                                                                                               dMean, dRstd);
+            const Parts p = few_parts(c, F, B, cols, [&](uint32_t workgroups, const Parts &from, float2 *to) {
+                norm_group_kernel<LC * so_elements<T>::V><<<workgroups, kThreads, 0, ctx->stream>>>(F, B, from.count, from.rows, c.tiles, from.at, to);
+            });
+            norm_apply_kernel<T, LC, kRows><<<(uint32_t)c.groups, kThreads, 0, ctx->stream>>>(F, B, p.count, p.rows, c.tiles, (const T *)dX, x_stride, p.at, dGamma, dBeta, eps, (T *)dY,
+                                                                                               y_stride, dMean, dRstd);
         });
     });
     SO_LAUNCH_CHECK();

@@ -172,6 +172,27 @@ void norm_grad_parts_kernel(uint32_t F, uint32_t B, uint32_t tiles, const T *X, 
     });
 }
 
+// The sums of a column over parts, from part `first` on.
+template <int COLS, class Meanwhile>
+__device__ __forceinline__ float2 join_sums(float2 *lds, uint32_t column, uint32_t B, uint32_t first, uint32_t parts, const float2 *__restrict__ cols, Meanwhile &&meanwhile)
+{
+    return join_parts<COLS>(lds, column, B, parts, make_float2(0.0f, 0.0f), [&](uint32_t p, uint32_t c) { return cols[(size_t)(first + p) * B + c]; },
+                            [](float2 &a, float2 b) { a.x += b.x; a.y += b.y; }, meanwhile);
+}
+
+// A group of parts to one.
+template <int COLS>
+__global__ __launch_bounds__(kThreads)
+void norm_grad_group_kernel(uint32_t B, uint32_t parts, uint32_t tiles, const float2 *__restrict__ cols, float2 *__restrict__ out)
+{
+    __shared__ float2 lds[kThreads];
+    const uint2 which = tile_and_part(tiles);
+    const uint32_t first = which.y * group_of(COLS);
+    const float2 all = join_sums<COLS>(lds, which.x * COLS, B, first, min(parts - first, group_of(COLS)), cols, [] {});
+    const uint64_t c = (uint64_t)which.x * COLS + threadIdx.x;
+    if (threadIdx.x < COLS && c < B) out[(size_t)which.y * B + c] = all;
+}
+
 // dx of a part and a tile; the workgroups behind those join the rows' sums over the tiles.
 template <class T, int LC, int RPT>
 __global__ __launch_bounds__(kThreads)
@@ -190,12 +211,10 @@ void norm_grad_apply_kernel(uint32_t F, uint32_t B, uint32_t parts, uint32_t til
         const Place<T, LC, RPT, kThreads, decltype(full)::value> at(F, B, which.x, which.y);
         typename so_elements<T>::plain x[RPT], dy[RPT];
         float ga[RPT];
-        const float2 all = join_parts<COLS>(lds, at.tile * COLS, B, parts, make_float2(0.0f, 0.0f), [&](uint32_t p, uint32_t c) { return cols[(size_t)p * B + c]; },
-                                            [](float2 &a, float2 b) { a.x += b.x; a.y += b.y; },
-                                            [&] {
-                                                load_rows(at, ga, gamma, 1.0f);
-                                                at.load(x, dy, X, ldx, Dy, lddy);
-                                            });
+        const float2 all = join_sums<COLS>(lds, at.tile * COLS, B, 0, parts, cols, [&] {
+            load_rows(at, ga, gamma, 1.0f);
+            at.load(x, dy, X, ldx, Dy, lddy);
+        });
         if (threadIdx.x < COLS) joined[threadIdx.x] = make_float2(all.x / (float)F, all.y / (float)F);
         __syncthreads();
         const Columns<V> c(mean, rstd, at.c0, at.left);
@@ -289,7 +308,7 @@ extern "C" so_status so_layer_norm_grad(so_ctx *ctx, int type, uint32_t F, uint3
         return SO_OK;
     }
     if (const so_status s = workspace(ctx, "so_layer_norm_grad", so_norm_grad_bytes(ctx, type, F, B)); s != SO_OK) return s;
-    float2 *cols = (float2 *)ctx->mm_part->p, *rows = params ? cols + (size_t)c.parts * B : nullptr;
+    float2 *cols = (float2 *)ctx->mm_part->p, *rows = params ? cols + c.cols_bytes / sizeof(float2) : nullptr;
     const uint32_t workers = dDx ? (uint32_t)c.groups : 0, joiners = params ? so_ceil_div(F, 16) : 0;
     so_for_type(type, [&](auto t) {
         using T = decltype(t);
@@ -297,8 +316,13 @@ extern "C" so_status so_layer_norm_grad(so_ctx *ctx, int type, uint32_t F, uint3
             constexpr int LC = decltype(lanes)::value;
             norm_grad_parts_kernel<T, LC, kRows><<<(uint32_t)c.groups, kThreads, 0, ctx->stream>>>(F, B, c.tiles, (const T *)dX, x_stride, (const T *)dDy, dy_stride, dGamma, dMean,
                                                                                                     dRstd, dDx ? cols : nullptr, rows);
-            norm_grad_apply_kernel<T, LC, kRows><<<workers + joiners, kThreads, 0, ctx->stream>>>(F, B, c.parts, c.tiles, workers, (const T *)dX, x_stride, (const T *)dDy, dy_stride,
-                                                                                                   dGamma, dMean, dRstd, cols, rows, (T *)dDx, dx_stride, dDgamma, dDbeta);
+            Parts p = {cols, c.parts, 0};
+            if (dDx)
+                p = few_parts(c, F, B, cols, [&](uint32_t workgroups, const Parts &from, float2 *to) {
+                    norm_grad_group_kernel<LC * so_elements<T>::V><<<workgroups, kThreads, 0, ctx->stream>>>(B, from.count, c.tiles, from.at, to);
+                });
+            norm_grad_apply_kernel<T, LC, kRows><<<workers + joiners, kThreads, 0, ctx->stream>>>(F, B, p.count, c.tiles, workers, (const T *)dX, x_stride, (const T *)dDy, dy_stride,
+                                                                                                   dGamma, dMean, dRstd, p.at, rows, (T *)dDx, dx_stride, dDgamma, dDbeta);
         });
     });
     SO_LAUNCH_CHECK();

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import hipabi
-from elements import TYPES, U, fetch, place, stored, values
+from elements import HALF_STEP, SMALLEST, TYPES, U, fetch, place, stored, values
 from test_gpu_layer_norm import EPS, check_forward, check_grad, check_statistics, problem, statistics
 
 pytestmark = pytest.mark.gpu
@@ -128,3 +128,65 @@ def test_forced_tiles_that_a_launch_does_not_hold(ctx):
             ctx.layer_norm(a, 1, 1 << 28, None, None, EPS, a)
     assert e.value.status == hipabi.SO_ERR_INVALID
     a.free()
+
+
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+@pytest.mark.parametrize("F,B", [(300000, 33), (100352, 8), (1000003, 1), (1 << 18, 200)])
+def test_very_many_features(ctx, F, B, type_):
+    """The features of whole images.  A column's parts are 1024 / lanes rows; 256 / columns threads join up to 48 of them each, one after the other, and one thread what these have, first in
+    groups where there are more: so many additions more than test_gpu_layer_norm.py counts, up to the 48 that stand for all there."""
+    V = 4 if type_ == "f32" else 8
+    lanes = 8 if B > 4 * V else 4 if B > 2 * V else 2 if B > V else 1
+    shares, parts, more = 256 // (lanes * V), -(-F * lanes // 1024), 0
+    while parts > 48 * shares:
+        parts, more = -(-parts // (48 * shares)), more + 48 + shares
+    more += 48 + shares
+    rng, X, gamma, beta = problem(F, B, type_, seed=5)
+    dY = values(stored(0.1 * rng.standard_normal((F, B)), type_), type_)
+    dX, dDy, out, dDx = (place(ctx, M, type_)[0] for M in (X, dY, np.zeros((F, B)), np.zeros((F, B))))
+    dG, dB, dM, dR, dDg, dDb = ctx.array(gamma), ctx.array(beta), ctx.empty((B,)), ctx.empty((B,)), ctx.empty((F,)), ctx.empty((F,))
+    ctx.layer_norm(dX, F, B, dG, dB, EPS, out, dM, dR, type=type_)
+    ctx.layer_norm_grad(dX, dDy, F, B, dG, dM, dR, dDx, dDg, dDb, type=type_)
+    mean, rstd = statistics(X)
+    h = (X - mean) * rstd
+    n = (48 + more) * U
+    off = n * np.abs(X).max(axis=0)
+    g_mean, g_rstd = dM.download().astype(np.float64), dR.download().astype(np.float64)
+    assert np.all(np.abs(g_mean - mean) <= off)
+    assert np.all(np.abs(g_rstd - rstd) <= rstd * (n + np.square(off * rstd)))
+    g = gamma.astype(np.float64)[:, None]
+    want = h * g + beta.astype(np.float64)[:, None]
+    tol = n * (np.abs(X).max(axis=0) * rstd * np.abs(g) + np.abs(h * g)) + 2 * U * np.abs(want) + HALF_STEP[type_] * np.abs(want) + SMALLEST[type_]
+    assert np.all(np.abs(fetch(out, F, B, type_)[0] - want) <= tol)
+    h = (X - g_mean) * g_rstd
+    dyg = dY * g
+    a, b = dyg.mean(axis=0), (dyg * h).mean(axis=0)
+    want = g_rstd * (dyg - a - h * b)
+    tol = g_rstd * (n * (np.abs(dyg).mean(axis=0) + np.abs(h) * np.abs(dyg * h).mean(axis=0)) + 8 * U * (np.abs(dyg) + np.abs(a) + np.abs(h * b))) + HALF_STEP[type_] * np.abs(want) + SMALLEST[type_]
+    assert np.all(np.abs(fetch(dDx, F, B, type_)[0] - want) <= tol)
+    assert np.all(np.abs(dDg.download() - (dY * h).sum(axis=1)) <= 48 * U * np.abs(dY * h).sum(axis=1) + 1e-40)
+    assert np.all(np.abs(dDb.download() - dY.sum(axis=1)) <= 48 * U * np.abs(dY).sum(axis=1) + 1e-40)
+    for t in (dX, dDy, out, dDx, dG, dB, dM, dR, dDg, dDb):
+        t.free()
+
+
+@pytest.mark.parametrize("gradient", [False, True])
+def test_time_grows_as_the_features_do(ctx, gradient):
+    """Four times the features take about four times as long: what a workgroup joins does not grow with them, which would make it sixteen times."""
+    B, times = 32, []
+    for F in (1 << 20, 1 << 22):
+        dX, dM, dR, dDg = ctx.empty((F, B)), ctx.empty((B,)), ctx.empty((B,)), ctx.empty((F,))
+        for a in (dX, dM, dR):
+            ctx.fill_zero(a)
+        took = []
+        for _ in range(4):
+            ctx.timer_begin()
+            if gradient:
+                ctx.layer_norm_grad(dX, dX, F, B, None, dM, dR, dX, dDg, None)
+            else:
+                ctx.layer_norm(dX, F, B, None, None, EPS, dX, dM, dR)
+            took.append(ctx.timer_end())
+        times.append(min(took))
+        for a in (dX, dM, dR, dDg):
+            a.free()
+    assert times[1] <= 8 * times[0], times
