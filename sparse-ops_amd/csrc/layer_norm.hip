@@ -122,8 +122,8 @@ __device__ __forceinline__ void write_rows(const Place<T, LC, RPT, NT, FULL> &at
 }
 
 // All features of a tile of columns in one workgroup's registers: X is read once.  The tiles go to the XCDs in runs of neighbours, which share cache lines where LC is less than 8.
-// Bound by the memory where there are tiles enough, in three phases that do not overlap, since a compute unit holds one large tile: 4096 x 8192 bf16 34.5 us, 3.9 TB/s (a copy 24); by latencies
-// where not: 4096 x 1 fp32 5.2 us.
+// Bound by the memory where there are tiles enough, in three phases that do not overlap, since a compute unit holds one large tile: 4096 x 8192 bf16 34.5 us, 3.9 TB/s (a copy 21); by instructions
+// where not: 4096 x 1 fp32 5.2 us, of which the 520 vector instructions of each of 16 waves on four SIMDs take 3.5, most of them joins of four columns, three of which do not exist.
 template <class T, int LC, int RPT, int NT>
 __global__ __launch_bounds__(NT)
 void norm_whole_kernel(uint32_t F, uint32_t B, uint32_t tiles, uint32_t per_xcd, const T *X, size_t ldx, const float *__restrict__ gamma, const float *__restrict__ beta, float eps, T *Y,
@@ -267,7 +267,7 @@ Whole whole_of(const so_ctx *ctx, int type, uint32_t F, uint32_t B)
     const uint32_t per = F * lanes;                               // threads at a row each
     const bool few = so_ceil_div(B, lanes * V) < cus;
     // One launch and one reading against two: it is the slower one only where long columns leave most compute units without a tile or give them 16 bytes of a row each (a cache line a
-    // row and workgroup, in and out).  Whole / in parts, us: fp32 1024 x 1024 6.0 / 6.4, 8192 x 1 6.7 / 7.2, 4096 x 256 9.8 / 6.6, 4096 x 1024 17 / 11, 4096 x 4096 23 / 34; bf16 512 x 1024
+    // row and workgroup, in and out).  Whole / in parts, us, on one X that stays in the caches where they hold it: fp32 1024 x 1024 6.0 / 6.4, 8192 x 1 6.7 / 7.2, 4096 x 256 9.8 / 6.6, 4096 x 1024 17 / 11, 4096 x 4096 23 / 34; bf16 512 x 1024
     // 4.7 / 6.4, 1024 x 1024 7.6 / 6.6, 2048 x 16 6.8 / 6.6, 4096 x 1 8.3 / 7.5, 2048 x 16384 25 / 39, 8192 x 4096 34 / 40.
     if (lanes == 1 && F * V * V > 131072) return {0, 0, 0};
     if (asked < 0 && (few || lanes == 1) && F * V > 4096 && (uint64_t)F * B > 65536) return {0, 0, 0};

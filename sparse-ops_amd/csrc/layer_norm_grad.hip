@@ -3,11 +3,12 @@
 //   dx = rstd (g - sum_f g / F - h sum_f (g h) / F),  dgamma_f = sum_b dy h,  dbeta_f = sum_b dy
 //
 // dx needs two sums down every column, dgamma and dbeta two sums along every row; 1 / deviation is taken out of the former.  A batch of a few columns is one workgroup's, in one launch.
-// Otherwise two launches cut the matrix into tiles of 128 bytes a row and parts of 128 features (256 with fewer lanes a row): the first takes the sums of a tile and a part, the second
-// adds a tile's parts and writes dx, and its last workgroups add a row's tiles.  All sums are taken in the same order on every call: no atomics.
+// Otherwise two launches cut the matrix into tiles of 1, 2, 4 or 8 lanes of 16 bytes a row and parts of 1024, 512, 256 or 128 features: the first takes the sums of a tile and a part, the
+// second adds a tile's parts and writes dx, and its last workgroups add a row's tiles.  All sums are taken in the same order on every call: no atomics.
 //
 // What bounds it: X and dY come twice, since a workgroup's registers do not hold a tile's columns; 4096 x 8192 bf16 takes 67 us, 34.6 + 33.8, where the 335 MB that it then moves take
-// 60 at a large copy's rate (36 for one reading).  The second launch runs at that rate, the first, all reading, at 3.9 TB/s: its 16 vector instructions an element are 14 us of it.
+// 53 at a large copy's rate of 6.35 TB/s (32 for one reading).  The second launch runs at 6 TB/s, the first, all reading, at 3.9: its 21 vector instructions an element are 18 us of it.  More
+// than a third of them are sums over lanes and the way out, once for every four rows of a thread.
 #include "layer_norm.h"
 
 using namespace so_norm;
@@ -229,7 +230,7 @@ void norm_grad_apply_kernel(uint32_t F, uint32_t B, uint32_t parts, uint32_t til
     });
 }
 
-// One workgroup for everything: lanes of a row, rows a thread, threads.  None: lanes 0.  In one workgroup / in parts, us: fp32 64 x 1 3.3 / 5.7, 2048 x 1 5.7 / 7.5, 256 x 16 4.7 / 5.9,
+// One workgroup for everything: lanes of a row, rows a thread, threads.  None: lanes 0.  In one workgroup / in parts, us, on one X and dY that stay in the caches: fp32 64 x 1 3.3 / 5.7, 2048 x 1 5.7 / 7.5, 256 x 16 4.7 / 5.9,
 // 1024 x 16 6.4 / 6.3; bf16 256 x 16 4.4 / 6.0, 1024 x 1 7.7 / 9.0, 784 x 16 7.6 / 7.1.  (With all features held for any batch, one reading instead of two, a workgroup for every tile
 // of 32 bytes a row took longer than the two launches: 4096 x 8192 bf16 93 us, 67 in parts: each cache line goes to four compute units, and nothing is loaded while a tile is worked on.)
 struct One { uint32_t lanes, rows, threads; };

@@ -47,8 +47,8 @@ __device__ __forceinline__ MxTile mx_tile_of(uint32_t mgroups, uint32_t cgroups,
 }
 
 // A tile of Y of 16 MH x 16 CH, WK waves that share the blocks between them, a unit of 8 each in turn, straight from memory to registers; their sums meet in LDS.
-// Bound by the caches, which bring a workgroup (rows + columns) n / 2 bytes, and by the chain of first loads, sums and stores: 4096 x 4096 x 256 fp32 on 64 x 64 8.4 us (17 MB from memory, 71
-// from the L2s), 3001 x 2777 x 101 fp16 on 32 x 32 5.1.
+// Bound by the caches, which bring a workgroup (rows + columns) n / 2 bytes, and by loads that the products wait for: 4096 x 4096 x 256 fp32 on 64 x 64 8.4 us (17 MB from memory, 71 from the
+// L2s and half as much again for units that are asked for twice), 3001 x 2777 x 101 fp16 on 32 x 32 5.1.
 template <class T, int MH, int CH, int WK, int ACT>
 __global__ __launch_bounds__(64 * WK)
 void mx_matmul_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restrict__ Ws, const so_u32x4 *__restrict__ Xc, const uint32_t *__restrict__ Xs, uint32_t m, uint32_t C,
@@ -105,7 +105,8 @@ void mx_matmul_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restric
             });
         });
     };
-    // two units at a time, the next on its way while one is multiplied; behind the last one that one again
+    // Two units in registers; behind the last one that one again, for nothing (a third of the loads where a wave has two units).  As compiled, a unit's loads are asked for behind most of
+    // the products of the one before it, not ahead of them, so that little of their way is hidden.
     const uint32_t turns = wave < units ? (units - wave + WK - 1u) / WK : 0u;
     if (turns) {
         const uint32_t last = wave + (turns - 1u) * WK;
@@ -433,7 +434,8 @@ void mx_matvec_kernel(const so_u32x4 *__restrict__ Wc, const uint32_t *__restric
     };
     for (uint32_t u0 = 0; u0 < units; u0 += CU) {
         const uint32_t here = min(units - u0, CU), turns = wave < here ? (here - wave + WAVES - 1u) / WAVES : 0u;
-        // two units at a time, the next on its way while one is multiplied, the first ones also while x is; behind the last one that one again
+        // Two units in registers, the first ones on their way while x is; behind the last one that one again, for nothing.  As compiled, the next two are asked for together behind the products
+        // of both, and waited for in part at the next turn's beginning.
         const uint32_t last = wave + (turns ? turns - 1u : 0u) * WAVES;
         Unit a, b;
         if (turns) {

@@ -23,7 +23,8 @@
 // bits.  Larger fully connected layers add a row's products in another order (within 1e-5 of the largest output,
 // measured 1e-6), which also depends on the batch, so a sample's bits do -- in every model without convolutions, and in
 // one with convolutions that is loaded at a batch of 64 or more.  SPARSEOPS_MATMUL_RBM=0 in the environment at load
-// time keeps the reference's bits everywhere.
+// time keeps the reference's bits everywhere.  LayerNormalization, which the reference does not have, adds in an order
+// that depends on the batch too.
 #pragma once
 
 #include <cstddef>

@@ -529,7 +529,7 @@ SparseOnnxModel::SparseOnnxModel(const std::string &onnx_path) : impl_(new Impl(
     // So does a model with convolutions that is loaded at a batch below 64, whatever batch it is resized to later: its
     // samples have the same bits in every batch, and its classifier is a few microseconds of the pass.  Loaded at 64 or
     // more it keeps the fast layers at every batch, and a sample's bits then depend on the batch (the kernel is chosen
-    // by launch), as they do in a model without convolutions.
+    // by launch), as they do in a model without convolutions and, whatever its batch, in one with LayerNormalization.
     bool convs = false;
     for (const auto &p : pend) convs = convs || p.plan.op == Op::Conv;
     const bool fast_fc = !(rbm_env && rbm_env[0] == '0') && !(convs && B0 < 64);
