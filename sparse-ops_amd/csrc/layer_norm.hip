@@ -34,9 +34,10 @@ __device__ __forceinline__ float2 results_of(float2 all, uint32_t F, float eps)
     return make_float2(all.x + none, 1.0f / sqrtf(all.y / (float)F + eps) + none);
 }
 
-// done(column of the tile, its mean and sum of squared deviations over the rows of the workgroup), in one thread for each column: a thread's own rows first, in one pass as
-// they come, as differences from the first of them, then the rows of a wave pair by pair, then the waves.  A thread holds 32 rows at most, and the value that it counts from is one
-// of them: the squares that cancel are at most as many times what is left, so the sum keeps all but 5 of its bits wherever the column lies and whatever sticks out of it.  `lds` holds NT / 64 * LC * V values.
+// done(column of the tile, its mean and sum of squared deviations over the rows of the workgroup), in one thread for each column: a thread's own rows first, their mean in one pass as
+// they come, as differences from the first of them, then the deviations from it out of the registers; then the rows of a wave pair by pair, then the waves.  (Squares of the differences
+// from the first row in the same pass, less the share of its own, cancel where that row sticks out: 4096 x 4096 fp32 32.3 us instead of 32.8, 2048 x 16384 bf16 28.2 instead of 29.1,
+// and 1 / deviation off by up to 350 roundings where one feature carries a column; 21 now.)  `lds` holds NT / 64 * LC * V values.
 template <class T, int LC, int RPT, int NT, bool FULL, class Done>
 __device__ __forceinline__ void tile_moments(const Place<T, LC, RPT, NT, FULL> &at, typename so_elements<T>::plain (&x)[RPT], float2 *lds, Done &&done)
 {
@@ -54,17 +55,21 @@ __device__ __forceinline__ void tile_moments(const Place<T, LC, RPT, NT, FULL> &
     for (int k = 1; k < RPT; ++k)
         if (at.in(k))
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float t = (float)x[k][e] - from[e];
-                s[e].x += t;
-                s[e].y = fmaf(t, t, s[e].y);
-            }
+            for (int e = 0; e < V; ++e) s[e].x += (float)x[k][e] - from[e];
     const float per = n > 0.0f ? 1.0f / n : 0.0f;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const float off = s[e].x * per, q = fmaf(-s[e].x, off, s[e].y);
-        s[e] = make_float2(from[e] + off, q < 0.0f ? 0.0f : q);                      // NaN stays
-    }
+    for (int e = 0; e < V; ++e) from[e] = s[e].x = fmaf(s[e].x, per, from[e]);
+    if constexpr (V == 8)
+#pragma unroll
+        for (int k = 0; k < RPT; ++k) so_group_afresh(x[k]);
+#pragma unroll
+    for (int k = 0; k < RPT; ++k)
+        if (at.in(k))
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float t = (float)x[k][e] - from[e];
+                s[e].y = fmaf(t, t, s[e].y);
+            }
     if constexpr (V == 8)
 #pragma unroll
         for (int k = 0; k < RPT; ++k) so_group_afresh(x[k]);

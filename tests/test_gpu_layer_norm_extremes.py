@@ -190,3 +190,20 @@ def test_time_grows_as_the_features_do(ctx, gradient):
         for a in (dX, dM, dR, dDg):
             a.free()
     assert times[1] <= 8 * times[0], times
+
+
+@pytest.mark.parametrize("lanes", LANES)
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("F,B", [(257, 40), (2000, 64), (4096, 700), (8192, 33)])
+def test_one_feature_that_carries_a_column(ctx, F, B, type_, lanes):
+    """A value of 10 to 30000 in one of the first rows or another, beside normal values or zeros: its squares are not taken off each other, so the tolerances are those of any column."""
+    rng, _, gamma, beta = problem(F, B, type_)
+    for quiet in (0.0, 1e-3, 1.0):
+        X = quiet * rng.standard_normal((F, B))
+        row = rng.integers(0, F, B)
+        row[::2] = rng.integers(0, min(F, 64), row[::2].size)
+        X[row, np.arange(B)] = 10 ** rng.uniform(1, 4.4, B)
+        X = values(stored(X, type_), type_)
+        Y, mean, rstd = forward(ctx, X, gamma, beta, type_, lanes)
+        check_statistics(mean, rstd, X)
+        check_forward(Y, X, gamma, beta, type_)
