@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import hipabi
-from elements import HALF_STEP, SMALLEST, TYPES, U, fetch, place, stored, values
+from elements import HALF_STEP, SMALLEST, STORAGE, TYPES, U, fetch, place, stored, values
 from test_gpu_layer_norm import EPS, check_forward, check_grad, check_statistics, problem, statistics
 
 pytestmark = pytest.mark.gpu
@@ -207,3 +207,50 @@ def test_one_feature_that_carries_a_column(ctx, F, B, type_, lanes):
         Y, mean, rstd = forward(ctx, X, gamma, beta, type_, lanes)
         check_statistics(mean, rstd, X)
         check_forward(Y, X, gamma, beta, type_)
+
+
+@pytest.mark.parametrize("type_,F,B", [("f32", 3300007, 1), ("bf16", 1700003, 5), ("f32", 900001, 7), ("f32", 210001, 12), ("f16", 4800011, 33)])
+def test_groups_of_parts(ctx, type_, F, B):
+    """Groups of parts for every number of columns a tile, the last two times over (37501 parts, 196 groups of 192, 2): rows that repeat every 1009, whose statistics are those of so many times
+    each.  Tolerances as in test_very_many_features, of 2 (48 + 64) additions and the 48 there."""
+    P = 1009
+    rng = np.random.default_rng(F)
+    base = values(stored(rng.standard_normal((P, B)) + 0.5, type_), type_)
+    often = np.bincount(np.arange(F) % P, minlength=P).astype(np.float64)[:, None]
+    whole = np.arange(F) % P
+    gamma, dY = (1 + 0.2 * rng.standard_normal(P)).astype(np.float32), values(stored(0.1 * rng.standard_normal((P, B)), type_), type_)
+    dX, dDy = ctx.array(stored(base, type_)[whole], STORAGE[type_]), ctx.array(stored(dY, type_)[whole], STORAGE[type_])
+    out, dDx = ctx.empty((F, B), STORAGE[type_]), ctx.empty((F, B), STORAGE[type_])
+    dG, dM, dR, dDg, dDb = ctx.array(gamma[whole]), ctx.empty((B,)), ctx.empty((B,)), ctx.empty((F,)), ctx.empty((F,))
+    ctx.layer_norm(dX, F, B, dG, None, EPS, out, dM, dR, type=type_)
+    ctx.layer_norm_grad(dX, dDy, F, B, dG, dM, dR, dDx, dDg, dDb, type=type_)
+    n = U * (48 + 2 * (48 + 64))
+    mean = (base * often).sum(axis=0) / F
+    rstd = 1.0 / np.sqrt((np.square(base - mean) * often).sum(axis=0) / F + np.float64(np.float32(EPS)))
+    off = n * np.abs(base).max(axis=0)
+    g_mean, g_rstd = dM.download().astype(np.float64), dR.download().astype(np.float64)
+    assert np.all(np.abs(g_mean - mean) <= off)
+    assert np.all(np.abs(g_rstd - rstd) <= rstd * (n + np.square(off * rstd)))
+
+    def check(array, want, tol):
+        """A row of every repetition, most of them taken together: the largest and the smallest of each."""
+        got = values(array.download(), type_) if array.shape == (F, B) else array.download().astype(np.float64).reshape(F, 1)
+        low, high = got[:P].copy(), got[:P].copy()
+        for at in range(P, F, P):
+            part = got[at:at + P]
+            np.minimum(low[:len(part)], part, out=low[:len(part)])
+            np.maximum(high[:len(part)], part, out=high[:len(part)])
+        assert np.all(np.abs(low - want) <= tol) and np.all(np.abs(high - want) <= tol)
+
+    h, g = (base - mean) * rstd, gamma.astype(np.float64)[:, None]
+    check(out, h * g, n * (np.abs(base).max(axis=0) * rstd * np.abs(g) + np.abs(h * g)) + (2 * U + HALF_STEP[type_]) * np.abs(h * g) + SMALLEST[type_])
+    h = (base - g_mean) * g_rstd
+    dyg = dY * g
+    a, b = (dyg * often).sum(axis=0) / F, (dyg * h * often).sum(axis=0) / F
+    want = g_rstd * (dyg - a - h * b)
+    mags = (np.abs(dyg) * often).sum(axis=0) / F + np.abs(h) * (np.abs(dyg * h) * often).sum(axis=0) / F
+    check(dDx, want, g_rstd * (n * mags + 8 * U * (np.abs(dyg) + np.abs(a) + np.abs(h * b))) + HALF_STEP[type_] * np.abs(want) + SMALLEST[type_])
+    check(dDg, (dY * h).sum(axis=1, keepdims=True), 48 * U * np.abs(dY * h).sum(axis=1, keepdims=True) + 1e-40)
+    check(dDb, dY.sum(axis=1, keepdims=True), 48 * U * np.abs(dY).sum(axis=1, keepdims=True) + 1e-40)
+    for t in (dX, dDy, out, dDx, dG, dM, dR, dDg, dDb):
+        t.free()
