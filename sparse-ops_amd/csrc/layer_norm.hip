@@ -36,7 +36,7 @@ __device__ __forceinline__ float2 results_of(float2 all, uint32_t F, float eps)
 
 // done(column of the tile, its mean and sum of squared deviations over the rows of the workgroup), in one thread for each column: a thread's own rows first, their mean in one pass as
 // they come, as differences from the first of them, then the deviations from it out of the registers; then the rows of a wave pair by pair, then the waves.  (Squares of the differences
-// from the first row in the same pass, less the share of its own, cancel where that row sticks out: 4096 x 4096 fp32 32.3 us instead of 32.8, 2048 x 16384 bf16 28.2 instead of 29.1,
+// from the first row in the same pass, less the share of its own, cancel where that row sticks out: 4096 x 8192 bf16 34.8 us instead of 35.6, 4096 x 4096 fp32 32.3 instead of 32.8,
 // and 1 / deviation off by up to 350 roundings where one feature carries a column; 21 now.)  `lds` holds NT / 64 * LC * V values.
 template <class T, int LC, int RPT, int NT, bool FULL, class Done>
 __device__ __forceinline__ void tile_moments(const Place<T, LC, RPT, NT, FULL> &at, typename so_elements<T>::plain (&x)[RPT], float2 *lds, Done &&done)
@@ -127,8 +127,8 @@ __device__ __forceinline__ void write_rows(const Place<T, LC, RPT, NT, FULL> &at
 }
 
 // All features of a tile of columns in one workgroup's registers: X is read once.  The tiles go to the XCDs in runs of neighbours, which share cache lines where LC is less than 8.
-// Bound by the memory where there are tiles enough, in three phases that do not overlap, since a compute unit holds one large tile: 4096 x 8192 bf16 34.5 us, 3.9 TB/s (a copy 21); by instructions
-// where not: 4096 x 1 fp32 5.2 us, of which the 520 vector instructions of each of 16 waves on four SIMDs take 3.5, most of them joins of four columns, three of which do not exist.
+// Bound by the memory where there are tiles enough, in three phases that do not overlap, since a compute unit holds one large tile: 4096 x 8192 bf16 35.6 us, 3.8 TB/s (a copy 21); by instructions
+// where not: 4096 x 1 fp32 5.3 us, of which the 530 vector instructions of each of 16 waves on four SIMDs take 3.5, most of them joins of four columns, three of which do not exist.
 template <class T, int LC, int RPT, int NT>
 __global__ __launch_bounds__(NT)
 void norm_whole_kernel(uint32_t F, uint32_t B, uint32_t tiles, uint32_t per_xcd, const T *X, size_t ldx, const float *__restrict__ gamma, const float *__restrict__ beta, float eps, T *Y,
