@@ -1,4 +1,4 @@
-"""Gated feed-forward blocks and low-rank adapters as a user of the framework calls them: what is timed and compared.
+"""Gated feed-forward blocks, low-rank adapters and rotary positions as a user of the framework calls them: what is timed and compared.
 
 Every case is one pass through an entry point of the C ABI, by its ctypes binding (`hipabi.Context`), on operands that lie in
 device memory.  Activations are [features x batch] with the batch contiguous, as in the framework's layer chain, a column
@@ -8,6 +8,9 @@ being a token; `pad` is how many places longer the input's rows are than the bat
               the two sums as well, which the gradient takes, `add` says that there are G0 and U0 (what adapters make of X).
   gated_grad  so_gated_grad: the gradients of X, Wg and Wu from that of H and the saved sums.
   adapters    so_adapters: Y = base + scale_a B_a (A_a X), a the adapter that each column's request has, if it has one.
+  rotary      so_head_rotary: every head of a column's queries and keys over the root of its mean square (if `norm`), times a gain per
+              feature, and turned by the column's position; `save` asks for the norms' factors, which the gradient takes.
+  rotary_grad so_head_rotary_grad: the gradients of the input and of both gains.
 
 With `own` false the same passes are made of elementary torch operations in 32 bits.
 
@@ -24,13 +27,13 @@ own = False
 
 TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 BYTES = {"f32": 4, "f16": 2, "bf16": 2}
+EPS = 1e-6
+AMPLITUDE = 1.1                # of turned features, as scalings for long contexts have it
 ACTS = ("silu", "gelu", "gelu_tanh", "relu", "sigmoid", "tanh", "none")
 
 
 def listed():
     return [
-        # one token through a small block: all latency
-        {"name": "gated_token_small", "kind": "gated", "m": 2048, "n": 1024, "B": 1, "pad": 0, "type": "bf16", "act": "silu", "save": False, "add": False},
         # one token through a large block: a stream of weights
         {"name": "gated_token", "kind": "gated", "m": 16384, "n": 4096, "B": 1, "pad": 0, "type": "bf16", "act": "silu", "save": False, "add": False},
         # the next tokens of a few requests, with adapters on both projections
@@ -43,16 +46,18 @@ def listed():
         {"name": "gated_grad_ragged", "kind": "gated_grad", "m": 1531, "n": 1003, "B": 331, "pad": 6, "type": "f16", "act": "gelu"},
         # a training batch, backward
         {"name": "gated_grad_prompt", "kind": "gated_grad", "m": 8192, "n": 4096, "B": 4096, "pad": 0, "type": "bf16", "act": "silu"},
-        # one token of one request
-        {"name": "adapters_token", "kind": "adapters", "m": 1024, "n": 1024, "C": 1, "requests": 1, "count": 4, "rank": 8, "pad": 0, "type": "bf16"},
         # the next tokens of a served batch, nearly every request with an adapter of its own
         {"name": "adapters_requests", "kind": "adapters", "m": 4096, "n": 4096, "C": 48, "requests": 48, "count": 64, "rank": 16, "pad": 0, "type": "f16"},
         # ragged everywhere, fp32
         {"name": "adapters_ragged", "kind": "adapters", "m": 2777, "n": 1531, "C": 203, "requests": 9, "count": 5, "rank": 10, "pad": 3, "type": "f32"},
         # the prompts of a few requests
         {"name": "adapters_prompt", "kind": "adapters", "m": 4096, "n": 4096, "C": 8192, "requests": 6, "count": 8, "rank": 16, "pad": 0, "type": "bf16"},
-        # the same with the largest rank that is usual, into a wide layer
-        {"name": "adapters_rank64", "kind": "adapters", "m": 8192, "n": 4096, "C": 2048, "requests": 20, "count": 8, "rank": 64, "pad": 0, "type": "bf16"},
+        # one token of one request: all latency
+        {"name": "rotary_token", "kind": "rotary", "q": 32, "k": 8, "D": 128, "rot": 128, "B": 1, "pad": 0, "type": "bf16", "layout": "halves", "norm": True, "save": False},
+        # the prompts of a few requests, far into long contexts
+        {"name": "rotary_prompt", "kind": "rotary", "q": 32, "k": 8, "D": 128, "rot": 128, "B": 8192, "pad": 0, "type": "bf16", "layout": "halves", "norm": True, "save": True},
+        # a training batch's backward pass, neighbouring features in pairs, a part of the head turned, rows longer than the batch
+        {"name": "rotary_grad_ragged", "kind": "rotary_grad", "q": 24, "k": 8, "D": 96, "rot": 64, "B": 4099, "pad": 5, "type": "f16", "layout": "pairs", "norm": True},
     ]
 
 
@@ -62,7 +67,15 @@ def _log_size(rng, lo, hi):
 
 
 def draw(rng):
-    kind = rng.choice(("gated", "gated", "gated_grad", "adapters", "adapters"))
+    kind = rng.choice(("gated", "gated", "gated_grad", "adapters", "adapters", "rotary", "rotary_grad"))
+    if kind in ("rotary", "rotary_grad"):
+        k, D = rng.choice((1, 2, 4, 8)), rng.choice((32, 64, 80, 96, 128, 192, 256))
+        q = k * rng.choice((1, 2, 4, 7, 8))
+        case = {"kind": kind, "q": q, "k": k, "D": D, "rot": rng.choice((D, D, D // 2, D // 4)), "B": _log_size(rng, 1, min(16384, (1 << 25) // (D * (q + k)))), "pad": rng.choice((0, 0, 1, 8)),
+                "type": rng.choice(("f32", "f16", "bf16", "bf16")), "layout": rng.choice(("halves", "pairs")), "norm": rng.random() < 0.7}
+        if kind == "rotary":
+            case["save"] = case["norm"] and rng.random() < 0.5
+        return case
     if kind == "adapters":
         rank = rng.choice((4, 8, 10, 16, 24, 32, 64))
         C = _log_size(rng, 1, 8192 * 16 // max(rank, 16))
@@ -150,9 +163,29 @@ def _which(case, g):
     return adapter[first.cumsum(0)].to(torch.int32)
 
 
+def _positions(B, g):
+    """Four runs of consecutive positions that begin anywhere in a long context."""
+    column = torch.arange(B, device="cuda")
+    start = torch.randint(0, 1000000, (4,), device="cuda", generator=g)
+    return (start[column * 4 // B] + column).to(torch.int32)
+
+
 def _inputs(case, seed):
     kind, g, type_ = case["kind"], _generator(seed), case["type"]
-    s, m, n = dict(case), case["m"], case["n"]
+    s = dict(case)
+    if kind in ("rotary", "rotary_grad"):
+        heads, D, B = case["q"] + case["k"], case["D"], case["B"]
+        s["X"] = _activations(heads * D, B, case["pad"], type_, g)
+        s["position"] = _positions(B, g)
+        s["frequency"] = (500000.0 ** (-torch.arange(case["rot"] // 2, device="cuda") * 2.0 / case["rot"])).float() * (0.5 + 0.5 * torch.rand(case["rot"] // 2, device="cuda", generator=g))
+        if case["norm"]:
+            s["gain_q"], s["gain_k"] = (1.0 + 0.1 * torch.randn(D, device="cuda", generator=g) for _ in range(2))
+        if kind == "rotary_grad":
+            s["dY"] = (0.02 * torch.randn(heads * D, B, device="cuda", generator=g)).to(TYPES[type_])
+            if case["norm"]:
+                s["rstd"] = _rstd(s["X"][:, :B].float().view(heads, D, B))
+        return s
+    m, n = case["m"], case["n"]
     if kind == "adapters":
         C, count, rank = case["C"], case["count"], case["rank"]
         s["X"] = _activations(n, C, case["pad"], type_, g)
@@ -178,11 +211,24 @@ def prepare(case, seed):
     s = {"in_use": InUse()} if own else {}          # the first to go
     s.update(_inputs(case, seed))
     if own:
-        kind, m, n, new = case["kind"], case["m"], case["n"], lambda *shape: torch.zeros(*shape, dtype=TYPES[case["type"]], device="cuda")
-        if kind == "adapters":
+        kind, new = case["kind"], lambda *shape, type=case["type"]: torch.zeros(*shape, dtype=TYPES[type], device="cuda")
+        if kind in ("rotary", "rotary_grad"):
+            heads, D, B = s["q"] + s["k"], s["D"], s["B"]
+            if kind == "rotary":
+                s["Y"] = new(heads * D, B)
+                if s["save"]:
+                    s["rstd"] = new(heads, B, type="f32")
+            else:
+                s["dX"] = new(heads * D, B)
+                if s["norm"]:
+                    s.update(dgain_q=new(D, type="f32"), dgain_k=new(D, type="f32"))
+                context().head_rotary_reserve(s["q"], s["k"], D, B, type=s["type"])
+        elif kind == "adapters":
+            m, n = s["m"], s["n"]
             s["Y"] = new(m, s["C"])
             context().adapters_reserve(m, n, s["C"], s["rank"], type=s["type"])
         else:
+            m, n = s["m"], s["n"]
             if kind == "gated":
                 s["H"] = new(m, s["B"])
                 if s["save"]:
@@ -207,6 +253,15 @@ def _run_own(s):
         ctx.gated_grad(on["Wg"], on["Wu"], s["m"], s["n"], on["X"], s["B"], s["act"], on["G"], on["U"], on["dH"], on["dX"], on["dWg"], on["dWu"], type=s["type"],
                        x_stride=s["B"] + s["pad"])
         return {"dX": s["dX"], "dWg": s["dWg"], "dWu": s["dWu"]}
+    if kind == "rotary":
+        ctx.head_rotary(on["X"], s["q"], s["k"], s["D"], s["B"], on["position"], on["frequency"], s["rot"], on["Y"], layout=s["layout"], amplitude=AMPLITUDE, norm=s["norm"], eps=EPS,
+                        dGainQ=on.get("gain_q"), dGainK=on.get("gain_k"), dRstd=on.get("rstd"), type=s["type"], x_stride=s["B"] + s["pad"])
+        return {k: s[k] for k in ("Y", "rstd") if k in s}
+    if kind == "rotary_grad":
+        ctx.head_rotary_grad(on["X"], on["dY"], s["q"], s["k"], s["D"], s["B"], on["position"], on["frequency"], s["rot"], on["dX"], layout=s["layout"], amplitude=AMPLITUDE, norm=s["norm"],
+                             dGainQ=on.get("gain_q"), dGainK=on.get("gain_k"), dRstd=on.get("rstd"), dDgainQ=on.get("dgain_q"), dDgainK=on.get("dgain_k"), type=s["type"],
+                             x_stride=s["B"] + s["pad"])
+        return {k: s[k] for k in ("dX", "dgain_q", "dgain_k") if k in s}
     ctx.adapters(on["A"], on["B"], on["scale"], s["count"], s["rank"], on["which"], s["m"], s["n"], on["X"], s["C"], on["base"], on["Y"], type=s["type"],
                  x_stride=s["C"] + s["pad"])
     return s["Y"]
@@ -249,10 +304,59 @@ def _slope(G, act):
     return torch.ones_like(G)
 
 
+def _rstd(X):
+    return 1.0 / torch.sqrt(X.square().mean(dim=1) + EPS)
+
+
+def _gains(s):
+    """[heads, D, 1]: the queries' for the first heads, the keys' for the others."""
+    return torch.cat([s["gain_q"].expand(s["q"], -1), s["gain_k"].expand(s["k"], -1)]).unsqueeze(2)
+
+
+def _turn(X, s, back=False):
+    """The first `rot` features of every head of X [heads, D, B] turned by the columns' angles (64 bits: positions are far), times the amplitude."""
+    rot = s["rot"]
+    angle = s["position"].double().unsqueeze(0) * s["frequency"].double().unsqueeze(1)
+    cos, sin = (AMPLITUDE * torch.cos(angle)).float(), (AMPLITUDE * torch.sin(angle)).float()
+    if back:
+        sin = -sin
+    if s["layout"] == "halves":
+        a, b = X[:, :rot // 2], X[:, rot // 2:rot]
+        turned = torch.cat([a * cos - b * sin, b * cos + a * sin], dim=1)
+    else:
+        a, b = X[:, 0:rot:2], X[:, 1:rot:2]
+        turned = torch.stack([a * cos - b * sin, b * cos + a * sin], dim=2).reshape(X.shape[0], rot, X.shape[2])
+    return torch.cat([turned, X[:, rot:]], dim=1)
+
+
+def _run_rotary(s):
+    type_, heads, D, B = s["X"].dtype, s["q"] + s["k"], s["D"], s["B"]
+    X = s["X"][:, :B].float().view(heads, D, B)
+    if s["kind"] == "rotary":
+        out = {}
+        if s["norm"]:
+            rstd = _rstd(X)
+            X = X * rstd.unsqueeze(1) * _gains(s)
+            if s["save"]:
+                out["rstd"] = rstd
+        return {"Y": _turn(X, s).reshape(heads * D, B).to(type_), **out}
+    g = _turn(s["dY"].float().view(heads, D, B), s, back=True)
+    if not s["norm"]:
+        return {"dX": g.reshape(heads * D, B).to(type_)}
+    rstd = s["rstd"].unsqueeze(1)
+    h = X * rstd
+    along = g * _gains(s)
+    dX = (along - h * (along * h).mean(dim=1, keepdim=True)) * rstd
+    dgain = (g * h).sum(dim=2)
+    return {"dX": dX.reshape(heads * D, B).to(type_), "dgain_q": dgain[:s["q"]].sum(dim=0), "dgain_k": dgain[s["q"]:].sum(dim=0)}
+
+
 def run(s):
     if own:
         return _run_own(s)
     kind, type_ = s["kind"], s["X"].dtype
+    if kind in ("rotary", "rotary_grad"):
+        return _run_rotary(s)
     if kind == "adapters":
         # every adapter on every column, and of these the column's own
         C, m, count, rank = s["C"], s["m"], s["count"], s["rank"]
@@ -298,8 +402,41 @@ def _gate(G, act):
     return G * (1 + half) / 2, (1 + half) / 2 + G * (1 - half * half) * along / math.sqrt(2 * math.pi)
 
 
+def _exact_rotary(case, s):
+    q, k, D, B, rot = (case[name] for name in ("q", "k", "D", "B", "rot"))
+    first = torch.arange(rot // 2, device="cuda") * (1 if case["layout"] == "halves" else 2)
+    second = first + (rot // 2 if case["layout"] == "halves" else 1)
+    turn = AMPLITUDE * torch.exp(1j * s["frequency"].double()[:, None] * s["position"].double()[None, :])
+    X = s["X"][:, :B].double().view(q + k, D, B)
+    if case["norm"]:
+        gain = torch.stack([s["gain_q"].double()] * q + [s["gain_k"].double()] * k)[:, :, None]
+    if case["kind"] == "rotary":
+        out = {}
+        if case["norm"]:
+            size = ((X * X).sum(1, keepdim=True) / D + EPS).sqrt()
+            X = X / size * gain
+            if case["save"]:
+                out["rstd"] = 1 / size[:, 0]
+        pair = torch.complex(X[:, first], X[:, second]) * turn
+        Y = X.clone()
+        Y[:, first], Y[:, second] = pair.real, pair.imag
+        return {"Y": Y.view(-1, B), **out}
+    g = s["dY"].double().view(q + k, D, B).clone()
+    pair = torch.complex(g[:, first], g[:, second]) * turn.conj()
+    g[:, first], g[:, second] = pair.real, pair.imag
+    if not case["norm"]:
+        return {"dX": g.view(-1, B)}
+    r = s["rstd"].double()[:, None, :]
+    inner = (g * gain * X).sum(1, keepdim=True)
+    dX = g * gain * r - X * inner * r ** 3 / D
+    each = torch.einsum("hdb,hdb->hd", g, X * r)
+    return {"dX": dX.view(-1, B), "dgain_q": each[:q].sum(0), "dgain_k": each[q:].sum(0)}
+
+
 def exact(case, seed):
     s = _inputs(case, seed)
+    if case["kind"] in ("rotary", "rotary_grad"):
+        return _exact_rotary(case, s)
     if case["kind"] == "adapters":
         m, rank, X = case["m"], case["rank"], s["X"][:, :case["C"]].double()
         Y = s["base"].double()
@@ -326,7 +463,13 @@ def exact(case, seed):
 # ---- what a pass cannot do without --------------------------------------------------------------------------------
 
 def work(case):
-    e, m, n = BYTES[case["type"]], case["m"], case["n"]
+    e = BYTES[case["type"]]
+    if case["kind"] in ("rotary", "rotary_grad"):
+        heads, D, B = case["q"] + case["k"], case["D"], case["B"]
+        arrays = 2 if case["kind"] == "rotary" else 3 if case["norm"] else 2
+        statistics = 4.0 * heads * B if case["kind"] == "rotary_grad" and case["norm"] or case.get("save") else 0.0
+        return {"bytes": float(arrays * e * heads * D * B + 4 * B + 4 * case["rot"] // 2 + (8 * D if case["norm"] else 0)) + statistics, "flops": (8.0 if case["kind"] == "rotary" else 14.0) * heads * D * B}
+    m, n = case["m"], case["n"]
     if case["kind"] == "adapters":
         C, rank = case["C"], case["rank"]
         used = {_adapter_of(r, case["count"]) for r in range(min(case["requests"], C))} - {-1}
