@@ -51,6 +51,9 @@ enum {
  * the reference's separate activation layers applied to the matmul result
  * (src/layers/activation.cpp:38-40, 58-60). */
 enum { SO_ACT_NONE = 0, SO_ACT_RELU = 1, SO_ACT_SIGMOID = 2, SO_ACT_TANH = 3 };
+/* More activations, of so_gated and its gradient alone: x / (1 + exp(-x)), x Phi(x) with the normal distribution Phi, and
+ * x / (1 + exp(-2 z)), z = sqrt(2 / pi) (x + 0.044715 x^3), the approximation of the latter. */
+enum { SO_ACT_SILU = 4, SO_ACT_GELU = 5, SO_ACT_GELU_TANH = 6 };
 
 /* Device layouts kept for an uploaded ELLPACK matrix (bit flags).
  * ROW  : Wd[i*r + k], idx[i*r + k]  -- the encoder's own layout
@@ -401,6 +404,70 @@ so_status so_mxfp4_matmul(so_ctx *ctx, const so_mxfp4 *W, int type, const void *
 so_status so_mxfp4_matmul_reserve(so_ctx *ctx, const so_mxfp4 *W, uint32_t C);
 /* y [m] = W x + bias with x in fp32 as it is: the form for a single token, bound by the 4.25 bits per entry of W. */
 so_status so_mxfp4_matvec(so_ctx *ctx, const so_mxfp4 *W, const float *dx, const float *dBias, float *dy);
+
+/* ---- gated feed-forward block ---------------------------------------------------
+ * No counterpart in the reference.  Activations are [features x B], batch contiguous, their rows a stride apart, weights
+ * [m x n] row-major; all are of one element type.  Sums are taken in fp32, in the same order on every call, and a result of
+ * 16 bits is rounded once. */
+
+/* H [m x B] = act(Wg X + G0) * (Wu X + U0), both projections of X [n x B], the activation (any SO_ACT_*) and the product.
+ * dG0, dU0 [m x B], either may be NULL for zeros: what is added to the projections, as low-rank adapters make it of X (so_adapters).
+ * dG, dU [m x B], either may be NULL: the two sums as they go into the activation and the product, which so_gated_grad takes.
+ * dG may be dG0 and dU may be dU0, with the same stride; other overlaps are not allowed.  m or B may be 0, n may not.
+ * SO_ACT_RELU keeps NaN here. */
+so_status so_gated(so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t B, const void *dWg, const void *dWu, size_t w_stride,
+                   const void *dX, size_t x_stride, int act, const void *dG0, const void *dU0, size_t g0_stride,
+                   void *dH, size_t h_stride, void *dG, void *dU, size_t g_stride);
+/* Its gradient, from that of H and the saved sums G and U: dG = dH U act'(G) and dU = dH act(G), rounded to the element type
+ * (relu's slope at 0 is 0); dX = Wg^T dG + Wu^T dU, dWg = dG X^T, dWu = dU X^T, written, not added to.  Any result may be NULL:
+ * dDg and dDu [m x B] are the gradients of G0 and U0 too; dWg, dWu may be NULL where dDx is, dX where both dDwg and dDwu are.
+ * dDg and dDu may be dG, dU or dDh with the same stride; other overlaps are not allowed.  With B = 0 the weights' gradients are zeros. */
+so_status so_gated_grad(so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t B, const void *dWg, const void *dWu, size_t w_stride,
+                        const void *dX, size_t x_stride, int act, const void *dG, const void *dU, size_t g_stride,
+                        const void *dDh, size_t dh_stride, void *dDx, size_t dx_stride, void *dDwg, void *dDwu, size_t dw_stride,
+                        void *dDg, void *dDu, size_t dg_stride);
+/* Grows the context's workspace to what both need: before recording them into a graph, as so_matmul_reserve. */
+so_status so_gated_reserve(so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t B);
+
+/* ---- low-rank adapters --------------------------------------------------------------
+ * No counterpart in the reference.  Y [m x C] = base + scale_a B_a (A_a X), where every column of X [n x C] has an adapter of
+ * its own: a = which[c].  It goes beside a projection that the columns share: base is what so_mxfp4_matmul or so_matmul made
+ * of the same X.  A [count][rank x n] and B [count][m x rank] lie row-major without gaps, in the element type of X, base and Y;
+ * an adapter of a smaller rank is filled up with zeros.  A column whose which[c] is not in 0 .. count - 1 has none: Y = base there, and the
+ * adapters' values do not touch it.  dBase NULL: zeros; dY may be dBase with the same stride, other overlaps are not allowed.
+ * dScale [count] (fp32) NULL: ones.  rank is 1 .. 256; m, C and count may be 0, n may not.  Sums are taken in fp32, a
+ * column's in the same order whatever the other columns are; a result of 16 bits is rounded once. */
+so_status so_adapters(so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t C, uint32_t count, uint32_t rank, const void *dA,
+                      const void *dB, const float *dScale, const int32_t *dWhich, const void *dX, size_t x_stride,
+                      const void *dBase, size_t base_stride, void *dY, size_t y_stride);
+/* Grows the context's workspace to what a call needs: before recording it into a graph, as so_matmul_reserve. */
+so_status so_adapters_reserve(so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t C, uint32_t rank);
+
+/* ---- rotary positions, with norms of queries and keys ----------------------------------
+ * No counterpart in the reference.  X holds the heads_q heads of the queries and behind them the heads_k heads of the keys, D features each:
+ * [(heads_q + heads_k) D x B], batch contiguous, of an element type; column b stands at position pos[b].  What a fused projection leaves behind
+ * them (the values) is not touched.  Arithmetic is fp32, but for the angles, which are reduced in fp64: positions may be as far as int32 has them. */
+enum { SO_ROTARY_HALVES = 0, SO_ROTARY_PAIRS = 1 };
+
+/* With `norm`, first every head: h = x rstd, rstd = 1 / sqrt(sum_d x^2 / D + eps), times gain_d, dGainQ's or dGainK's [D] (fp32, NULL: ones); the factors
+ * [heads x B] (fp32) go to dRstd, unless it is NULL.  Without it eps, the gains and dRstd are not looked at.
+ * Then the first `rot` features (even, 0 .. D) of every head are turned: features i and i + rot / 2 (SO_ROTARY_HALVES), or 2 i and 2 i + 1
+ * (SO_ROTARY_PAIRS), as (a cos - b sin, b cos + a sin) times `amplitude`, by the angle pos[b] * freq[i].  freq [rot / 2] (fp32, radians) and amplitude carry
+ * whatever scaling a long context asks for.  The other features are left as they are.  D is 1 .. 512.  dPos and dFreq may be NULL where rot is 0.
+ * dY may be dX with the same stride, other overlaps are not allowed.  heads_q, heads_k or B may be 0. */
+so_status so_head_rotary(so_ctx *ctx, int type, uint32_t heads_q, uint32_t heads_k, uint32_t D, uint32_t B, const void *dX, size_t x_stride,
+                         int norm, const float *dGainQ, const float *dGainK, float eps, const int32_t *dPos, const float *dFreq, uint32_t rot,
+                         float amplitude, int layout, void *dY, size_t y_stride, float *dRstd);
+/* Its gradient.  g is dY turned back, times the amplitude; without `norm` dX = g.  With it, from X and the saved factors, h = x rstd:
+ * dX = rstd (g gain - h sum_d (g gain h) / D), dDgainQ_d = sum g h over the queries' heads and all columns, dDgainK over the keys' (fp32 [D]),
+ * written, not added to.  Any result may be NULL.  Without norm X, dRstd and the gains are not looked at and dDgainQ, dDgainK are left as they are.
+ * dDx may be dX or dDy with the same stride, other overlaps are not allowed.  Sums are taken in the same order on every call. */
+so_status so_head_rotary_grad(so_ctx *ctx, int type, uint32_t heads_q, uint32_t heads_k, uint32_t D, uint32_t B, const void *dX, size_t x_stride,
+                              const void *dDy, size_t dy_stride, int norm, const float *dGainQ, const float *dGainK, const float *dRstd,
+                              const int32_t *dPos, const float *dFreq, uint32_t rot, float amplitude, int layout, void *dDx, size_t dx_stride,
+                              float *dDgainQ, float *dDgainK);
+/* Grows the context's workspace to what the gradient needs: before recording it into a graph, as so_matmul_reserve. */
+so_status so_head_rotary_reserve(so_ctx *ctx, int type, uint32_t heads_q, uint32_t heads_k, uint32_t D, uint32_t B);
 
 /* ---- launch graphs -------------------------------------------------------
  * Record every launch made on the context between begin and end into one

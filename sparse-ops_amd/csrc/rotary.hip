@@ -1,0 +1,390 @@
+// Rotary positions of queries and keys, with a norm of every head ahead of them, and the gradient.
+#include "layer_norm.h"
+
+namespace {
+
+constexpr uint32_t kMostFeatures = 512;
+
+struct Shape {
+    uint32_t heads_q, heads, D, B, rot;
+    int pairs;                          // SO_ROTARY_PAIRS
+    uint32_t tiles, per, groups_q, groups;      // tiles of columns; heads of a workgroup; groups of them, first the queries'
+};
+
+// The rows of a head that a thread holds: pair p is two features that are turned together, or two neighbours of those behind them.
+__device__ __forceinline__ uint2 rows_of(const Shape &s, uint32_t p)
+{
+    const uint32_t half = s.rot / 2u;
+    if (p >= half) return make_uint2(s.rot + 2u * (p - half), s.rot + 2u * (p - half) + 1u);
+    return s.pairs ? make_uint2(2u * p, 2u * p + 1u) : make_uint2(p, p + half);
+}
+
+// cos and sin of pos * freq, times the amplitude.  The product is exact in fp64; of it the whole turns are taken off there, so that a position of 2^31 costs 2^-22 of a turn and one of 2^20 less
+// than fp32 can tell.
+__device__ __forceinline__ float2 turn_of(int32_t pos, double turns, float amplitude)
+{
+    const double t = (double)pos * turns;
+    float c, s;
+    sincospif(2.0f * (float)(t - rint(t)), &s, &c);
+    return make_float2(amplitude * c, amplitude * s);
+}
+
+constexpr double kTurnsPerRadian = 0.15915494309189533577;
+
+// What forward pass and gradient share: a workgroup of NT threads takes LC * V columns of `per` heads, one after the other; a thread PPT pairs of a head's features, for which it keeps the turns of its columns.
+template <class T, int LC, int PPT, int NT>
+struct Seat {
+    static constexpr int V = so_elements<T>::V, RL = NT / LC;
+    typedef typename so_elements<T>::plain group;
+    uint32_t tile, c0, left, first, last, wide;     // its columns; heads first .. last - 1
+    bool query;
+    uint2 row[PPT];                                 // inside a head
+    bool has[PPT], two[PPT];
+    __device__ __forceinline__ Seat(const Shape &s, size_t ld)
+    {
+        tile = blockIdx.x % s.tiles;
+        const uint32_t g = blockIdx.x / s.tiles;
+        query = g < s.groups_q;
+        first = query ? g * s.per : s.heads_q + (g - s.groups_q) * s.per;
+        last = min(first + s.per, query ? s.heads_q : s.heads);
+        const uint64_t c = (uint64_t)tile * (LC * V) + threadIdx.x % LC * V;
+        left = c >= s.B ? 0u : (uint32_t)min((uint64_t)s.B - c, (uint64_t)V);
+        c0 = (uint32_t)c;
+        wide = so_group_wide_rows<T>(left, s.heads * s.D, ld);
+#pragma unroll
+        for (int k = 0; k < PPT; ++k) {
+            row[k] = rows_of(s, threadIdx.x / LC + k * RL);
+            has[k] = left && row[k].x < s.D;
+            two[k] = left && row[k].y < s.D;
+        }
+    }
+    __device__ __forceinline__ void turns(const Shape &s, const int32_t *pos, const float *freq, float amplitude, float2 (&t)[PPT][V]) const
+    {
+        int32_t p[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) p[e] = s.rot && (uint32_t)e < left ? pos[c0 + e] : 0;
+#pragma unroll
+        for (int k = 0; k < PPT; ++k) {
+            const uint32_t i = threadIdx.x / LC + k * RL;
+            const bool turned = i < s.rot / 2u;
+            const double f = turned ? (double)freq[i] * kTurnsPerRadian : 0.0;
+#pragma unroll
+            for (int e = 0; e < V; ++e) t[k][e] = turned ? turn_of(p[e], f, amplitude) : make_float2(1.0f, 0.0f);
+        }
+    }
+    __device__ __forceinline__ void load(const Shape &s, uint32_t head, const T *X, size_t ld, group (&x)[PPT][2]) const
+    {
+#pragma unroll
+        for (int k = 0; k < PPT; ++k) {
+            const uint32_t r0 = head * s.D + row[k].x, r1 = head * s.D + row[k].y;
+            x[k][0] = group{};
+            x[k][1] = group{};
+            if (has[k]) x[k][0] = so_group_load(X + (size_t)r0 * ld + c0, left, r0 < wide);
+            if (two[k]) x[k][1] = so_group_load(X + (size_t)r1 * ld + c0, left, r1 < wide);
+        }
+    }
+};
+
+template <class T, int LC, int PPT, int NT, bool NORM>
+__global__ __launch_bounds__(NT)
+void rotary_kernel(Shape s, const T *X, size_t ldx, const float *gain_q, const float *gain_k, float eps, const int32_t *pos, const float *freq, float amplitude, float direction, T *Y, size_t ldy,
+                   float *rstd)
+{
+    constexpr int V = so_elements<T>::V;
+    __shared__ float lds[(NT / 64 + 1) * LC * V];
+    const Seat<T, LC, PPT, NT> at(s, ldx);
+    typename so_elements<T>::plain x[PPT][2], next[PPT][2];
+    at.load(s, at.first, X, ldx, x);
+    float2 turn[PPT][V];
+    at.turns(s, pos, freq, amplitude, turn);
+    const float *gain = at.query ? gain_q : gain_k;
+    float2 g[PPT];
+#pragma unroll
+    for (int k = 0; k < PPT; ++k) {
+        g[k] = make_float2(1.0f, 1.0f);
+        if (NORM && gain && at.has[k]) g[k].x = gain[at.row[k].x];
+        if (NORM && gain && at.two[k]) g[k].y = gain[at.row[k].y];
+    }
+    for (uint32_t head = at.first; head < at.last; ++head) {
+        if (head + 1u < at.last) at.load(s, head + 1u, X, ldx, next);
+        float r[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) r[e] = 0.0f;
+        if constexpr (NORM) {
+#pragma unroll
+            for (int k = 0; k < PPT; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) r[e] = fmaf((float)x[k][1][e], (float)x[k][1][e], fmaf((float)x[k][0][e], (float)x[k][0][e], r[e]));
+            so_norm::sum_tile<NT, LC, V>(r, lds);
+#pragma unroll
+            for (int e = 0; e < V; ++e) r[e] = 1.0f / sqrtf(r[e] / (float)s.D + eps);
+            if (rstd && threadIdx.x < LC)
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if ((uint32_t)e < at.left) rstd[(size_t)head * s.B + at.c0 + e] = r[e];
+        }
+#pragma unroll
+        for (int k = 0; k < PPT; ++k) {
+            float a[V], b[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float u = NORM ? (float)x[k][0][e] * r[e] * g[k].x : (float)x[k][0][e], v = NORM ? (float)x[k][1][e] * r[e] * g[k].y : (float)x[k][1][e];
+                const float c = turn[k][e].x, d = direction * turn[k][e].y;
+                a[e] = fmaf(u, c, -(v * d));
+                b[e] = fmaf(v, c, u * d);
+            }
+            if (at.has[k]) so_group_store(Y + (size_t)(head * s.D + at.row[k].x) * ldy + at.c0, at.left, a);
+            if (at.two[k]) so_group_store(Y + (size_t)(head * s.D + at.row[k].y) * ldy + at.c0, at.left, b);
+        }
+#pragma unroll
+        for (int k = 0; k < PPT; ++k) x[k][0] = next[k][0], x[k][1] = next[k][1];
+    }
+}
+
+// With norms: dX, and of every workgroup its share of the gains' gradients, [tiles * groups][D].
+template <class T, int LC, int PPT, int NT>
+__global__ __launch_bounds__(NT)
+void rotary_grad_kernel(Shape s, const T *X, size_t ldx, const T *dY, size_t ldd, const float *gain_q, const float *gain_k, const float *rstd, const int32_t *pos, const float *freq, float amplitude,
+                        T *dX, size_t ldo, float *shares)
+{
+    constexpr int V = so_elements<T>::V;
+    __shared__ float lds[(NT / 64 + 1) * LC * V];
+    const Seat<T, LC, PPT, NT> at(s, ldx);
+    const uint32_t wide_d = so_group_wide_rows<T>(at.left, s.heads * s.D, ldd);
+    Seat<T, LC, PPT, NT> of_dy = at;
+    of_dy.wide = wide_d;
+    float2 turn[PPT][V];
+    at.turns(s, pos, freq, amplitude, turn);
+    const float *gain = at.query ? gain_q : gain_k;
+    float2 g[PPT], sum[PPT];
+#pragma unroll
+    for (int k = 0; k < PPT; ++k) {
+        g[k] = make_float2(1.0f, 1.0f);
+        sum[k] = make_float2(0.0f, 0.0f);
+        if (gain && at.has[k]) g[k].x = gain[at.row[k].x];
+        if (gain && at.two[k]) g[k].y = gain[at.row[k].y];
+    }
+    for (uint32_t head = at.first; head < at.last; ++head) {
+        typename so_elements<T>::plain x[PPT][2], d[PPT][2];
+        at.load(s, head, X, ldx, x);
+        of_dy.load(s, head, dY, ldd, d);
+        float r[V], dot[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            r[e] = (uint32_t)e < at.left ? rstd[(size_t)head * s.B + at.c0 + e] : 0.0f;
+            dot[e] = 0.0f;
+        }
+        float a[PPT][V], b[PPT][V];
+#pragma unroll
+        for (int k = 0; k < PPT; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float u = (float)d[k][0][e], v = (float)d[k][1][e], c = turn[k][e].x, w = turn[k][e].y;
+                a[k][e] = fmaf(u, c, v * w);
+                b[k][e] = fmaf(v, c, -(u * w));
+                const float p = a[k][e] * ((float)x[k][0][e] * r[e]), q = b[k][e] * ((float)x[k][1][e] * r[e]);
+                if ((uint32_t)e < at.left) {
+                    sum[k].x += p;
+                    sum[k].y += q;
+                }
+                dot[e] += fmaf(p, g[k].x, q * g[k].y);
+            }
+        if (!dX) continue;
+        so_norm::sum_tile<NT, LC, V>(dot, lds);
+#pragma unroll
+        for (int k = 0; k < PPT; ++k) {
+            float p[V], q[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float mean = dot[e] / (float)s.D;
+                p[e] = r[e] * fmaf(a[k][e], g[k].x, -(((float)x[k][0][e] * r[e]) * mean));
+                q[e] = r[e] * fmaf(b[k][e], g[k].y, -(((float)x[k][1][e] * r[e]) * mean));
+            }
+            if (at.has[k]) so_group_store(dX + (size_t)(head * s.D + at.row[k].x) * ldo + at.c0, at.left, p);
+            if (at.two[k]) so_group_store(dX + (size_t)(head * s.D + at.row[k].y) * ldo + at.c0, at.left, q);
+        }
+    }
+    if (!shares) return;
+#pragma unroll
+    for (int k = 0; k < PPT; ++k) {
+        const float p = so_norm::sum_lanes<LC>(sum[k].x), q = so_norm::sum_lanes<LC>(sum[k].y);
+        if (threadIdx.x % LC == 0) {                                 // the first of a row's lanes: its columns exist where any do
+            if (at.has[k]) shares[(size_t)blockIdx.x * s.D + at.row[k].x] = p;
+            if (at.two[k]) shares[(size_t)blockIdx.x * s.D + at.row[k].y] = q;
+        }
+    }
+}
+
+// The shares of the queries' workgroups and of the keys' to one gradient each: 16 features a workgroup, 16 runs of shares.
+__global__ __launch_bounds__(256)
+void rotary_gains_kernel(uint32_t D, uint32_t shares_q, uint32_t shares, uint32_t blocks, const float *from, float *gain_q, float *gain_k)
+{
+    __shared__ float sums[16][17];
+    const bool query = blockIdx.x < blocks;
+    float *out = query ? gain_q : gain_k;
+    const uint32_t d = blockIdx.x % blocks * 16u + threadIdx.x % 16u, run = threadIdx.x / 16u, end = query ? shares_q : shares;
+    float s = 0.0f;
+    if (d < D)
+        for (uint32_t p = (query ? 0u : shares_q) + run; p < end; p += 16u) s += from[(size_t)p * D + d];
+    sums[run][threadIdx.x % 16u] = s;
+    __syncthreads();
+    if (run || d >= D || !out) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += sums[i][threadIdx.x];
+    out[d] = s;
+}
+
+// Lanes of a row and threads, and the pairs of a thread, 1, 2 or 4: 32 lanes down a head of up to 256 features, 128 of a larger one, 64 where a row is one group.
+struct Cut { uint32_t lanes, threads, pairs; };
+Cut cut_of(int type, uint32_t D, uint32_t rot, uint32_t B)
+{
+    const uint32_t V = 16u / (uint32_t)so_type_bytes(type), pairs = rot / 2u + (D - rot + 1u) / 2u;
+    Cut c;
+    c.lanes = B <= V ? 1 : pairs > 128 ? 4 : B <= 2 * V ? 2 : B <= 4 * V ? 4 : 8;
+    c.threads = c.lanes == 1 ? 64 : pairs > 128 ? 512 : 32 * c.lanes;
+    const uint32_t each = so_ceil_div(pairs, c.threads / c.lanes);
+    c.pairs = each <= 1 ? 1 : each <= 2 ? 2 : 4;
+    return c;
+}
+
+Shape shape_of(const so_ctx *ctx, const Cut &c, int type, uint32_t heads_q, uint32_t heads_k, uint32_t D, uint32_t B, uint32_t rot, int layout)
+{
+    Shape s = {heads_q, heads_q + heads_k, D, B, rot, layout == SO_ROTARY_PAIRS, 0, 1, 0, 0};
+    s.tiles = so_ceil_div(B, c.lanes * (16u / (uint32_t)so_type_bytes(type)));
+    // as many heads a workgroup as leave every compute unit 2048 threads: the turns are worked out once for all of them
+    const uint64_t want = (uint64_t)ctx->compute_units * (2048u / c.threads);
+    s.per = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((uint64_t)s.tiles * s.heads / want, s.heads));
+    s.groups_q = so_ceil_div(heads_q, s.per);
+    s.groups = s.groups_q + so_ceil_div(heads_k, s.per);
+    return s;
+}
+
+size_t share_bytes(const Shape &s) { return (size_t)s.tiles * s.groups * s.D * sizeof(float); }
+
+template <class F>
+void for_cut(const Cut &c, F &&f)
+{
+    const auto with = [&](auto lanes, auto threads) {
+        if (c.pairs == 1) f(lanes, std::integral_constant<int, 1>(), threads);
+        else if (c.pairs == 2) f(lanes, std::integral_constant<int, 2>(), threads);
+        else f(lanes, std::integral_constant<int, 4>(), threads);
+    };
+    if (c.lanes == 1) with(std::integral_constant<int, 1>(), std::integral_constant<int, 64>());
+    else if (c.lanes == 2) with(std::integral_constant<int, 2>(), std::integral_constant<int, 64>());
+    else if (c.threads == 512) f(std::integral_constant<int, 4>(), std::integral_constant<int, 2>(), std::integral_constant<int, 512>());
+    else if (c.lanes == 4) with(std::integral_constant<int, 4>(), std::integral_constant<int, 128>());
+    else with(std::integral_constant<int, 8>(), std::integral_constant<int, 256>());
+}
+
+so_status workspace(so_ctx *ctx, const char *who, size_t bytes)
+{
+    SO_REQUIRE(!ctx->capturing || (ctx->mm_part && ctx->mm_part->bytes >= bytes),
+               "%s: the context's workspace must grow, which cannot be done while a graph is being recorded (call so_head_rotary_reserve, or launch this shape once, before recording)", who);
+    return so_matmul_workspace(ctx, bytes, 4);
+}
+
+bool launch_fits(const Shape &s, const Cut &c) { return so_grid_fits((uint64_t)s.tiles * s.groups, c.threads) && (uint64_t)s.heads * s.D < (1ull << 32); }
+
+} // namespace
+
+#define SO_ROTARY_CHECKS(who)                                                                                               \
+    SO_REQUIRE(ctx != nullptr, who ": ctx is null");                                                                        \
+    SO_REQUIRE(type >= SO_F32 && type <= SO_BF16, who ": unknown element type %d", type);                                   \
+    SO_REQUIRE(D >= 1 && D <= kMostFeatures, who ": %u features a head are not 1 .. %u", D, kMostFeatures);                 \
+    SO_REQUIRE((uint64_t)heads_q + heads_k < (1ull << 32) / kMostFeatures, who ": too many heads")
+
+extern "C" so_status so_head_rotary_reserve(so_ctx *ctx, int type, uint32_t heads_q, uint32_t heads_k, uint32_t D, uint32_t B)
+{
+    SO_ROTARY_CHECKS("so_head_rotary_reserve");
+    SO_REQUIRE(!ctx->capturing, "so_head_rotary_reserve: a graph is being recorded");
+    if (heads_q + heads_k == 0 || B == 0) return SO_OK;
+    const so_on_device on(ctx->device);
+    SO_HIP(on.status);
+    // the number of pairs depends on rot where D is odd, and with it the cut
+    size_t bytes = 0;
+    for (const uint32_t rot : {0u, D & ~1u}) bytes = std::max(bytes, share_bytes(shape_of(ctx, cut_of(type, D, rot, B), type, heads_q, heads_k, D, B, rot, 0)));
+    return workspace(ctx, "so_head_rotary_reserve", bytes);
+}
+
+extern "C" so_status so_head_rotary(so_ctx *ctx, int type, uint32_t heads_q, uint32_t heads_k, uint32_t D, uint32_t B, const void *dX, size_t x_stride, int norm, const float *dGainQ,
+                                    const float *dGainK, float eps, const int32_t *dPos, const float *dFreq, uint32_t rot, float amplitude, int layout, void *dY, size_t y_stride, float *dRstd)
+{
+    SO_ROTARY_CHECKS("so_head_rotary");
+    SO_REQUIRE(rot % 2 == 0 && rot <= D, "so_head_rotary: %u features to turn are not an even number of 0 .. %u", rot, D);
+    SO_REQUIRE(layout == SO_ROTARY_HALVES || layout == SO_ROTARY_PAIRS, "so_head_rotary: unknown layout %d", layout);
+    SO_REQUIRE(!norm || eps >= 0.0f, "so_head_rotary: eps is negative or not a number");
+    if (heads_q + heads_k == 0 || B == 0) return SO_OK;
+    SO_REQUIRE(dX && dY, "so_head_rotary: null tensor");
+    SO_REQUIRE(rot == 0 || (dPos && dFreq), "so_head_rotary: null positions or frequencies");
+    SO_REQUIRE(x_stride >= B && y_stride >= B, "so_head_rotary: a stride is shorter than a row");
+    SO_REQUIRE(dX != dY || x_stride == y_stride, "so_head_rotary: in place needs one stride");
+    SO_REQUIRE(!norm || !dRstd || (dRstd != dX && dRstd != dY), "so_head_rotary: a result is an input, or one array for both results");
+    const so_on_device on(ctx->device);
+    SO_HIP(on.status);
+    const Cut c = cut_of(type, D, rot, B);
+    const Shape s = shape_of(ctx, c, type, heads_q, heads_k, D, B, rot, layout);
+    SO_REQUIRE(launch_fits(s, c), "so_head_rotary: %u x %u is too large for one launch", s.heads * D, B);
+    so_for_type(type, [&](auto t) {
+        using T = decltype(t);
+        for_cut(c, [&](auto lanes, auto pairs, auto threads) {
+            constexpr int LC = decltype(lanes)::value, PPT = decltype(pairs)::value, NT = decltype(threads)::value;
+            const auto kernel = norm ? rotary_kernel<T, LC, PPT, NT, true> : rotary_kernel<T, LC, PPT, NT, false>;
+            kernel<<<s.tiles * s.groups, NT, 0, ctx->stream>>>(s, (const T *)dX, x_stride, dGainQ, dGainK, eps, dPos, dFreq, amplitude, 1.0f, (T *)dY, y_stride, dRstd);
+        });
+    });
+    SO_LAUNCH_CHECK();
+    return SO_OK;
+}
+
+extern "C" so_status so_head_rotary_grad(so_ctx *ctx, int type, uint32_t heads_q, uint32_t heads_k, uint32_t D, uint32_t B, const void *dX, size_t x_stride, const void *dDy, size_t dy_stride,
+                                         int norm, const float *dGainQ, const float *dGainK, const float *dRstd, const int32_t *dPos, const float *dFreq, uint32_t rot, float amplitude,
+                                         int layout, void *dDx, size_t dx_stride, float *dDgainQ, float *dDgainK)
+{
+    SO_ROTARY_CHECKS("so_head_rotary_grad");
+    SO_REQUIRE(rot % 2 == 0 && rot <= D, "so_head_rotary_grad: %u features to turn are not an even number of 0 .. %u", rot, D);
+    SO_REQUIRE(layout == SO_ROTARY_HALVES || layout == SO_ROTARY_PAIRS, "so_head_rotary_grad: unknown layout %d", layout);
+    const bool gains = norm && (dDgainQ || dDgainK), any = heads_q + heads_k > 0 && B > 0;
+    if (!gains && (!dDx || !any)) return SO_OK;
+    if (any) {
+        SO_REQUIRE(dDy && (!norm || dX), "so_head_rotary_grad: null tensor");
+        SO_REQUIRE(!norm || dRstd, "so_head_rotary_grad: null factors");
+        SO_REQUIRE(rot == 0 || (dPos && dFreq), "so_head_rotary_grad: null positions or frequencies");
+        SO_REQUIRE((!norm || x_stride >= B) && dy_stride >= B && (!dDx || dx_stride >= B), "so_head_rotary_grad: a stride is shorter than a row");
+        SO_REQUIRE(!dDx || ((dDx != dDy || dx_stride == dy_stride) && (!norm || dDx != dX || dx_stride == x_stride)), "so_head_rotary_grad: in place needs one stride");
+    }
+    if (gains) {
+        SO_REQUIRE(!dDgainQ || dDgainQ != dDgainK, "so_head_rotary_grad: one array for two results");
+        for (const void *result : {(const void *)dDgainQ, (const void *)dDgainK})
+            SO_REQUIRE(!result || (result != dX && result != dDy && result != dDx && result != dRstd && result != dGainQ && result != dGainK && result != dFreq),
+                       "so_head_rotary_grad: a result is an input, or one array for two results");
+    }
+    const so_on_device on(ctx->device);
+    SO_HIP(on.status);
+    const Cut c = cut_of(type, D, rot, std::max(B, 1u));
+    const Shape s = shape_of(ctx, c, type, heads_q, heads_k, D, B, rot, layout);
+    SO_REQUIRE(launch_fits(s, c), "so_head_rotary_grad: %u x %u is too large for one launch", s.heads * D, B);
+    float *shares = nullptr;
+    if (gains && any) {
+        if (const so_status st = workspace(ctx, "so_head_rotary_grad", share_bytes(s)); st != SO_OK) return st;
+        shares = (float *)ctx->mm_part->p;
+    }
+    if (any)
+        so_for_type(type, [&](auto t) {
+            using T = decltype(t);
+            for_cut(c, [&](auto lanes, auto pairs, auto threads) {
+                constexpr int LC = decltype(lanes)::value, PPT = decltype(pairs)::value, NT = decltype(threads)::value;
+                if (norm)
+                    rotary_grad_kernel<T, LC, PPT, NT><<<s.tiles * s.groups, NT, 0, ctx->stream>>>(s, (const T *)dX, x_stride, (const T *)dDy, dy_stride, dGainQ, dGainK, dRstd, dPos, dFreq,
+                                                                                                     amplitude, (T *)dDx, dx_stride, shares);
+                else
+                    rotary_kernel<T, LC, PPT, NT, false><<<s.tiles * s.groups, NT, 0, ctx->stream>>>(s, (const T *)dDy, dy_stride, nullptr, nullptr, 0.0f, dPos, dFreq, amplitude, -1.0f, (T *)dDx,
+                                                                                                       dx_stride, nullptr);
+            });
+        });
+    if (gains) {
+        const uint32_t blocks = so_ceil_div(D, 16);
+        rotary_gains_kernel<<<2 * blocks, 256, 0, ctx->stream>>>(D, s.tiles * s.groups_q, s.tiles * s.groups, blocks, shares, dDgainQ, dDgainK);
+    }
+    SO_LAUNCH_CHECK();
+    return SO_OK;
+}

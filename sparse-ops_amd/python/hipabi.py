@@ -13,8 +13,9 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "libsparseops_hip.so")
 
 SO_OK, SO_ERR_NO_DEVICE, SO_ERR_INVALID, SO_ERR_OOM, SO_ERR_HIP, SO_ERR_BOUNDS = range(6)
-ACT = {"none": 0, "relu": 1, "sigmoid": 2, "tanh": 3}
+ACT = {"none": 0, "relu": 1, "sigmoid": 2, "tanh": 3, "silu": 4, "gelu": 5, "gelu_tanh": 6}     # from 4 on: of gated() alone
 TYPE = {"f32": 0, "f16": 1, "bf16": 2}
+ROTARY = {"halves": 0, "pairs": 1}
 LAYOUT_ROW, LAYOUT_SLOT, LAYOUT_BINS, LAYOUT_TILED, LAYOUT_RBM, LAYOUT_IDX16 = 1, 2, 4, 8, 16, 32
 
 # Every symbol include/sparseops_hip.h declares.
@@ -25,7 +26,7 @@ SYMBOLS = (
     "so_conv2d so_maxpool so_gap so_add so_act so_transpose so_reverse_axes3 so_copy_rows so_graph_begin so_graph_end "
     "so_graph_launch so_graph_free so_rbm_upload so_rbm_free so_rbm_dims so_conv_plan_set_rbm so_conv_plan_rbm_info "
     "so_layer_norm so_layer_norm_grad so_layer_norm_reserve so_mxfp4_quantize so_mxfp4_dequantize so_mxfp4_create so_mxfp4_free so_mxfp4_dims so_mxfp4_matmul "
-    "so_mxfp4_matmul_reserve so_mxfp4_matvec").split()
+    "so_mxfp4_matmul_reserve so_mxfp4_matvec so_gated so_gated_grad so_gated_reserve so_adapters so_adapters_reserve so_head_rotary so_head_rotary_grad so_head_rotary_reserve").split()
 
 _vp = ct.c_void_p
 _u32 = ct.c_uint32
@@ -126,6 +127,15 @@ def load_library(path=None):
         "so_mxfp4_matmul": [_vp, _vp, ct.c_int, _vp, ct.c_size_t, _u32, _vp, _vp, ct.c_size_t, ct.c_int],
         "so_mxfp4_matmul_reserve": [_vp, _vp, _u32],
         "so_mxfp4_matvec": [_vp, _vp, _vp, _vp, _vp],
+        "so_gated": [_vp, ct.c_int, _u32, _u32, _u32, _vp, _vp, ct.c_size_t, _vp, ct.c_size_t, ct.c_int, _vp, _vp, ct.c_size_t, _vp, ct.c_size_t, _vp, _vp, ct.c_size_t],
+        "so_gated_grad": [_vp, ct.c_int, _u32, _u32, _u32, _vp, _vp, ct.c_size_t, _vp, ct.c_size_t, ct.c_int, _vp, _vp, ct.c_size_t, _vp, ct.c_size_t, _vp, ct.c_size_t,
+                          _vp, _vp, ct.c_size_t, _vp, _vp, ct.c_size_t],
+        "so_gated_reserve": [_vp, ct.c_int, _u32, _u32, _u32],
+        "so_adapters": [_vp, ct.c_int, _u32, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp, ct.c_size_t, _vp, ct.c_size_t, _vp, ct.c_size_t],
+        "so_adapters_reserve": [_vp, ct.c_int, _u32, _u32, _u32, _u32],
+        "so_head_rotary": [_vp, ct.c_int, _u32, _u32, _u32, _u32, _vp, ct.c_size_t, ct.c_int, _vp, _vp, ct.c_float, _vp, _vp, _u32, ct.c_float, ct.c_int, _vp, ct.c_size_t, _vp],
+        "so_head_rotary_grad": [_vp, ct.c_int, _u32, _u32, _u32, _u32, _vp, ct.c_size_t, _vp, ct.c_size_t, ct.c_int, _vp, _vp, _vp, _vp, _vp, _u32, ct.c_float, ct.c_int, _vp, ct.c_size_t, _vp, _vp],
+        "so_head_rotary_reserve": [_vp, ct.c_int, _u32, _u32, _u32, _u32],
     }
     for name, argtypes in sig.items():
         fn = getattr(lib, name)
@@ -367,6 +377,44 @@ class Context:
 
     def mxfp4_matvec(self, W, dx, dBias, dy):
         self._ck(self.lib.so_mxfp4_matvec(self.h, W.h, _at(dx), _at(dBias), _at(dy)))
+
+    def gated(self, dWg, dWu, m, n, dX, B, act, dH, dG=None, dU=None, dG0=None, dU0=None, type="f32", w_stride=None, x_stride=None, h_stride=None, g_stride=None, g0_stride=None):
+        """H (m, B) = act(Wg X + G0) * (Wu X + U0); dG and dU receive the two sums."""
+        self._ck(self.lib.so_gated(self.h, TYPE[type], m, n, B, _at(dWg), _at(dWu), n if w_stride is None else w_stride, _at(dX), B if x_stride is None else x_stride, ACT[act],
+                                   _at(dG0), _at(dU0), B if g0_stride is None else g0_stride, _at(dH), B if h_stride is None else h_stride,
+                                   _at(dG), _at(dU), B if g_stride is None else g_stride))
+
+    def gated_grad(self, dWg, dWu, m, n, dX, B, act, dG, dU, dDh, dDx=None, dDwg=None, dDwu=None, dDg=None, dDu=None, type="f32", w_stride=None, x_stride=None, g_stride=None,
+                   dh_stride=None, dx_stride=None, dw_stride=None, dg_stride=None):
+        self._ck(self.lib.so_gated_grad(self.h, TYPE[type], m, n, B, _at(dWg), _at(dWu), n if w_stride is None else w_stride, _at(dX), B if x_stride is None else x_stride, ACT[act],
+                                        _at(dG), _at(dU), B if g_stride is None else g_stride, _at(dDh), B if dh_stride is None else dh_stride, _at(dDx), B if dx_stride is None else dx_stride,
+                                        _at(dDwg), _at(dDwu), n if dw_stride is None else dw_stride, _at(dDg), _at(dDu), B if dg_stride is None else dg_stride))
+
+    def gated_reserve(self, m, n, B, type="f32"):
+        self._ck(self.lib.so_gated_reserve(self.h, TYPE[type], m, n, B))
+
+    def adapters(self, dA, dB, dScale, count, rank, dWhich, m, n, dX, C, dBase, dY, type="f32", x_stride=None, base_stride=None, y_stride=None):
+        """Y (m, C) = base + scale_a B_a (A_a X), a = which[c] the adapter of a column (int32; none where it is not in 0 .. count - 1)."""
+        self._ck(self.lib.so_adapters(self.h, TYPE[type], m, n, C, count, rank, _at(dA), _at(dB), _at(dScale), _at(dWhich), _at(dX), C if x_stride is None else x_stride,
+                                      _at(dBase), C if base_stride is None else base_stride, _at(dY), C if y_stride is None else y_stride))
+
+    def adapters_reserve(self, m, n, C, rank, type="f32"):
+        self._ck(self.lib.so_adapters_reserve(self.h, TYPE[type], m, n, C, rank))
+
+    def head_rotary(self, dX, heads_q, heads_k, D, B, dPos, dFreq, rot, dY, layout="halves", amplitude=1.0, norm=False, eps=0.0, dGainQ=None, dGainK=None, dRstd=None, type="f32",
+                    x_stride=None, y_stride=None):
+        """Queries and keys ((heads_q + heads_k) * D, B), normed by head where asked, and turned by the positions of their columns."""
+        self._ck(self.lib.so_head_rotary(self.h, TYPE[type], heads_q, heads_k, D, B, _at(dX), B if x_stride is None else x_stride, int(norm), _at(dGainQ), _at(dGainK), eps, _at(dPos), _at(dFreq),
+                                         rot, amplitude, ROTARY[layout], _at(dY), B if y_stride is None else y_stride, _at(dRstd)))
+
+    def head_rotary_grad(self, dX, dDy, heads_q, heads_k, D, B, dPos, dFreq, rot, dDx, layout="halves", amplitude=1.0, norm=False, dGainQ=None, dGainK=None, dRstd=None, dDgainQ=None, dDgainK=None,
+                         type="f32", x_stride=None, dy_stride=None, dx_stride=None):
+        self._ck(self.lib.so_head_rotary_grad(self.h, TYPE[type], heads_q, heads_k, D, B, _at(dX), B if x_stride is None else x_stride, _at(dDy), B if dy_stride is None else dy_stride, int(norm),
+                                              _at(dGainQ), _at(dGainK), _at(dRstd), _at(dPos), _at(dFreq), rot, amplitude, ROTARY[layout], _at(dDx), B if dx_stride is None else dx_stride,
+                                              _at(dDgainQ), _at(dDgainK)))
+
+    def head_rotary_reserve(self, heads_q, heads_k, D, B, type="f32"):
+        self._ck(self.lib.so_head_rotary_reserve(self.h, TYPE[type], heads_q, heads_k, D, B))
 
     def conv_plan(self, E, geom):
         h = _vp()
