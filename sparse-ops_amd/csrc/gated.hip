@@ -1,39 +1,14 @@
 // The gated feed-forward block: both projections, the activation and the product, and their gradients.
+#include "dense.h"
 #include "gate.h"
 
 namespace {
 
-constexpr int kTile = 64, kDeep = 16, kThreads = 256;
+using so_dense::f32x4;
+using so_dense::Grid;
+using so_dense::Operand;
 
-// One operand of a product: entry (i, k) at p[i * ld + k], or at p[k * ld + i] where it lies across the contraction.
-template <class T> struct Operand { const T *p; size_t ld; };
-
-// acc[a][b] += sum over k of A(row 4 ty + a, k) B(column 4 tx + b, k), from tiles of 64 x 16 of both in LDS.
-template <class T, bool AX, bool BX>
-__device__ void add_product(float (&acc)[4][4], Operand<T> A, Operand<T> B, uint64_t i0, uint64_t rows, uint64_t j0, uint64_t cols, uint32_t K, float (*a)[kTile + 1], float (*b)[kTile + 1])
-{
-    const uint32_t ty = threadIdx.x / 16u, tx = threadIdx.x % 16u;
-    const auto bring = [&](auto across, const Operand<T> &M, uint64_t at, uint64_t end, uint32_t k0, float (*to)[kTile + 1]) {
-        for (uint32_t e = threadIdx.x; e < kTile * kDeep; e += kThreads) {
-            const uint32_t i = decltype(across)::value ? e % kTile : e / kDeep, k = decltype(across)::value ? e / kTile : e % kDeep;
-            float v = 0.0f;
-            if (at + i < end && (uint64_t)k0 + k < K) v = (float)(decltype(across)::value ? M.p[((size_t)k0 + k) * M.ld + at + i] : M.p[(size_t)(at + i) * M.ld + k0 + k]);
-            to[k][i] = v;
-        }
-    };
-    for (uint32_t k0 = 0; k0 < K; k0 += kDeep) {
-        __syncthreads();
-        bring(std::integral_constant<bool, AX>(), A, i0, rows, k0, a);
-        bring(std::integral_constant<bool, BX>(), B, j0, cols, k0, b);
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kDeep; ++k)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[r][c] = fmaf(a[k][4 * ty + r], b[k][4 * tx + c], acc[r][c]);
-    }
-}
+constexpr int kThreads = 256;
 
 template <class T> struct Forward {
     const T *Wg, *Wu, *X, *G0, *U0;
@@ -43,27 +18,47 @@ template <class T> struct Forward {
     int act;
 };
 
+// The results of V neighbouring columns of a row from its two sums.
 template <class T>
-__global__ __launch_bounds__(kThreads)
-void gated_kernel(Forward<T> f)
+__device__ __forceinline__ void finish(const Forward<T> &f, uint64_t row, uint64_t col, float (&g)[so_elements<T>::V], float (&u)[so_elements<T>::V])
 {
-    __shared__ float a[kDeep][kTile + 1], b[kDeep][kTile + 1];
-    const uint32_t across = (f.B + kTile - 1u) / kTile;
-    const uint64_t i0 = (uint64_t)(blockIdx.x / across) * kTile, j0 = (uint64_t)(blockIdx.x % across) * kTile;
-    float g[4][4] = {}, u[4][4] = {};
-    add_product<T, false, true>(g, {f.Wg, f.ldw}, {f.X, f.ldx}, i0, f.m, j0, f.B, f.n, a, b);
-    add_product<T, false, true>(u, {f.Wu, f.ldw}, {f.X, f.ldx}, i0, f.m, j0, f.B, f.n, a, b);
+    constexpr int V = so_elements<T>::V;
+    if (row >= f.m || col >= f.B) return;
+    const uint32_t left = (uint32_t)min((uint64_t)V, f.B - col);
+    if (f.G0) {
+        const auto v = so_group_load(f.G0 + row * f.ld0 + col, left);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+        for (int e = 0; e < V; ++e) g[e] += (float)v[e];
+    }
+    if (f.U0) {
+        const auto v = so_group_load(f.U0 + row * f.ld0 + col, left);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const uint64_t row = i0 + threadIdx.x / 16u * 4u + r, col = j0 + threadIdx.x % 16u * 4u + c;
-            if (row >= f.m || col >= f.B) continue;
-            const float gs = g[r][c] + (f.G0 ? (float)f.G0[row * f.ld0 + col] : 0.0f), us = u[r][c] + (f.U0 ? (float)f.U0[row * f.ld0 + col] : 0.0f);
-            f.H[row * f.ldh + col] = (T)(so_gate::value(f.act, gs) * us);
-            if (f.G) f.G[row * f.ldg + col] = (T)gs;
-            if (f.U) f.U[row * f.ldg + col] = (T)us;
-        }
+        for (int e = 0; e < V; ++e) u[e] += (float)v[e];
+    }
+    if (f.G) so_group_store(f.G + row * f.ldg + col, left, g);
+    if (f.U) so_group_store(f.U + row * f.ldg + col, left, u);
+#pragma unroll
+    for (int e = 0; e < V; ++e) g[e] = so_gate::value(f.act, g[e]) * u[e];
+    so_group_store(f.H + row * f.ldh + col, left, g);
+}
+
+// A tile of both projections: half of its rows are the gate's, half the other's, so that every wave holds both sums of its part of H.
+template <class T, class TILE>
+__global__ __launch_bounds__(TILE::THREADS)
+void gated_kernel(Forward<T> f, Grid grid)
+{
+    extern __shared__ char stage[];
+    const auto spot = so_dense::spot_of(grid);
+    if (spot.none) return;
+    constexpr int HALF = TILE::RT / 2;
+    so_dense::Loop<T, TILE, false, true, true> loop;
+    const uint64_t i0 = (uint64_t)spot.m * (TILE::ROWS / 2), j0 = (uint64_t)spot.c * TILE::COLS;
+    loop.add(stage, {{f.Wg, f.ldw, f.m, f.n}, {f.Wu, f.ldw, f.m, f.n}}, i0, {f.X, f.ldx, f.B, f.n}, j0);
+    __syncthreads();
+    const uint64_t row0 = i0 + threadIdx.x / 64u / TILE::WC * (HALF * 16);
+#pragma unroll
+    for (int i = 0; i < HALF; ++i)
+        loop.out(stage, {i, HALF + i}, [&](uint32_t r, uint32_t c, float (&v)[2][so_elements<T>::V]) { finish(f, row0 + i * 16 + r, j0 + c, v[0], v[1]); });
 }
 
 template <class T>
@@ -79,27 +74,83 @@ void gated_slopes_kernel(uint32_t m, uint32_t B, int act, const T *G, const T *U
     if (dU) dU[row * ldd + col] = (T)(h * s.value);
 }
 
-// Y = A1 B1 (+ A2 B2).
-template <class T, bool AX, bool BX>
-__global__ __launch_bounds__(kThreads)
-void product_kernel(Operand<T> A1, Operand<T> B1, Operand<T> A2, Operand<T> B2, uint32_t rows, uint32_t cols, uint32_t K, T *Y, size_t ldy)
+// Y = A[0] B[0] + A[1] B[1], or either's rows one after the other where the result has two parts (Y2 is not null).
+template <class T> struct Product {
+    Operand<T> A[2], B[2];
+    T *Y, *Y2;
+    size_t ldy;
+    uint32_t rows, cols, terms;      // of one part; products to add
+};
+
+template <class T, class TILE, bool AX, bool BX>
+__global__ __launch_bounds__(TILE::THREADS)
+void product_kernel(Product<T> p, Grid grid)
 {
-    __shared__ float a[kDeep][kTile + 1], b[kDeep][kTile + 1];
-    const uint32_t across = (cols + kTile - 1u) / kTile;
-    const uint64_t i0 = (uint64_t)(blockIdx.x / across) * kTile, j0 = (uint64_t)(blockIdx.x % across) * kTile;
-    float acc[4][4] = {};
-    add_product<T, AX, BX>(acc, A1, B1, i0, rows, j0, cols, K, a, b);
-    if (A2.p) add_product<T, AX, BX>(acc, A2, B2, i0, rows, j0, cols, K, a, b);
+    extern __shared__ char stage[];
+    const auto spot = so_dense::spot_of(grid);
+    if (spot.none) return;
+    const uint32_t each = (p.rows + TILE::ROWS - 1u) / TILE::ROWS, second = spot.m >= each ? 1u : 0u;
+    so_dense::Loop<T, TILE, AX, BX, false> loop;
+    const uint64_t i0 = (uint64_t)(spot.m - second * each) * TILE::ROWS, j0 = (uint64_t)spot.c * TILE::COLS;
+    for (uint32_t t = 0; t < p.terms; ++t) loop.add(stage, {p.A[second + t]}, i0, p.B[second + t], j0);
+    __syncthreads();
+    T *Y = second ? p.Y2 : p.Y;
+    const uint64_t row0 = i0 + threadIdx.x / 64u / TILE::WC * (TILE::RT * 16);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const uint64_t row = i0 + threadIdx.x / 16u * 4u + r, col = j0 + threadIdx.x % 16u * 4u + c;
-            if (row < rows && col < cols) Y[row * ldy + col] = (T)acc[r][c];
-        }
+    for (int i = 0; i < TILE::RT; ++i)
+        loop.out(stage, {i}, [&](uint32_t r, uint32_t c, float (&v)[1][so_elements<T>::V]) {
+            const uint64_t row = row0 + i * 16 + r, col = j0 + c;
+            if (row < p.rows && col < p.cols) so_group_store(Y + row * p.ldy + col, (uint32_t)min((uint64_t)so_elements<T>::V, p.cols - col), v[0]);
+        });
 }
 
-uint64_t tiles(uint32_t rows, uint32_t cols) { return (uint64_t)so_ceil_div(rows, kTile) * so_ceil_div(cols, kTile); }
+// Tiles, by rows and columns of the result (of both projections together in the forward pass).
+typedef so_dense::Tile<8, 4, 2, 4, 64, 4> Large;        // 256 x 256
+typedef so_dense::Tile<4, 4, 2, 2, 64, 4> Middle;       // 128 x 128
+typedef so_dense::Tile<2, 2, 2, 2, 128, 4> Small;       // 64 x 64
+typedef so_dense::Tile<2, 1, 2, 2, 128, 5> Narrow;      // 64 x 32
+
+// f(a tile): the largest that gives every compute unit a workgroup.
+template <class F>
+so_status for_tile(const so_ctx *ctx, uint64_t rows, uint64_t cols, F &&f)
+{
+    const uint64_t cus = (uint64_t)ctx->compute_units;
+    const auto tiles = [&](uint32_t r, uint32_t c) { return (uint64_t)so_ceil_div(rows, r) * so_ceil_div(cols, c); };
+    if (cols > 128 && tiles(256, 256) >= cus) return f(Large());
+    if (cols > 64 && tiles(128, 128) >= cus) return f(Middle());
+    if (cols > 32) return f(Small());
+    return f(Narrow());
+}
+
+template <class TILE, class Kernel, class Arg>
+so_status launch_tiles(so_ctx *ctx, const char *who, Kernel kernel, const Arg &arg, uint64_t mgroups, uint64_t cgroups)
+{
+    SO_REQUIRE(so_grid_fits(mgroups * cgroups + 8, TILE::THREADS), "%s: the result is too large for one launch", who);
+    const Grid g = so_dense::grid_of(mgroups, cgroups);
+    SO_HIP(so_allow_big_lds(ctx, (const void *)kernel));
+    kernel<<<g.groups(), TILE::THREADS, TILE::lds, ctx->stream>>>(arg, g);
+    SO_LAUNCH_CHECK();
+    return SO_OK;
+}
+
+template <class T>
+so_status forward(so_ctx *ctx, const Forward<T> &f)
+{
+    return for_tile(ctx, 2 * (uint64_t)f.m, f.B, [&](auto t) {
+        typedef decltype(t) TILE;
+        return launch_tiles<TILE>(ctx, "so_gated", gated_kernel<T, TILE>, f, so_ceil_div(f.m, TILE::ROWS / 2), so_ceil_div(f.B, TILE::COLS));
+    });
+}
+
+template <class T, bool AX, bool BX>
+so_status product(so_ctx *ctx, const Product<T> &p)
+{
+    const uint32_t parts = p.Y2 ? 2 : 1;
+    return for_tile(ctx, (uint64_t)parts * p.rows, p.cols, [&](auto t) {
+        typedef decltype(t) TILE;
+        return launch_tiles<TILE>(ctx, "so_gated_grad", product_kernel<T, TILE, AX, BX>, p, (uint64_t)parts * so_ceil_div(p.rows, TILE::ROWS), so_ceil_div(p.cols, TILE::COLS));
+    });
+}
 
 size_t grad_bytes(int type, uint32_t m, uint32_t B) { return 2 * (size_t)m * B * so_type_bytes(type); }
 
@@ -140,16 +191,15 @@ extern "C" so_status so_gated(so_ctx *ctx, int type, uint32_t m, uint32_t n, uin
     SO_REQUIRE(dH != dG && dH != dU && (!dG || dG != dU), "so_gated: one array for two results");
     SO_REQUIRE(dH != dG0 && dH != dU0 && (!dG || dG != dU0) && (!dU || dU != dG0), "so_gated: a result is an input");
     SO_REQUIRE(!((dG && dG == dG0) || (dU && dU == dU0)) || g_stride == g0_stride, "so_gated: in place needs one stride");
-    SO_REQUIRE(so_grid_fits(tiles(m, B), kThreads), "so_gated: %u x %u is too large for one launch", m, B);
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
+    so_status status = SO_OK;
     so_for_type(type, [&](auto t) {
         using T = decltype(t);
-        gated_kernel<T><<<(uint32_t)tiles(m, B), kThreads, 0, ctx->stream>>>({(const T *)dWg, (const T *)dWu, (const T *)dX, (const T *)dG0, (const T *)dU0, (T *)dH, (T *)dG, (T *)dU, w_stride,
-                                                                             x_stride, g0_stride, h_stride, g_stride, m, n, B, act});
+        status = forward<T>(ctx, {(const T *)dWg, (const T *)dWu, (const T *)dX, (const T *)dG0, (const T *)dU0, (T *)dH, (T *)dG, (T *)dU, w_stride, x_stride, g0_stride, h_stride, g_stride,
+                                  m, n, B, act});
     });
-    SO_LAUNCH_CHECK();
-    return SO_OK;
+    return status;
 }
 
 extern "C" so_status so_gated_grad(so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t B, const void *dWg, const void *dWu, size_t w_stride, const void *dX, size_t x_stride, int act,
@@ -168,7 +218,7 @@ extern "C" so_status so_gated_grad(so_ctx *ctx, int type, uint32_t m, uint32_t n
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
     const uint64_t slopes = so_ceil_div((uint64_t)m * B, kThreads);
-    SO_REQUIRE((uint64_t)m * B < (1ull << 32) - kThreads && so_grid_fits(tiles(n, B), kThreads) && so_grid_fits(tiles(m, n), kThreads), "so_gated_grad: %u x %u x %u is too large for one launch", m, n, B);
+    SO_REQUIRE((uint64_t)m * B < (1ull << 32) - kThreads, "so_gated_grad: %u x %u is too large for one launch", m, B);
     if (m > 0 && B > 0) {
         SO_REQUIRE(dG && dU && dDh, "so_gated_grad: null tensor");
         SO_REQUIRE(!dDx || (dWg && dWu), "so_gated_grad: null weights");
@@ -197,9 +247,11 @@ extern "C" so_status so_gated_grad(so_ctx *ctx, int type, uint32_t m, uint32_t n
         }
         if (m && B) gated_slopes_kernel<T><<<(uint32_t)slopes, kThreads, 0, ctx->stream>>>(m, B, act, (const T *)dG, (const T *)dU, g_stride, (const T *)dDh, dh_stride, g, u, ldg);
         if (dDx && B)
-            product_kernel<T, true, true><<<(uint32_t)tiles(n, B), kThreads, 0, ctx->stream>>>({(const T *)dWg, w_stride}, {g, ldg}, {(const T *)dWu, w_stride}, {u, ldu}, n, B, m, (T *)dDx, dx_stride);
-        if (dDwg && m) product_kernel<T, false, false><<<(uint32_t)tiles(m, n), kThreads, 0, ctx->stream>>>({g, ldg}, {(const T *)dX, x_stride}, {nullptr, 0}, {nullptr, 0}, m, n, B, (T *)dDwg, dw_stride);
-        if (dDwu && m) product_kernel<T, false, false><<<(uint32_t)tiles(m, n), kThreads, 0, ctx->stream>>>({u, ldu}, {(const T *)dX, x_stride}, {nullptr, 0}, {nullptr, 0}, m, n, B, (T *)dDwu, dw_stride);
+            status = product<T, true, true>(ctx, {{{(const T *)dWg, w_stride, n, m}, {(const T *)dWu, w_stride, n, m}}, {{g, ldg, B, m}, {u, ldu, B, m}}, (T *)dDx, nullptr, dx_stride, n, B, 2});
+        const Operand<T> x = {(const T *)dX, x_stride, n, B}, dg = {g, ldg, m, B}, du = {u, ldu, m, B};
+        if (status == SO_OK && m && dDwg && dDwu) status = product<T, false, false>(ctx, {{dg, du}, {x, x}, (T *)dDwg, (T *)dDwu, dw_stride, m, n, 1});
+        else if (status == SO_OK && m && weights) status = product<T, false, false>(ctx, {{dDwg ? dg : du, du}, {x, x}, (T *)(dDwg ? dDwg : dDwu), nullptr, dw_stride, m, n, 1});
+        if (status != SO_OK) return;
         if ((dDg && g != (T *)dDg) || (dDu && u != (T *)dDu)) {      // one of the two asked for
             gated_slopes_kernel<T><<<(uint32_t)slopes, kThreads, 0, ctx->stream>>>(m, B, act, (const T *)dG, (const T *)dU, g_stride, (const T *)dDh, dh_stride, (T *)dDg, (T *)dDu, dg_stride);
         }

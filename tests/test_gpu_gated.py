@@ -68,6 +68,18 @@ def test_forward(ctx, m, n, B, type_):
         run_forward(ctx, rng, m, n, B, type_, ACTS[(m + n + B + i) % len(ACTS)], pad, shift, wpad=(0, 5, 8)[i])
 
 
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("m,n,B", [(70, 75, 3), (66, 261, 21), (130, 517, 129), (301, 131, 267), (517, 1029, 35)])
+def test_rows_that_are_aligned_and_end_inside_a_group(ctx, m, n, B, type_):
+    """Every row begins at a multiple of 16 bytes, and ends at none; the last one is the end of its array."""
+    rng = np.random.default_rng(m + n + B)
+    up = lambda v: -v % 8
+    for make in (lambda pad, wpad: run_forward(ctx, rng, m, n, B, type_, "silu", pad, 0, wpad), lambda pad, wpad: run_backward(ctx, rng, m, n, B, type_, "silu", pad, 0, wpad)):
+        make(up(B), up(n))
+        make(up(B), 0)
+        make(0, up(n))
+
+
 @pytest.mark.parametrize("act", ACTS)
 def test_forward_of_every_activation(ctx, act):
     rng = np.random.default_rng(5)
