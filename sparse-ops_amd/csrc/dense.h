@@ -37,6 +37,8 @@ template <class T> struct Operand {
     const T *p;
     size_t ld;
     uint32_t own, depth;
+    // Whether it can go to LDS past the registers: groups of 16 bytes, and the offsets of a step's 256 rows at most in 31 bits.
+    bool direct() const { return ((uintptr_t)p | ld * sizeof(T)) % 16 == 0 && (uint64_t)ld * sizeof(T) * 256 < (1ull << 31); }
 };
 
 // LEN entries of an operand's own index times KB bytes of the contraction in LDS, brought by WAVES waves.
@@ -59,7 +61,6 @@ struct Side {
     const T *at;             // entry (i0, 0)
     size_t ld;
     uint32_t own, depth;     // from i0 on
-    bool direct;             // past the registers
     uint32_t from[ASKS];     // byte offsets of this lane's groups, of a step
     __device__ __forceinline__ void start(const Operand<T> &m, uint64_t i0)
     {
@@ -67,7 +68,6 @@ struct Side {
         ld = m.ld;
         own = (uint32_t)(m.own - i0);
         depth = m.depth;
-        direct = ((uintptr_t)m.p | m.ld * E) % 16 == 0 && (uint64_t)m.ld * E * ROWS < (1ull << 31);
         const uint32_t wave = threadIdx.x / 64u, lane = threadIdx.x % 64u;
 #pragma unroll
         for (int a = 0; a < ASKS; ++a) {
@@ -80,18 +80,21 @@ struct Side {
     __device__ __forceinline__ bool whole(uint32_t step) const
     {
         const uint64_t end = (uint64_t)(step + 1u) * BK;
-        return direct && end <= depth && (!ACROSS || own >= (uint32_t)LEN || own % V == 0 || end < depth);
+        return end <= depth && (!ACROSS || own >= (uint32_t)LEN || own % V == 0 || end < depth);
     }
-    // Such a step to LDS at `to`.  Whole rows beyond `own` are kept off by the buffer's size.
-    __device__ __forceinline__ void bring(uint32_t step, uint32_t to) const
+    // Request `piece` of this wave for such a step, or all of them, straight to LDS at `to`.  Whole rows beyond `own` are kept off by the buffer's size.
+    __device__ __forceinline__ void bring(uint32_t step, uint32_t to, int piece) const
     {
         const char *base = reinterpret_cast<const char *>(at) + (ACROSS ? (size_t)step * BK * ld : (size_t)step * BK) * E;
         const uint64_t left = ((uint64_t)(ACROSS ? depth - step * BK - 1u : own - 1u) * ld + (ACROSS ? own : depth - step * BK)) * E;
         const u32x4 buffer = {(uint32_t)(uintptr_t)base, (uint32_t)((uintptr_t)base >> 32) & 0xffffu, (uint32_t)min(left, (uint64_t)0xfffffffcu), 0x00020000u};
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(to + (piece * WAVES + wave) * 1024u), "v"(from[piece]), "s"(buffer) : "memory", "m0");
+    }
+    __device__ __forceinline__ void bring(uint32_t step, uint32_t to) const
+    {
 #pragma unroll
-        for (int a = 0; a < ASKS; ++a)
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(to + (a * WAVES + wave) * 1024u), "v"(from[a]), "s"(buffer) : "memory", "m0");
+        for (int p = 0; p < ASKS; ++p) bring(step, to, p);
     }
     // Any step, by way of registers: what does not exist is zero.
     __device__ __forceinline__ void ask(uint32_t step, u32x4 (&r)[ASKS]) const
@@ -174,46 +177,141 @@ struct Loop {
 #pragma unroll
             for (int k = 0; k < CT; ++k) acc[i][k] = f32x4{};
     }
-    // acc += the product of rows from i0 on (of both operands, with HALVES) and columns from j0 on.
-    __device__ __forceinline__ void add(char *stage, const Operand<T> (&A)[PARTS], uint64_t i0, const Operand<T> &B, uint64_t j0)
+    SideA a[PARTS];
+    SideB b;
+    typename SideA::template Reader<RT> ra;
+    typename SideB::template Reader<CT> rb;
+    __device__ __forceinline__ void start(const Operand<T> (&A)[PARTS], uint64_t i0, const Operand<T> &B, uint64_t j0)
     {
-        SideA a[PARTS];
-        SideB b;
 #pragma unroll
         for (int h = 0; h < PARTS; ++h) a[h].start(A[h], i0);
         b.start(B, j0);
+        const uint32_t wave = threadIdx.x / 64u;
+        ra.start(wave / WC * (RT / PARTS));
+        rb.start(wave % WC * CT);
+    }
+    __device__ __forceinline__ u32x4 row_tile(const char *slot, int i, int q) const { return ra.get(slot + (HALVES && i >= RT / 2 ? SideA::BYTES : 0), HALVES ? i % (RT / 2) : i, q); }
+    struct Asked { u32x4 a[PARTS][SideA::ASKS], b[SideB::ASKS]; };
+    __device__ __forceinline__ void ask(uint32_t step, Asked &w) const
+    {
+#pragma unroll
+        for (int h = 0; h < PARTS; ++h) a[h].ask(step, w.a[h]);
+        b.ask(step, w.b);
+    }
+    static __device__ __forceinline__ void put(char *slot, const Asked &w)
+    {
+#pragma unroll
+        for (int h = 0; h < PARTS; ++h) SideA::put(slot + h * SideA::BYTES, w.a[h]);
+        SideB::put(slot + B0, w.b);
+    }
+
+    // acc += the product of rows from i0 on (of both operands, with HALVES) and columns from j0 on, both operands aligned.  All steps go straight to LDS, but for a last one that is not whole.
+    // A run (64 bytes of k) is multiplied from registers while the next one's operands are read: those of the rows into a second set, those of the columns into the places that have been multiplied
+    // for the last time.  Once a step's last run is in registers its place in the ring is free for the step that comes RING later, whose requests go out one by one between the products.
+    __device__ __forceinline__ void add_direct(char *stage)
+    {
+        constexpr int Q = KB / 64;
+        static_assert(Q == 1 || Q == 2, "runs of a step");
         const uint32_t steps = b.steps(), lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)stage;
-        const uint32_t wave = threadIdx.x / 64u, wm = wave / WC, wc = wave % WC;
-        typename SideA::template Reader<RT> ra;
-        typename SideB::template Reader<CT> rb;
-        ra.start(wm * (RT / PARTS));
-        rb.start(wc * CT);
-        const bool direct = a[0].direct && a[PARTS - 1].direct && b.direct;
-        u32x4 wa[PARTS][SideA::ASKS], wb[SideB::ASKS];
-        const auto bring = [&](uint32_t step) {
-            const uint32_t to = step % RING * STAGE;
+        uint32_t whole = steps;
+        if (steps && !(a[0].whole(steps - 1u) && b.whole(steps - 1u))) whole = steps - 1u;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");      // what an earlier call has in LDS is read
+        if (!steps) return;
+        Asked last;
+        if (whole < steps && whole < RING) ask(whole, last);
+        const auto bring_all = [&](uint32_t step) {
 #pragma unroll
-            for (int h = 0; h < PARTS; ++h) {
-                if (a[h].whole(step)) a[h].bring(step, lds0 + to + h * SideA::BYTES);
-                else a[h].ask(step, wa[h]);
+            for (int h = 0; h < PARTS; ++h) a[h].bring(step, lds0 + step % RING * STAGE + h * SideA::BYTES);
+            b.bring(step, lds0 + step % RING * STAGE + B0);
+        };
+        for (uint32_t s = 0; s < RING && s < whole; ++s) bring_all(s);
+        if (whole < steps && whole < RING) put(stage + whole % RING * STAGE, last);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+        u32x4 x[2][RT], y[CT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) x[0][i] = row_tile(stage, i, 0);
+#pragma unroll
+        for (int k = 0; k < CT; ++k) y[k] = rb.get(stage + B0, k, 0);
+        // Run `run` of a step; SET: which set of the rows' operands it has.  STREAM: the step that comes RING later exists, and all before it.
+        const auto multiply_run = [&](uint32_t step, auto run, auto set, auto stream) {
+            constexpr int R = decltype(run)::value, SET = decltype(set)::value, NEXT = (R + 1) % Q;
+            constexpr bool STREAM = decltype(stream)::value, END = R + 1 == Q;
+            if constexpr (END) {
+                // the next step is there, and all waves have this one in registers
+                if constexpr (STREAM) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(ASKS * (RING - 2)) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+                if constexpr (!STREAM) {
+                    if (whole < steps && step + RING == whole) {
+                        ask(whole, last);
+                        put(stage + step % RING * STAGE, last);
+                    }
+                    if (step + RING < whole) bring_all(step + RING);
+                }
             }
-            if (b.whole(step)) b.bring(step, lds0 + to + B0);
-            else b.ask(step, wb);
-        };
-        const auto settle = [&](uint32_t step) {
-            char *to = stage + step % RING * STAGE;
+            const char *next = stage + (END ? step + 1u : step) % RING * STAGE;      // behind the last step: an older one, for nothing
 #pragma unroll
-            for (int h = 0; h < PARTS; ++h)
-                if (!a[h].whole(step)) SideA::put(to + h * SideA::BYTES, wa[h]);
-            if (!b.whole(step)) SideB::put(to + B0, wb);
+            for (int i = 0; i < RT; ++i) x[1 - SET][i] = row_tile(next, i, NEXT);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < CT; ++k) {
+#pragma unroll
+                for (int i = 0; i < RT; ++i) acc[i][k] = multiply<T>(x[SET][i], y[k], acc[i][k]);
+                y[k] = rb.get(next + B0, k, NEXT);
+                if constexpr (END && STREAM) {
+                    const uint32_t to = lds0 + step % RING * STAGE;
+#pragma unroll
+                    for (int p = k * ASKS / CT; p < (k + 1) * ASKS / CT; ++p) {
+                        if (p < SideA::ASKS * PARTS) a[p / SideA::ASKS].bring(step + RING, to + p / SideA::ASKS * SideA::BYTES, p % SideA::ASKS);
+                        else b.bring(step + RING, to + B0, p - SideA::ASKS * PARTS);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         };
-        const auto compute = [&](uint32_t step) {
-            const char *slot = stage + step % RING * STAGE;
+        const std::integral_constant<int, 0> zero;
+        const std::integral_constant<int, 1> one;
+        const std::true_type yes;
+        const std::false_type no;
+        uint32_t s = 0;
+        if constexpr (Q == 2) {
+            for (; s + RING < whole; ++s) {
+                multiply_run(s, zero, zero, yes);
+                multiply_run(s, one, one, yes);
+            }
+            for (; s < steps; ++s) {
+                multiply_run(s, zero, zero, no);
+                multiply_run(s, one, one, no);
+            }
+        } else {
+            for (; s + 1u + RING < whole; s += 2u) {
+                multiply_run(s, zero, zero, yes);
+                multiply_run(s + 1u, zero, one, yes);
+            }
+            for (; s < steps; s += 2u) {
+                multiply_run(s, zero, zero, no);
+                if (s + 1u < steps) multiply_run(s + 1u, zero, one, no);
+            }
+        }
+    }
+
+    // The same for operands at any address: a step is asked for while the one before it is multiplied, and put into LDS behind that.
+    __device__ __forceinline__ void add_any(char *stage)
+    {
+        const uint32_t steps = b.steps();
+        __syncthreads();
+        if (!steps) return;
+        Asked w;
+        ask(0, w);
+        put(stage, w);
+        for (uint32_t s = 0; s < steps; ++s) {
+            __syncthreads();
+            if (s + 1u < steps) ask(s + 1u, w);
+            const char *slot = stage + s % 2u * STAGE;
 #pragma unroll
             for (int q = 0; q < KB / 64; ++q) {
                 u32x4 x[RT], y[CT];
 #pragma unroll
-                for (int i = 0; i < RT; ++i) x[i] = ra.get(slot + (HALVES && i >= RT / 2 ? SideA::BYTES : 0), HALVES ? i % (RT / 2) : i, q);
+                for (int i = 0; i < RT; ++i) x[i] = row_tile(slot, i, q);
 #pragma unroll
                 for (int k = 0; k < CT; ++k) y[k] = rb.get(slot + B0, k, q);
 #pragma unroll
@@ -221,54 +319,51 @@ struct Loop {
 #pragma unroll
                     for (int i = 0; i < RT; ++i) acc[i][k] = multiply<T>(x[i], y[k], acc[i][k]);
             }
-        };
-        // what an earlier call has in LDS is read
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-        for (uint32_t s = 0; s < RING - 1u && s < steps; ++s) {
-            bring(s);
-            settle(s);
-        }
-        uint32_t s = 0;
-        for (; s + RING - 1u < steps; ++s) {
-            // step s is there (only what later steps asked for may still be on its way), and all waves are done with step s - 1
-            if (direct) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(ASKS * (RING - 2)) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-            bring(s + RING - 1u);
-            compute(s);
-            settle(s + RING - 1u);
-        }
-        for (; s < steps; ++s) {
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-            compute(s);
+            if (s + 1u < steps) put(stage + (s + 1u) % 2u * STAGE, w);
         }
     }
-    // f(row, column, values) for each group of V neighbouring results of 16 (or 32) rows, those of tiles i .. of acc, by way of LDS; rows and columns within the tile's.
-    template <int N, class F>
-    __device__ __forceinline__ void out(char *stage, const int (&tiles)[N], F &&f) const
+    template <bool DIRECT>
+    __device__ __forceinline__ void add(char *stage, const Operand<T> (&A)[PARTS], uint64_t i0, const Operand<T> &B, uint64_t j0)
     {
-        constexpr int V = so_elements<T>::V, PITCH = TILE::OUT_PITCH, LANES = CT * 16 / V, ROWS = 64 / LANES;
+        start(A, i0, B, j0);
+        if constexpr (DIRECT) add_direct(stage);
+        else add_any(stage);
+    }
+    // f(i, row, column, values) for each group of V neighbouring results of tile i of the wave's N x RT / N tiles of rows, i running over RT / N, by way of LDS: rows within a tile of 16, columns within the
+    // workgroup's; the values of tile i, of tile i + RT / N and so on.  One copy of f's code, whatever RT is.
+    template <int N, class F>
+    __device__ __forceinline__ void out(char *stage, F &&f) const
+    {
+        constexpr int V = so_elements<T>::V, PITCH = TILE::OUT_PITCH, LANES = CT * 16 / V, ROWS = 64 / LANES, EACH = RT / N;
         float *mine = reinterpret_cast<float *>(stage) + threadIdx.x / 64u * 32u * PITCH;
         const uint32_t lane = threadIdx.x % 64u;
+#pragma unroll 1
+        for (int i = 0; i < EACH; ++i) {
 #pragma unroll
-        for (int j = 0; j < N; ++j)
+            for (int t = 0; t < EACH; ++t)
+                if (t == i) {
 #pragma unroll
-            for (int k = 0; k < CT; ++k) *reinterpret_cast<f32x4 *>(mine + (j * 16 + lane % 16u) * PITCH + k * 16 + 4 * (lane / 16u)) = acc[tiles[j]][k];
-        __builtin_amdgcn_wave_barrier();
+                    for (int j = 0; j < N; ++j)
 #pragma unroll
-        for (int r0 = 0; r0 < 16; r0 += ROWS < 16 ? ROWS : 16) {
-            const uint32_t r = r0 + lane / LANES;
-            float v[N][V];
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-#pragma unroll
-                for (int e = 0; e < V; e += 4) {
-                    const f32x4 s = *reinterpret_cast<const f32x4 *>(mine + (j * 16 + r % 16u) * PITCH + lane % LANES * V + e);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) v[j][e + c] = s[c];
+                        for (int k = 0; k < CT; ++k) *reinterpret_cast<f32x4 *>(mine + (j * 16 + lane % 16u) * PITCH + k * 16 + 4 * (lane / 16u)) = acc[j * EACH + t][k];
                 }
-            if (r < 16u) f(r, (uint32_t)(threadIdx.x / 64u % WC) * (CT * 16) + lane % LANES * V, v);
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+            for (int r0 = 0; r0 < 16; r0 += ROWS < 16 ? ROWS : 16) {
+                const uint32_t r = r0 + lane / LANES;
+                float v[N][V];
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+#pragma unroll
+                    for (int e = 0; e < V; e += 4) {
+                        const f32x4 s = *reinterpret_cast<const f32x4 *>(mine + (j * 16 + r % 16u) * PITCH + lane % LANES * V + e);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) v[j][e + c] = s[c];
+                    }
+                if (r < 16u) f(i, r, (uint32_t)(threadIdx.x / 64u % WC) * (CT * 16) + lane % LANES * V, v);
+            }
+            __builtin_amdgcn_wave_barrier();
         }
-        __builtin_amdgcn_wave_barrier();
     }
 };
 

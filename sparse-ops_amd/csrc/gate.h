@@ -19,17 +19,22 @@ constexpr float kRootHalf = 0.70710678f, kRootTwoOverPi = 0.79788456f, kCubic = 
 
 __device__ __forceinline__ float tanh_argument(float v) { return kRootTwoOverPi * fmaf(kCubic * v * v, v, v); }
 
-// The activation is the same for a whole launch, so that the branch on it costs a few scalar instructions.
-__device__ __forceinline__ float value(int act, float v)
+// g[e] = act(g[e]) u[e].  The activation is the same for a whole launch, so that the branch on it costs a few scalar instructions.
+template <int V>
+__device__ __forceinline__ void apply(int act, float (&g)[V], const float (&u)[V])
 {
+    const auto each = [&](auto &&f) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) g[e] = f(g[e]) * u[e];
+    };
     switch (act) {
-    case SO_ACT_RELU: return v <= 0.0f ? 0.0f : v;
-    case SO_ACT_SIGMOID: return logistic(v).of;
-    case SO_ACT_TANH: return tanhf(v);
-    case SO_ACT_SILU: return v * logistic(v).of;
-    case SO_ACT_GELU: return 0.5f * v * erfcf(-kRootHalf * v);
-    case SO_ACT_GELU_TANH: return v * logistic(2.0f * tanh_argument(v)).of;
-    default: return v;
+    case SO_ACT_RELU: return each([](float v) { return v <= 0.0f ? 0.0f : v; });
+    case SO_ACT_SIGMOID: return each([](float v) { return logistic(v).of; });
+    case SO_ACT_TANH: return each([](float v) { return tanhf(v); });
+    case SO_ACT_SILU: return each([](float v) { return v * logistic(v).of; });
+    case SO_ACT_GELU: return each([](float v) { return 0.5f * v * erfcf(-kRootHalf * v); });
+    case SO_ACT_GELU_TANH: return each([](float v) { return v * logistic(2.0f * tanh_argument(v)).of; });
+    default: return each([](float v) { return v; });
     }
 }
 

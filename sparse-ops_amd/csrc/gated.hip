@@ -37,28 +37,24 @@ __device__ __forceinline__ void finish(const Forward<T> &f, uint64_t row, uint64
     }
     if (f.G) so_group_store(f.G + row * f.ldg + col, left, g);
     if (f.U) so_group_store(f.U + row * f.ldg + col, left, u);
-#pragma unroll
-    for (int e = 0; e < V; ++e) g[e] = so_gate::value(f.act, g[e]) * u[e];
+    so_gate::apply<V>(f.act, g, u);
     so_group_store(f.H + row * f.ldh + col, left, g);
 }
 
 // A tile of both projections: half of its rows are the gate's, half the other's, so that every wave holds both sums of its part of H.
-template <class T, class TILE>
+template <class T, class TILE, bool DIRECT>
 __global__ __launch_bounds__(TILE::THREADS)
 void gated_kernel(Forward<T> f, Grid grid)
 {
     extern __shared__ char stage[];
     const auto spot = so_dense::spot_of(grid);
     if (spot.none) return;
-    constexpr int HALF = TILE::RT / 2;
     so_dense::Loop<T, TILE, false, true, true> loop;
     const uint64_t i0 = (uint64_t)spot.m * (TILE::ROWS / 2), j0 = (uint64_t)spot.c * TILE::COLS;
-    loop.add(stage, {{f.Wg, f.ldw, f.m, f.n}, {f.Wu, f.ldw, f.m, f.n}}, i0, {f.X, f.ldx, f.B, f.n}, j0);
+    loop.template add<DIRECT>(stage, {{f.Wg, f.ldw, f.m, f.n}, {f.Wu, f.ldw, f.m, f.n}}, i0, {f.X, f.ldx, f.B, f.n}, j0);
     __syncthreads();
-    const uint64_t row0 = i0 + threadIdx.x / 64u / TILE::WC * (HALF * 16);
-#pragma unroll
-    for (int i = 0; i < HALF; ++i)
-        loop.out(stage, {i, HALF + i}, [&](uint32_t r, uint32_t c, float (&v)[2][so_elements<T>::V]) { finish(f, row0 + i * 16 + r, j0 + c, v[0], v[1]); });
+    const uint64_t row0 = i0 + threadIdx.x / 64u / TILE::WC * (TILE::RT / 2 * 16);
+    loop.template out<2>(stage, [&](int i, uint32_t r, uint32_t c, float (&v)[2][so_elements<T>::V]) { finish(f, row0 + i * 16 + r, j0 + c, v[0], v[1]); });
 }
 
 template <class T>
@@ -82,7 +78,7 @@ template <class T> struct Product {
     uint32_t rows, cols, terms;      // of one part; products to add
 };
 
-template <class T, class TILE, bool AX, bool BX>
+template <class T, class TILE, bool AX, bool BX, bool DIRECT>
 __global__ __launch_bounds__(TILE::THREADS)
 void product_kernel(Product<T> p, Grid grid)
 {
@@ -92,16 +88,14 @@ void product_kernel(Product<T> p, Grid grid)
     const uint32_t each = (p.rows + TILE::ROWS - 1u) / TILE::ROWS, second = spot.m >= each ? 1u : 0u;
     so_dense::Loop<T, TILE, AX, BX, false> loop;
     const uint64_t i0 = (uint64_t)(spot.m - second * each) * TILE::ROWS, j0 = (uint64_t)spot.c * TILE::COLS;
-    for (uint32_t t = 0; t < p.terms; ++t) loop.add(stage, {p.A[second + t]}, i0, p.B[second + t], j0);
+    for (uint32_t t = 0; t < p.terms; ++t) loop.template add<DIRECT>(stage, {p.A[second + t]}, i0, p.B[second + t], j0);
     __syncthreads();
     T *Y = second ? p.Y2 : p.Y;
     const uint64_t row0 = i0 + threadIdx.x / 64u / TILE::WC * (TILE::RT * 16);
-#pragma unroll
-    for (int i = 0; i < TILE::RT; ++i)
-        loop.out(stage, {i}, [&](uint32_t r, uint32_t c, float (&v)[1][so_elements<T>::V]) {
-            const uint64_t row = row0 + i * 16 + r, col = j0 + c;
-            if (row < p.rows && col < p.cols) so_group_store(Y + row * p.ldy + col, (uint32_t)min((uint64_t)so_elements<T>::V, p.cols - col), v[0]);
-        });
+    loop.template out<1>(stage, [&](int i, uint32_t r, uint32_t c, float (&v)[1][so_elements<T>::V]) {
+        const uint64_t row = row0 + i * 16 + r, col = j0 + c;
+        if (row < p.rows && col < p.cols) so_group_store(Y + row * p.ldy + col, (uint32_t)min((uint64_t)so_elements<T>::V, p.cols - col), v[0]);
+    });
 }
 
 // Tiles, by rows and columns of the result (of both projections together in the forward pass).
@@ -110,16 +104,19 @@ typedef so_dense::Tile<4, 4, 2, 2, 64, 4> Middle;       // 128 x 128
 typedef so_dense::Tile<2, 2, 2, 2, 128, 4> Small;       // 64 x 64
 typedef so_dense::Tile<2, 1, 2, 2, 128, 5> Narrow;      // 64 x 32
 
-// f(a tile): the largest that gives every compute unit a workgroup.
-template <class F>
-so_status for_tile(const so_ctx *ctx, uint64_t rows, uint64_t cols, F &&f)
+// f(a tile, whether operands go past the registers): the largest that gives every compute unit a workgroup.  fp32 has no use for the largest: its products take four times as long, and 128 x 128 feeds them.
+template <class T, class F>
+so_status for_tile(const so_ctx *ctx, uint64_t rows, uint64_t cols, bool direct, F &&f)
 {
     const uint64_t cus = (uint64_t)ctx->compute_units;
     const auto tiles = [&](uint32_t r, uint32_t c) { return (uint64_t)so_ceil_div(rows, r) * so_ceil_div(cols, c); };
-    if (cols > 128 && tiles(256, 256) >= cus) return f(Large());
-    if (cols > 64 && tiles(128, 128) >= cus) return f(Middle());
-    if (cols > 32) return f(Small());
-    return f(Narrow());
+    const bool middle = cols > 64 && tiles(128, 128) >= cus;
+    if (!direct) return middle ? f(Middle(), std::false_type()) : f(Small(), std::false_type());
+    if constexpr (sizeof(T) == 2)
+        if (cols > 128 && tiles(256, 256) >= cus) return f(Large(), std::true_type());
+    if (middle) return f(Middle(), std::true_type());
+    if (cols > 32) return f(Small(), std::true_type());
+    return f(Narrow(), std::true_type());
 }
 
 template <class TILE, class Kernel, class Arg>
@@ -136,9 +133,10 @@ so_status launch_tiles(so_ctx *ctx, const char *who, Kernel kernel, const Arg &a
 template <class T>
 so_status forward(so_ctx *ctx, const Forward<T> &f)
 {
-    return for_tile(ctx, 2 * (uint64_t)f.m, f.B, [&](auto t) {
+    const Operand<T> g = {f.Wg, f.ldw, f.m, f.n}, u = {f.Wu, f.ldw, f.m, f.n}, x = {f.X, f.ldx, f.B, f.n};
+    return for_tile<T>(ctx, 2 * (uint64_t)f.m, f.B, g.direct() && u.direct() && x.direct(), [&](auto t, auto direct) {
         typedef decltype(t) TILE;
-        return launch_tiles<TILE>(ctx, "so_gated", gated_kernel<T, TILE>, f, so_ceil_div(f.m, TILE::ROWS / 2), so_ceil_div(f.B, TILE::COLS));
+        return launch_tiles<TILE>(ctx, "so_gated", gated_kernel<T, TILE, decltype(direct)::value>, f, so_ceil_div(f.m, TILE::ROWS / 2), so_ceil_div(f.B, TILE::COLS));
     });
 }
 
@@ -146,9 +144,11 @@ template <class T, bool AX, bool BX>
 so_status product(so_ctx *ctx, const Product<T> &p)
 {
     const uint32_t parts = p.Y2 ? 2 : 1;
-    return for_tile(ctx, (uint64_t)parts * p.rows, p.cols, [&](auto t) {
+    bool direct = true;
+    for (uint32_t i = 0; i < std::max(parts, p.terms); ++i) direct = direct && p.A[i].direct() && p.B[i].direct();
+    return for_tile<T>(ctx, (uint64_t)parts * p.rows, p.cols, direct, [&](auto t, auto past) {
         typedef decltype(t) TILE;
-        return launch_tiles<TILE>(ctx, "so_gated_grad", product_kernel<T, TILE, AX, BX>, p, (uint64_t)parts * so_ceil_div(p.rows, TILE::ROWS), so_ceil_div(p.cols, TILE::COLS));
+        return launch_tiles<TILE>(ctx, "so_gated_grad", product_kernel<T, TILE, AX, BX, decltype(past)::value>, p, (uint64_t)parts * so_ceil_div(p.rows, TILE::ROWS), so_ceil_div(p.cols, TILE::COLS));
     });
 }
 
