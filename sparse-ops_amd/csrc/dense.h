@@ -96,29 +96,38 @@ struct Side {
 #pragma unroll
         for (int p = 0; p < ASKS; ++p) bring(step, to, p);
     }
-    // Any step, by way of registers: what does not exist is zero.
+    // Group q of any step, to a register: what does not exist is zero.
+    __device__ __forceinline__ u32x4 group(uint32_t step, uint32_t q) const
+    {
+        const uint32_t row = q / PER, group = q % PER ^ swap(row);
+        const uint64_t k = (uint64_t)step * BK + (ACROSS ? row : group * V), i = ACROSS ? group * V : row;
+        const uint64_t end = ACROSS ? own : depth, along = ACROSS ? i : k;
+        if (!((ACROSS ? k < depth : i < own) && along < end)) return u32x4{};
+        return __builtin_bit_cast(u32x4, so_group_load(at + (ACROSS ? (size_t)k * ld + i : (size_t)i * ld + k), (uint32_t)min(end - along, (uint64_t)V)));
+    }
+    static __device__ __forceinline__ uint32_t group_of(uint32_t a) { return (a * WAVES + threadIdx.x / 64u) * 64u + threadIdx.x % 64u; }
     __device__ __forceinline__ void ask(uint32_t step, u32x4 (&r)[ASKS]) const
     {
 #pragma unroll
-        for (int a = 0; a < ASKS; ++a) {
-            const uint32_t q = (a * WAVES + threadIdx.x / 64u) * 64u + threadIdx.x % 64u, row = q / PER, group = q % PER ^ swap(row);
-            const uint64_t k = (uint64_t)step * BK + (ACROSS ? row : group * V), i = ACROSS ? group * V : row;
-            const uint64_t end = ACROSS ? own : depth, along = ACROSS ? i : k;
-            r[a] = u32x4{};
-            if ((ACROSS ? k < depth : i < own) && along < end)
-                r[a] = __builtin_bit_cast(u32x4, so_group_load(at + (ACROSS ? (size_t)k * ld + i : (size_t)i * ld + k), (uint32_t)min(end - along, (uint64_t)V)));
-        }
+        for (int a = 0; a < ASKS; ++a) r[a] = group(step, group_of(a));
     }
     static __device__ __forceinline__ void put(char *to, const u32x4 (&r)[ASKS])
     {
 #pragma unroll
-        for (int a = 0; a < ASKS; ++a) *reinterpret_cast<u32x4 *>(to + ((a * WAVES + threadIdx.x / 64u) * 64u + threadIdx.x % 64u) * 16u) = r[a];
+        for (int a = 0; a < ASKS; ++a) *reinterpret_cast<u32x4 *>(to + group_of(a) * 16u) = r[a];
+    }
+    // One after the other, in as few registers as can be.
+    __device__ __forceinline__ void settle(uint32_t step, char *to) const
+    {
+#pragma unroll 1
+        for (uint32_t a = 0; a < ASKS; ++a) *reinterpret_cast<u32x4 *>(to + group_of(a) * 16u) = group(step, group_of(a));
     }
 
-    // What a lane reads of tiles of 16 entries, from tile `first` on: get(slot, T, Q) is tile first + T's operand of the step's 64-byte run Q.
+    // What a lane reads of tiles of 16 entries, from tile `first` (a multiple of TILES) on: get(slot, T, Q) is tile first + T's operand of the step's 64-byte run Q.
     template <int TILES>
     struct Reader {
-        uint32_t base[ACROSS ? TILES : KB / 64];
+        static_assert((TILES & (TILES - 1)) == 0, "a tile's place differs from the first's in bits of its own");
+        uint32_t base[ACROSS ? 1 : KB / 64];
         __device__ __forceinline__ void start(uint32_t first)
         {
             const uint32_t l = threadIdx.x % 16u, g = threadIdx.x % 64u / 16u;
@@ -127,8 +136,7 @@ struct Side {
                 for (int q = 0; q < KB / 64; ++q) base[q] = (first * 16u + l) * PITCH + ((4u * q + g) ^ swap(l)) * 16u;
             } else {
                 const uint32_t row = E == 2 ? 8u * g + l / 4u : 4u * g;
-#pragma unroll
-                for (int t = 0; t < TILES; ++t) base[t] = row * PITCH + ((first + t) * (E == 2 ? 32u : 64u) ^ swap(row) * 16u) + (E == 2 ? l % 4u * 8u : l * 4u);
+                base[0] = row * PITCH + (first * (E == 2 ? 32u : 64u) ^ swap(row) * 16u) + (E == 2 ? l % 4u * 8u : l * 4u);
             }
         }
         __device__ __forceinline__ u32x4 get(const char *slot, int t, int q) const
@@ -137,14 +145,14 @@ struct Side {
                 return *reinterpret_cast<const u32x4 *>(slot + base[q] + t * 16 * PITCH);
             } else if constexpr (E == 2) {
                 typedef __attribute__((address_space(3))) s16x4 place;
-                const uint32_t p = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)slot + base[t];
+                const uint32_t p = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)slot + (base[0] ^ t * 32u);
                 const s16x4 low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((place *)(p + q * 32 * PITCH)), high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((place *)(p + (q * 32 + 4) * PITCH));
                 struct Two { s16x4 a, b; } both = {low, high};
                 return __builtin_bit_cast(u32x4, both);
             } else {
                 u32x4 r;
 #pragma unroll
-                for (int s = 0; s < 4; ++s) r[s] = *reinterpret_cast<const uint32_t *>(slot + base[t] + (q * 16 + s) * PITCH);
+                for (int s = 0; s < 4; ++s) r[s] = *reinterpret_cast<const uint32_t *>(slot + (base[0] ^ t * 64u) + (q * 16 + s) * PITCH);
                 return r;
             }
         }
@@ -217,15 +225,19 @@ struct Loop {
         if (steps && !(a[0].whole(steps - 1u) && b.whole(steps - 1u))) whole = steps - 1u;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");      // what an earlier call has in LDS is read
         if (!steps) return;
-        Asked last;
-        if (whole < steps && whole < RING) ask(whole, last);
+        const auto settle = [&](uint32_t step) {
+            char *to = stage + step % RING * STAGE;
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h) a[h].settle(step, to + h * SideA::BYTES);
+            b.settle(step, to + B0);
+        };
         const auto bring_all = [&](uint32_t step) {
 #pragma unroll
             for (int h = 0; h < PARTS; ++h) a[h].bring(step, lds0 + step % RING * STAGE + h * SideA::BYTES);
             b.bring(step, lds0 + step % RING * STAGE + B0);
         };
         for (uint32_t s = 0; s < RING && s < whole; ++s) bring_all(s);
-        if (whole < steps && whole < RING) put(stage + whole % RING * STAGE, last);
+        if (whole < steps && whole < RING) settle(whole);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
         u32x4 x[2][RT], y[CT];
 #pragma unroll
@@ -241,10 +253,7 @@ struct Loop {
                 if constexpr (STREAM) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(ASKS * (RING - 2)) : "memory");
                 else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
                 if constexpr (!STREAM) {
-                    if (whole < steps && step + RING == whole) {
-                        ask(whole, last);
-                        put(stage + step % RING * STAGE, last);
-                    }
+                    if (whole < steps && step + RING == whole) settle(whole);
                     if (step + RING < whole) bring_all(step + RING);
                 }
             }

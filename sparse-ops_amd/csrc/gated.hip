@@ -1,6 +1,7 @@
 // The gated feed-forward block: both projections, the activation and the product, and their gradients.
 #include "dense.h"
 #include "gate.h"
+#include "lane_moves.h"
 
 namespace {
 
@@ -37,7 +38,7 @@ __device__ __forceinline__ void finish(const Forward<T> &f, uint64_t row, uint64
     }
     if (f.G) so_group_store(f.G + row * f.ldg + col, left, g);
     if (f.U) so_group_store(f.U + row * f.ldg + col, left, u);
-    so_gate::apply<V>(f.act, g, u);
+    so_gate::apply<T, V>(f.act, g, u);
     so_group_store(f.H + row * f.ldh + col, left, g);
 }
 
@@ -57,17 +58,137 @@ void gated_kernel(Forward<T> f, Grid grid)
     loop.template out<2>(stage, [&](int i, uint32_t r, uint32_t c, float (&v)[2][so_elements<T>::V]) { finish(f, row0 + i * 16 + r, j0 + c, v[0], v[1]); });
 }
 
+// One column: a wave takes R rows of both projections, 64 lanes a group of 16 bytes each, and holds a panel of kPanel groups a lane of X in registers for them.
+constexpr int kPanel = 8;
+template <class T, int R>
+__global__ __launch_bounds__(kThreads)
+void gated_token_kernel(Forward<T> f)
+{
+    constexpr int V = so_elements<T>::V;
+    typedef typename so_elements<T>::plain group;
+    const uint32_t lane = threadIdx.x % 64u, groups = f.n / V, rest = f.n % V;
+    const uint64_t row0 = ((uint64_t)blockIdx.x * (kThreads / 64) + threadIdx.x / 64u) * R;
+    if (row0 >= f.m) return;
+    const T *wg[R], *wu[R];
+    float g[R], u[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const uint64_t row = min(row0 + r, (uint64_t)f.m - 1u);          // not there: the last one again, not stored
+        wg[r] = f.Wg + row * f.ldw;
+        wu[r] = f.Wu + row * f.ldw;
+        g[r] = u[r] = 0.0f;
+    }
+    const auto panel = [&](uint32_t q0, auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        group x[kPanel];
+        uint32_t at[kPanel];
+#pragma unroll
+        for (int c = 0; c < kPanel; ++c) {
+            const uint32_t q = q0 + c * 64u + lane;
+            at[c] = (WHOLE ? q : min(q, groups - 1u)) * V;               // not there: the last one again, as zeros
+            if (f.ldx == 1) x[c] = *reinterpret_cast<const typename so_elements<T>::vec *>(f.X + at[c]);
+            else
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[c][e] = f.X[(size_t)(at[c] + e) * f.ldx];
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            group a[kPanel], b[kPanel];
+#pragma unroll
+            for (int c = 0; c < kPanel; ++c) {
+                a[c] = *reinterpret_cast<const typename so_elements<T>::vec *>(wg[r] + at[c]);
+                b[c] = *reinterpret_cast<const typename so_elements<T>::vec *>(wu[r] + at[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < kPanel; ++c) {
+                float p = 0.0f, q = 0.0f;
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    p = fmaf((float)a[c][e], (float)x[c][e], p);
+                    q = fmaf((float)b[c][e], (float)x[c][e], q);
+                }
+                const bool there = WHOLE || q0 + c * 64u + lane < groups;
+                g[r] += there ? p : 0.0f;
+                u[r] += there ? q : 0.0f;
+            }
+        }
+    };
+    uint32_t q0 = 0;
+    for (; q0 + 64u * kPanel <= groups; q0 += 64u * kPanel) panel(q0, std::true_type());
+    if (q0 < groups) panel(q0, std::false_type());
+    if (lane < rest) {
+        const size_t k = (size_t)groups * V + lane;
+        const float x = (float)f.X[k * f.ldx];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            g[r] = fmaf((float)wg[r][k], x, g[r]);
+            u[r] = fmaf((float)wu[r][k], x, u[r]);
+        }
+    }
+    float mine[1] = {}, other[1] = {};                                   // of row row0 + lane
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float p = so_lanes::reduce<64>(g[r], so_lanes::Sum()), q = so_lanes::reduce<64>(u[r], so_lanes::Sum());
+        if (lane == r) mine[0] = p, other[0] = q;
+    }
+    const uint64_t row = row0 + lane;
+    if (lane >= R || row >= f.m) return;
+    if (f.G0) mine[0] += (float)f.G0[row * f.ld0];
+    if (f.U0) other[0] += (float)f.U0[row * f.ld0];
+    if (f.G) f.G[row * f.ldg] = (T)mine[0];
+    if (f.U) f.U[row * f.ldg] = (T)other[0];
+    so_gate::apply<T, 1>(f.act, mine, other);
+    f.H[row * f.ldh] = (T)mine[0];
+}
+
+// The gradients of the two sums, to either or both of two places (the caller's and the products').  A thread takes a group of 16 bytes of a row; groups of whole rows follow one another.  It reads what it
+// needs before it writes, so that the caller's may be the inputs.  Bound by memory.
+template <class T> struct Place {
+    T *g, *u;
+    size_t ld;
+};
+template <class T> struct Slopes {
+    const T *G, *U, *dH;
+    size_t ldg, ldh;
+    uint32_t m, B, groups;           // groups of a row
+    int act;
+    Place<T> to[2];
+};
 template <class T>
 __global__ __launch_bounds__(kThreads)
-void gated_slopes_kernel(uint32_t m, uint32_t B, int act, const T *G, const T *U, size_t ldg, const T *dH, size_t ldh, T *dG, T *dU, size_t ldd)
+void gated_slopes_kernel(Slopes<T> s)
 {
-    const uint64_t at = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (at >= (uint64_t)m * B) return;
-    const uint64_t row = at / B, col = at % B;
-    const auto s = so_gate::value_and_slope(act, (float)G[row * ldg + col]);
-    const float u = (float)U[row * ldg + col], h = (float)dH[row * ldh + col];
-    if (dG) dG[row * ldd + col] = (T)(h * u * s.slope);
-    if (dU) dU[row * ldd + col] = (T)(h * s.value);
+    constexpr int V = so_elements<T>::V;
+    const uint64_t at = (uint64_t)blockIdx.x * kThreads + threadIdx.x, row = at / s.groups, col = at % s.groups * V;
+    if (row >= s.m) return;
+    const uint32_t left = (uint32_t)min((uint64_t)V, s.B - col);
+    const auto gv = so_group_load(s.G + row * s.ldg + col, left), uv = so_group_load(s.U + row * s.ldg + col, left), hv = so_group_load(s.dH + row * s.ldh + col, left);
+    float g[V], u[V];
+    so_gate::with_slope<sizeof(T) == 2>(s.act, [&](auto both) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const so_gate::Both b = both((float)gv[e]);
+            g[e] = (float)hv[e] * (float)uv[e] * b.slope;
+            u[e] = (float)hv[e] * b.value;
+        }
+    });
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (s.to[i].g) so_group_store(s.to[i].g + row * s.to[i].ld + col, left, g);
+        if (s.to[i].u) so_group_store(s.to[i].u + row * s.to[i].ld + col, left, u);
+    }
+}
+
+// A matrix with its rows at multiples of 16 bytes.
+template <class T>
+__global__ __launch_bounds__(kThreads)
+void align_rows_kernel(const T *X, size_t ldx, uint32_t rows, uint32_t cols, uint32_t groups, T *Y, size_t ldy)
+{
+    constexpr int V = so_elements<T>::V;
+    const uint64_t at = (uint64_t)blockIdx.x * kThreads + threadIdx.x, row = at / groups, col = at % groups * V;
+    if (row >= rows) return;
+    const auto v = so_group_load(X + row * ldx + col, (uint32_t)min((uint64_t)V, cols - col));
+    *reinterpret_cast<typename so_elements<T>::vec *>(Y + row * ldy + col) = v;      // zeros behind the row's end
 }
 
 // Y = A[0] B[0] + A[1] B[1], or either's rows one after the other where the result has two parts (Y2 is not null).
@@ -130,16 +251,6 @@ so_status launch_tiles(so_ctx *ctx, const char *who, Kernel kernel, const Arg &a
     return SO_OK;
 }
 
-template <class T>
-so_status forward(so_ctx *ctx, const Forward<T> &f)
-{
-    const Operand<T> g = {f.Wg, f.ldw, f.m, f.n}, u = {f.Wu, f.ldw, f.m, f.n}, x = {f.X, f.ldx, f.B, f.n};
-    return for_tile<T>(ctx, 2 * (uint64_t)f.m, f.B, g.direct() && u.direct() && x.direct(), [&](auto t, auto direct) {
-        typedef decltype(t) TILE;
-        return launch_tiles<TILE>(ctx, "so_gated", gated_kernel<T, TILE, decltype(direct)::value>, f, so_ceil_div(f.m, TILE::ROWS / 2), so_ceil_div(f.B, TILE::COLS));
-    });
-}
-
 template <class T, bool AX, bool BX>
 so_status product(so_ctx *ctx, const Product<T> &p)
 {
@@ -152,13 +263,101 @@ so_status product(so_ctx *ctx, const Product<T> &p)
     });
 }
 
-size_t grad_bytes(int type, uint32_t m, uint32_t B) { return 2 * (size_t)m * B * so_type_bytes(type); }
-
 so_status workspace(so_ctx *ctx, const char *who, size_t bytes)
 {
     SO_REQUIRE(!ctx->capturing || (ctx->mm_part && ctx->mm_part->bytes >= bytes),
                "%s: the context's workspace must grow, which cannot be done while a graph is being recorded (call so_gated_reserve, or launch this shape once, before recording)", who);
     return so_matmul_workspace(ctx, bytes, 4);
+}
+
+// Bytes of a matrix in the workspace, its rows at multiples of 16 bytes.
+size_t stride_of(uint32_t cols) { return (cols + 7u) / 8u * (size_t)8; }
+size_t bytes_of(int type, uint32_t rows, uint32_t cols) { return rows * stride_of(cols) * so_type_bytes(type); }
+
+template <class T> uint64_t blocks_of(uint32_t rows, uint32_t groups) { return ((uint64_t)rows * groups + kThreads - 1) / kThreads; }
+
+// m in the workspace at `to`, aligned.
+template <class T>
+so_status align_rows(so_ctx *ctx, const char *who, Operand<T> *m, uint32_t rows, uint32_t cols, void *to)
+{
+    const uint32_t groups = so_ceil_div(cols, so_elements<T>::V);
+    const uint64_t blocks = blocks_of<T>(rows, groups);
+    SO_REQUIRE(so_grid_fits(blocks, kThreads), "%s: %u x %u is too large for one launch", who, rows, cols);
+    align_rows_kernel<T><<<(uint32_t)blocks, kThreads, 0, ctx->stream>>>(m->p, m->ld, rows, cols, groups, (T *)to, stride_of(cols));
+    SO_LAUNCH_CHECK();
+    m->p = (const T *)to;
+    m->ld = stride_of(cols);
+    return SO_OK;
+}
+
+template <class T>
+so_status slopes(so_ctx *ctx, Slopes<T> s)
+{
+    s.groups = so_ceil_div(s.B, so_elements<T>::V);
+    const uint64_t blocks = blocks_of<T>(s.m, s.groups);
+    SO_REQUIRE(so_grid_fits(blocks, kThreads), "so_gated_grad: %u x %u is too large for one launch", s.m, s.B);
+    gated_slopes_kernel<T><<<(uint32_t)blocks, kThreads, 0, ctx->stream>>>(s);
+    SO_LAUNCH_CHECK();
+    return SO_OK;
+}
+
+template <class T>
+so_status forward(so_ctx *ctx, int type, Forward<T> f)
+{
+    if (f.B == 1) {
+        // four rows a wave where that leaves every compute unit eight waves: X is read once for them
+        const uint32_t waves = 8u * (uint32_t)ctx->compute_units, rows = f.m / 4u >= waves ? 4u : f.m / 2u >= waves ? 2u : 1u, blocks = so_ceil_div(f.m, rows * (kThreads / 64));
+        SO_REQUIRE(so_grid_fits(blocks, kThreads), "so_gated: %u rows are too many for one launch", f.m);
+        const auto kernel = rows == 4 ? gated_token_kernel<T, 4> : rows == 2 ? gated_token_kernel<T, 2> : gated_token_kernel<T, 1>;
+        kernel<<<blocks, kThreads, 0, ctx->stream>>>(f);
+        SO_LAUNCH_CHECK();
+        return SO_OK;
+    }
+    const Operand<T> g = {f.Wg, f.ldw, f.m, f.n}, u = {f.Wu, f.ldw, f.m, f.n};
+    Operand<T> x = {f.X, f.ldx, f.B, f.n};
+    if (g.direct() && u.direct() && !x.direct()) {
+        if (const so_status s = workspace(ctx, "so_gated", bytes_of(type, f.n, f.B)); s != SO_OK) return s;
+        if (const so_status s = align_rows(ctx, "so_gated", &x, f.n, f.B, ctx->mm_part->p); s != SO_OK) return s;
+        f.X = x.p;
+        f.ldx = x.ld;
+    }
+    return for_tile<T>(ctx, 2 * (uint64_t)f.m, f.B, g.direct() && u.direct() && x.direct(), [&](auto t, auto direct) {
+        typedef decltype(t) TILE;
+        return launch_tiles<TILE>(ctx, "so_gated", gated_kernel<T, TILE, decltype(direct)::value>, f, so_ceil_div(f.m, TILE::ROWS / 2), so_ceil_div(f.B, TILE::COLS));
+    });
+}
+
+// The three gradients from dG and dU, either of which may have to go to the caller too.
+struct Gradients {
+    void *dX, *dWg, *dWu;
+    size_t ldx, ldw;
+};
+template <class T>
+so_status backward(so_ctx *ctx, int type, Slopes<T> s, uint32_t n, const Operand<T> (&W)[2], Operand<T> x, const Gradients &r)
+{
+    const uint32_t m = s.m, B = s.B;
+    const bool weights = r.dWg || r.dWu, products = r.dX || weights;
+    so_status status = SO_OK;
+    Operand<T> d[2] = {{s.to[0].g, s.to[0].ld, B, m}, {s.to[0].u, s.to[0].ld, B, m}};
+    if (m && B) {
+        const bool to_workspace = products && !(s.to[0].g && s.to[0].u && d[0].direct() && d[1].direct()), align = weights && !x.direct();
+        if (to_workspace || align) {
+            const size_t each = bytes_of(type, m, B);
+            if ((status = workspace(ctx, "so_gated_grad", 2 * each + bytes_of(type, n, B))) != SO_OK) return status;
+            char *at = (char *)ctx->mm_part->p;
+            if (to_workspace) {
+                s.to[1] = {(T *)at, (T *)(at + each), stride_of(B)};
+                for (int i = 0; i < 2; ++i) d[i] = {(const T *)(at + i * each), stride_of(B), B, m};
+            }
+            if (align && (status = align_rows(ctx, "so_gated_grad", &x, n, B, at + 2 * each)) != SO_OK) return status;
+        }
+        if ((status = slopes(ctx, s)) != SO_OK) return status;
+    }
+    if (r.dX && B) status = product<T, true, true>(ctx, {{W[0], W[1]}, {d[0], d[1]}, (T *)r.dX, nullptr, r.ldx, n, B, 2});
+    if (status != SO_OK || !weights || !m) return status;
+    const Operand<T> along = {x.p, x.ld, n, B}, g = {d[0].p, d[0].ld, m, B}, u = {d[1].p, d[1].ld, m, B};
+    if (r.dWg && r.dWu) return product<T, false, false>(ctx, {{g, u}, {along, along}, (T *)r.dWg, (T *)r.dWu, r.ldw, m, n, 1});
+    return product<T, false, false>(ctx, {{r.dWg ? g : u, u}, {along, along}, (T *)(r.dWg ? r.dWg : r.dWu), nullptr, r.ldw, m, n, 1});
 }
 
 } // namespace
@@ -171,7 +370,7 @@ extern "C" so_status so_gated_reserve(so_ctx *ctx, int type, uint32_t m, uint32_
     if (m == 0 || B == 0) return SO_OK;
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
-    return workspace(ctx, "so_gated_reserve", grad_bytes(type, m, B));
+    return workspace(ctx, "so_gated_reserve", 2 * bytes_of(type, m, B) + bytes_of(type, n, B));
 }
 
 extern "C" so_status so_gated(so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t B, const void *dWg, const void *dWu, size_t w_stride, const void *dX, size_t x_stride, int act,
@@ -196,7 +395,7 @@ extern "C" so_status so_gated(so_ctx *ctx, int type, uint32_t m, uint32_t n, uin
     so_status status = SO_OK;
     so_for_type(type, [&](auto t) {
         using T = decltype(t);
-        status = forward<T>(ctx, {(const T *)dWg, (const T *)dWu, (const T *)dX, (const T *)dG0, (const T *)dU0, (T *)dH, (T *)dG, (T *)dU, w_stride, x_stride, g0_stride, h_stride, g_stride,
+        status = forward<T>(ctx, type, {(const T *)dWg, (const T *)dWu, (const T *)dX, (const T *)dG0, (const T *)dU0, (T *)dH, (T *)dG, (T *)dU, w_stride, x_stride, g0_stride, h_stride, g_stride,
                                   m, n, B, act});
     });
     return status;
@@ -214,11 +413,8 @@ extern "C" so_status so_gated_grad(so_ctx *ctx, int type, uint32_t m, uint32_t n
     SO_REQUIRE(n > 0, "so_gated_grad: no input features");
     SO_REQUIRE(!weights || dw_stride >= n, "so_gated_grad: a stride is shorter than a row");
     SO_REQUIRE(!dDx || dx_stride >= B, "so_gated_grad: a stride is shorter than a row");
-    const size_t e = so_type_bytes(type);
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
-    const uint64_t slopes = so_ceil_div((uint64_t)m * B, kThreads);
-    SO_REQUIRE((uint64_t)m * B < (1ull << 32) - kThreads, "so_gated_grad: %u x %u is too large for one launch", m, B);
     if (m > 0 && B > 0) {
         SO_REQUIRE(dG && dU && dDh, "so_gated_grad: null tensor");
         SO_REQUIRE(!dDx || (dWg && dWu), "so_gated_grad: null weights");
@@ -237,27 +433,8 @@ extern "C" so_status so_gated_grad(so_ctx *ctx, int type, uint32_t m, uint32_t n
     so_status status = SO_OK;
     so_for_type(type, [&](auto t) {
         using T = decltype(t);
-        T *g = (T *)dDg, *u = (T *)dDu;
-        size_t ldg = dg_stride, ldu = dg_stride;
-        if ((!g || !u) && (dDx || weights) && m && B) {
-            status = workspace(ctx, "so_gated_grad", grad_bytes(type, m, B));
-            if (status != SO_OK) return;
-            T *w = (T *)ctx->mm_part->p;
-            if (!g || !u) g = w, u = w + (size_t)m * B, ldg = ldu = B;
-        }
-        if (m && B) gated_slopes_kernel<T><<<(uint32_t)slopes, kThreads, 0, ctx->stream>>>(m, B, act, (const T *)dG, (const T *)dU, g_stride, (const T *)dDh, dh_stride, g, u, ldg);
-        if (dDx && B)
-            status = product<T, true, true>(ctx, {{{(const T *)dWg, w_stride, n, m}, {(const T *)dWu, w_stride, n, m}}, {{g, ldg, B, m}, {u, ldu, B, m}}, (T *)dDx, nullptr, dx_stride, n, B, 2});
-        const Operand<T> x = {(const T *)dX, x_stride, n, B}, dg = {g, ldg, m, B}, du = {u, ldu, m, B};
-        if (status == SO_OK && m && dDwg && dDwu) status = product<T, false, false>(ctx, {{dg, du}, {x, x}, (T *)dDwg, (T *)dDwu, dw_stride, m, n, 1});
-        else if (status == SO_OK && m && weights) status = product<T, false, false>(ctx, {{dDwg ? dg : du, du}, {x, x}, (T *)(dDwg ? dDwg : dDwu), nullptr, dw_stride, m, n, 1});
-        if (status != SO_OK) return;
-        if ((dDg && g != (T *)dDg) || (dDu && u != (T *)dDu)) {      // one of the two asked for
-            gated_slopes_kernel<T><<<(uint32_t)slopes, kThreads, 0, ctx->stream>>>(m, B, act, (const T *)dG, (const T *)dU, g_stride, (const T *)dDh, dh_stride, (T *)dDg, (T *)dDu, dg_stride);
-        }
+        status = backward<T>(ctx, type, {(const T *)dG, (const T *)dU, (const T *)dDh, g_stride, dh_stride, m, B, 0, act, {{(T *)dDg, (T *)dDu, dg_stride}, {nullptr, nullptr, 0}}}, n,
+                             {{(const T *)dWg, w_stride, n, m}, {(const T *)dWu, w_stride, n, m}}, {(const T *)dX, x_stride, n, B}, {dDx, dDwg, dDwu, dx_stride, dw_stride});
     });
-    (void)e;
-    if (status != SO_OK) return status;
-    SO_LAUNCH_CHECK();
-    return SO_OK;
+    return status;
 }
