@@ -106,10 +106,16 @@ struct Side {
         return __builtin_bit_cast(u32x4, so_group_load(at + (ACROSS ? (size_t)k * ld + i : (size_t)i * ld + k), (uint32_t)min(end - along, (uint64_t)V)));
     }
     static __device__ __forceinline__ uint32_t group_of(uint32_t a) { return (a * WAVES + threadIdx.x / 64u) * 64u + threadIdx.x % 64u; }
-    __device__ __forceinline__ void ask(uint32_t step, u32x4 (&r)[ASKS]) const
+    // The groups of a step that is whole, at any address.  Rows, or groups of a row, that do not exist are replaced by others that do, for nothing.
+    __device__ __forceinline__ void take(uint32_t step, u32x4 (&r)[ASKS]) const
     {
 #pragma unroll
-        for (int a = 0; a < ASKS; ++a) r[a] = group(step, group_of(a));
+        for (int a = 0; a < ASKS; ++a) {
+            const uint32_t q = group_of(a), row = q / PER, group = q % PER ^ swap(row);
+            const uint32_t i = ACROSS ? (group * V < own ? group * V : 0u) : min(row, own - 1u), k = ACROSS ? row : group * V;
+            const T *p = at + (ACROSS ? (size_t)step * BK * ld : (size_t)step * BK) + (ACROSS ? (size_t)k * ld + i : (size_t)i * ld + k);
+            r[a] = __builtin_bit_cast(u32x4, *reinterpret_cast<const typename so_elements<T>::vec *>(p));
+        }
     }
     static __device__ __forceinline__ void put(char *to, const u32x4 (&r)[ASKS])
     {
@@ -199,19 +205,27 @@ struct Loop {
         rb.start(wave % WC * CT);
     }
     __device__ __forceinline__ u32x4 row_tile(const char *slot, int i, int q) const { return ra.get(slot + (HALVES && i >= RT / 2 ? SideA::BYTES : 0), HALVES ? i % (RT / 2) : i, q); }
-    struct Asked { u32x4 a[PARTS][SideA::ASKS], b[SideB::ASKS]; };
-    __device__ __forceinline__ void ask(uint32_t step, Asked &w) const
+    struct Taken { u32x4 a[PARTS][SideA::ASKS], b[SideB::ASKS]; };
+    __device__ __forceinline__ void take(uint32_t step, Taken &w) const
     {
 #pragma unroll
-        for (int h = 0; h < PARTS; ++h) a[h].ask(step, w.a[h]);
-        b.ask(step, w.b);
+        for (int h = 0; h < PARTS; ++h) a[h].take(step, w.a[h]);
+        b.take(step, w.b);
     }
-    static __device__ __forceinline__ void put(char *slot, const Asked &w)
+    static __device__ __forceinline__ void put(char *slot, const Taken &w)
     {
 #pragma unroll
         for (int h = 0; h < PARTS; ++h) SideA::put(slot + h * SideA::BYTES, w.a[h]);
         SideB::put(slot + B0, w.b);
     }
+    __device__ __forceinline__ void settle(uint32_t step, char *slot) const
+    {
+#pragma unroll
+        for (int h = 0; h < PARTS; ++h) a[h].settle(step, slot + h * SideA::BYTES);
+        b.settle(step, slot + B0);
+    }
+    // Steps, and how many of them are whole: all, or all but the last.
+    __device__ __forceinline__ uint32_t whole_of(uint32_t steps) const { return steps && !(a[0].whole(steps - 1u) && b.whole(steps - 1u)) ? steps - 1u : steps; }
 
     // acc += the product of rows from i0 on (of both operands, with HALVES) and columns from j0 on, both operands aligned.  All steps go straight to LDS, but for a last one that is not whole.
     // A run (64 bytes of k) is multiplied from registers while the next one's operands are read: those of the rows into a second set, those of the columns into the places that have been multiplied
@@ -221,23 +235,16 @@ struct Loop {
         constexpr int Q = KB / 64;
         static_assert(Q == 1 || Q == 2, "runs of a step");
         const uint32_t steps = b.steps(), lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)stage;
-        uint32_t whole = steps;
-        if (steps && !(a[0].whole(steps - 1u) && b.whole(steps - 1u))) whole = steps - 1u;
+        const uint32_t whole = whole_of(steps);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");      // what an earlier call has in LDS is read
         if (!steps) return;
-        const auto settle = [&](uint32_t step) {
-            char *to = stage + step % RING * STAGE;
-#pragma unroll
-            for (int h = 0; h < PARTS; ++h) a[h].settle(step, to + h * SideA::BYTES);
-            b.settle(step, to + B0);
-        };
         const auto bring_all = [&](uint32_t step) {
 #pragma unroll
             for (int h = 0; h < PARTS; ++h) a[h].bring(step, lds0 + step % RING * STAGE + h * SideA::BYTES);
             b.bring(step, lds0 + step % RING * STAGE + B0);
         };
         for (uint32_t s = 0; s < RING && s < whole; ++s) bring_all(s);
-        if (whole < steps && whole < RING) settle(whole);
+        if (whole < steps && whole < RING) settle(whole, stage + whole % RING * STAGE);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
         u32x4 x[2][RT], y[CT];
 #pragma unroll
@@ -253,7 +260,7 @@ struct Loop {
                 if constexpr (STREAM) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(ASKS * (RING - 2)) : "memory");
                 else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
                 if constexpr (!STREAM) {
-                    if (whole < steps && step + RING == whole) settle(whole);
+                    if (whole < steps && step + RING == whole) settle(whole, stage + step % RING * STAGE);
                     if (step + RING < whole) bring_all(step + RING);
                 }
             }
@@ -303,19 +310,18 @@ struct Loop {
         }
     }
 
-    // The same for operands at any address: a step is asked for while the one before it is multiplied, and put into LDS behind that.
+    // The same for operands at any address, by way of registers: three steps are on their way there, two in LDS.
     __device__ __forceinline__ void add_any(char *stage)
     {
-        const uint32_t steps = b.steps();
+        const uint32_t steps = b.steps(), whole = whole_of(steps);
         __syncthreads();
         if (!steps) return;
-        Asked w;
-        ask(0, w);
-        put(stage, w);
-        for (uint32_t s = 0; s < steps; ++s) {
-            __syncthreads();
-            if (s + 1u < steps) ask(s + 1u, w);
-            const char *slot = stage + s % 2u * STAGE;
+        Taken w[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if ((uint32_t)i < whole) take(i, w[i]);
+        const auto compute = [&](uint32_t step) {
+            const char *slot = stage + step % 2u * STAGE;
 #pragma unroll
             for (int q = 0; q < KB / 64; ++q) {
                 u32x4 x[RT], y[CT];
@@ -328,7 +334,34 @@ struct Loop {
 #pragma unroll
                     for (int i = 0; i < RT; ++i) acc[i][k] = multiply<T>(x[i], y[k], acc[i][k]);
             }
-            if (s + 1u < steps) put(stage + (s + 1u) % 2u * STAGE, w);
+        };
+        // Step s from its registers to LDS, the one three later to them; the other half of LDS, which the step before it is read from, is free behind the barrier of the next turn.
+        const auto turn = [&](uint32_t s, Taken &own, auto more) {
+            put(stage + s % 2u * STAGE, own);
+            __syncthreads();
+            if constexpr (decltype(more)::value) take(s + 3u, own);
+            compute(s);
+        };
+        uint32_t s = 0;
+        for (; s + 5u < whole; s += 3u) {
+            turn(s, w[0], std::true_type());
+            turn(s + 1u, w[1], std::true_type());
+            turn(s + 2u, w[2], std::true_type());
+        }
+        for (; s < whole; s += 3u) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (s + i < whole) {
+                    put(stage + (s + i) % 2u * STAGE, w[i]);
+                    __syncthreads();
+                    if (s + i + 3u < whole) take(s + i + 3u, w[i]);
+                    compute(s + i);
+                }
+        }
+        if (whole < steps) {
+            settle(whole, stage + whole % 2u * STAGE);
+            __syncthreads();
+            compute(whole);
         }
     }
     template <bool DIRECT>
