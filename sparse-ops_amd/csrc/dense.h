@@ -49,11 +49,11 @@ struct Side {
     static constexpr int BYTES = ROWS * PITCH, ASKS = ROWS * PER / 64 / WAVES;                                   // requests of a wave, 64 groups each
     static_assert(ASKS * 64 * WAVES == ROWS * PER, "every wave brings as many groups as the others");
 
-    // A row's groups are exchanged by an exclusive or, so that lanes that read at the same place of neighbouring rows meet in different banks: along, 8 rows of one group; across, in 16 bits
+    // A row's groups are exchanged by an exclusive or, so that lanes that read at the same place of neighbouring rows meet in different banks: along, 16 rows of one group (8 of rows of 128 bytes, pairs of rows of 64); across, in 16 bits
     // 16 rows (4 neighbours, of 4 eights) of 32 bytes, in 32 bits 4 rows (each fourth) of 64 bytes.
     static __device__ __forceinline__ uint32_t swap(uint32_t row)
     {
-        if constexpr (!ACROSS) return PER == 8 ? row & 7u : row >> 1 & 3u;
+        if constexpr (!ACROSS) return PER == 16 ? row & 15u : PER == 8 ? row & 7u : row >> 1 & 3u;
         else if constexpr (E == 2) return PER >= 16 ? ((row & 3u) | (row >> 1 & 4u)) << 1 : PER == 8 ? ((row >> 1 & 1u) | (row >> 2 & 2u)) << 1 : PER == 4 ? (row >> 3 & 1u) << 1 : 0u;
         else return PER >= 16 ? (row >> 2 & 3u) << 2 : PER == 8 ? (row >> 2 & 1u) << 2 : 0u;
     }
@@ -166,9 +166,10 @@ struct Side {
 };
 
 // A tile of the result: WM x WC waves of RT x CT tiles of 16 x 16 each, KB bytes of the contraction a step, RING steps in LDS.  With HALVES the rows are those of two operands, half of each wave's
-// from either.
-template <int RT_, int CT_, int WM_, int WC_, int KB_, int RING_>
+// from either.  TURNED: workgroups begin at different steps, so that they do not all ask for the same places of their rows (and with them for the same channels of the memory) at the same time.
+template <int RT_, int CT_, int WM_, int WC_, int KB_, int RING_, bool TURNED_ = false>
 struct Tile {
+    static constexpr bool TURNED = TURNED_;
     static constexpr int RT = RT_, CT = CT_, WM = WM_, WC = WC_, KB = KB_, RING = RING_, WAVES = WM * WC, THREADS = WAVES * 64, ROWS = RT * WM * 16, COLS = CT * WC * 16;
     static constexpr int OUT_PITCH = CT * 16 + 4;                    // floats of a row on its way out, in a part of LDS of each wave's own: 32 rows of one result, or 16 of two
     static constexpr uint32_t lds = std::max((ROWS + COLS) * KB * RING, WAVES * 32 * OUT_PITCH * 4);
@@ -233,15 +234,20 @@ struct Loop {
     __device__ __forceinline__ void add_direct(char *stage)
     {
         constexpr int Q = KB / 64;
-        static_assert(Q == 1 || Q == 2, "runs of a step");
+        static_assert(Q == 1 || Q == 2 || Q == 4, "runs of a step");
         const uint32_t steps = b.steps(), lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)stage;
         const uint32_t whole = whole_of(steps);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");      // what an earlier call has in LDS is read
         if (!steps) return;
+        const uint32_t first = TILE::TURNED && whole ? blockIdx.x % whole : 0u;
+        const auto nth = [&](uint32_t step) {                            // of the whole steps
+            if constexpr (!TILE::TURNED) return step;
+            else return step + first >= whole ? step + first - whole : step + first;
+        };
         const auto bring_all = [&](uint32_t step) {
 #pragma unroll
-            for (int h = 0; h < PARTS; ++h) a[h].bring(step, lds0 + step % RING * STAGE + h * SideA::BYTES);
-            b.bring(step, lds0 + step % RING * STAGE + B0);
+            for (int h = 0; h < PARTS; ++h) a[h].bring(nth(step), lds0 + step % RING * STAGE + h * SideA::BYTES);
+            b.bring(nth(step), lds0 + step % RING * STAGE + B0);
         };
         for (uint32_t s = 0; s < RING && s < whole; ++s) bring_all(s);
         if (whole < steps && whole < RING) settle(whole, stage + whole % RING * STAGE);
@@ -277,8 +283,8 @@ struct Loop {
                     const uint32_t to = lds0 + step % RING * STAGE;
 #pragma unroll
                     for (int p = k * ASKS / CT; p < (k + 1) * ASKS / CT; ++p) {
-                        if (p < SideA::ASKS * PARTS) a[p / SideA::ASKS].bring(step + RING, to + p / SideA::ASKS * SideA::BYTES, p % SideA::ASKS);
-                        else b.bring(step + RING, to + B0, p - SideA::ASKS * PARTS);
+                        if (p < SideA::ASKS * PARTS) a[p / SideA::ASKS].bring(nth(step + RING), to + p / SideA::ASKS * SideA::BYTES, p % SideA::ASKS);
+                        else b.bring(nth(step + RING), to + B0, p - SideA::ASKS * PARTS);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -286,18 +292,22 @@ struct Loop {
         };
         const std::integral_constant<int, 0> zero;
         const std::integral_constant<int, 1> one;
+        const std::integral_constant<int, 2> two;
+        const std::integral_constant<int, 3> three;
         const std::true_type yes;
         const std::false_type no;
+        const auto multiply_step = [&](uint32_t step, auto stream) {
+            multiply_run(step, zero, zero, stream);
+            if constexpr (Q >= 2) multiply_run(step, one, one, stream);
+            if constexpr (Q == 4) {
+                multiply_run(step, two, zero, stream);
+                multiply_run(step, three, one, stream);
+            }
+        };
         uint32_t s = 0;
-        if constexpr (Q == 2) {
-            for (; s + RING < whole; ++s) {
-                multiply_run(s, zero, zero, yes);
-                multiply_run(s, one, one, yes);
-            }
-            for (; s < steps; ++s) {
-                multiply_run(s, zero, zero, no);
-                multiply_run(s, one, one, no);
-            }
+        if constexpr (Q > 1) {
+            for (; s + RING < whole; ++s) multiply_step(s, yes);
+            for (; s < steps; ++s) multiply_step(s, no);
         } else {
             for (; s + 1u + RING < whole; s += 2u) {
                 multiply_run(s, zero, zero, yes);

@@ -220,24 +220,49 @@ void product_kernel(Product<T> p, Grid grid)
 }
 
 // Tiles, by rows and columns of the result (of both projections together in the forward pass).
-typedef so_dense::Tile<8, 4, 2, 4, 64, 4> Large;        // 256 x 256
-typedef so_dense::Tile<4, 4, 2, 2, 64, 4> Middle;       // 128 x 128
-typedef so_dense::Tile<2, 2, 2, 2, 128, 4> Small;       // 64 x 64
-typedef so_dense::Tile<2, 1, 2, 2, 128, 5> Narrow;      // 64 x 32
+typedef so_dense::Tile<8, 4, 2, 4, 64, 4> T256x256;
+typedef so_dense::Tile<4, 4, 2, 2, 64, 4> T128x128;
+typedef so_dense::Tile<4, 2, 1, 4, 128, 3> T64x128;
+typedef so_dense::Tile<2, 2, 2, 2, 128, 4> T64x64;
+typedef so_dense::Tile<2, 1, 1, 4, 256, 3, true> T32x64;
+typedef so_dense::Tile<2, 1, 1, 2, 256, 4, true> T32x32;
 
-// f(a tile, whether operands go past the registers): the largest that gives every compute unit a workgroup.  fp32 has no use for the largest: its products take four times as long, and 128 x 128 feeds them.
-template <class T, class F>
-so_status for_tile(const so_ctx *ctx, uint64_t rows, uint64_t cols, bool direct, F &&f)
+struct Form { uint32_t rows, cols; const char *name; };
+constexpr Form kForms[] = {{32, 32, "gated-32x32"}, {32, 64, "gated-32x64"}, {64, 64, "gated-64x64"}, {64, 128, "gated-64x128"}, {128, 128, "gated-128x128"}, {256, 256, "gated-256x256"}};
+constexpr int kFormCount = 6;
+
+// The largest tile that gives every compute unit a workgroup, not half of whose columns would do: a larger one asks the caches for less, a smaller one leaves none idle.  From a sweep (bf16 forward, us, this form /
+// its neighbours): 8192 x 4096 (m x n) at B = 24 32 x 32 27 / 28, 64 64 x 64 32 / 33 and 37, 128 64 x 128 39 / 43 and 53; 4096 x 4096 at 24 32 x 32 15.8 / 19, 64 32 x 64 19.8 / 27 and 24, 256
+// 64 x 128 33 / 36 and 51; 2048 x 2048 at 128 32 x 64 10.5 / 11.4 and 11.5; 2048 x 1024 at 64 32 x 32 6.3 / 6.8.  fp32 has no use for the largest: its products take eight times as long.
+int choose_form(const so_ctx *ctx, int most, uint64_t rows, uint64_t cols)
 {
-    const uint64_t cus = (uint64_t)ctx->compute_units;
-    const auto tiles = [&](uint32_t r, uint32_t c) { return (uint64_t)so_ceil_div(rows, r) * so_ceil_div(cols, c); };
-    const bool middle = cols > 64 && tiles(128, 128) >= cus;
-    if (!direct) return middle ? f(Middle(), std::false_type()) : f(Small(), std::false_type());
-    if constexpr (sizeof(T) == 2)
-        if (cols > 128 && tiles(256, 256) >= cus) return f(Large(), std::true_type());
-    if (middle) return f(Middle(), std::true_type());
-    if (cols > 32) return f(Small(), std::true_type());
-    return f(Narrow(), std::true_type());
+    if (ctx->tune.gated_form >= 1 && ctx->tune.gated_form <= kFormCount) return std::min(ctx->tune.gated_form - 1, most);
+    const auto tiles = [&](int f) { return (uint64_t)so_ceil_div(rows, kForms[f].rows) * so_ceil_div(cols, kForms[f].cols); };
+    for (int f = most; f > 0; --f)
+        if (tiles(f) >= (uint64_t)ctx->compute_units && cols > kForms[f].cols / 2) return f;
+    return 0;
+}
+
+// f(a tile, whether operands go past the registers).  By way of them only two sizes, as large as they go.
+template <class T, class F>
+so_status for_tile(so_ctx *ctx, uint64_t rows, uint64_t cols, bool direct, F &&f)
+{
+    const int form = choose_form(ctx, direct ? (sizeof(T) == 2 ? 5 : 4) : 4, rows, cols);
+    ctx->last_kernel = kForms[form].name;
+    if (!direct) {
+        ctx->last_kernel = form == 4 ? "gated-128x128-any" : "gated-64x64-any";
+        return form == 4 ? f(T128x128(), std::false_type()) : f(T64x64(), std::false_type());
+    }
+    switch (form) {
+    case 0: return f(T32x32(), std::true_type());
+    case 1: return f(T32x64(), std::true_type());
+    case 2: return f(T64x64(), std::true_type());
+    case 3: return f(T64x128(), std::true_type());
+    case 4: return f(T128x128(), std::true_type());
+    default:
+        if constexpr (sizeof(T) == 2) return f(T256x256(), std::true_type());
+        return SO_ERR_INVALID;
+    }
 }
 
 template <class TILE, class Kernel, class Arg>
@@ -309,6 +334,7 @@ so_status forward(so_ctx *ctx, int type, Forward<T> f)
         const uint32_t waves = 8u * (uint32_t)ctx->compute_units, rows = f.m / 4u >= waves ? 4u : f.m / 2u >= waves ? 2u : 1u, blocks = so_ceil_div(f.m, rows * (kThreads / 64));
         SO_REQUIRE(so_grid_fits(blocks, kThreads), "so_gated: %u rows are too many for one launch", f.m);
         const auto kernel = rows == 4 ? gated_token_kernel<T, 4> : rows == 2 ? gated_token_kernel<T, 2> : gated_token_kernel<T, 1>;
+        ctx->last_kernel = "gated-token";
         kernel<<<blocks, kThreads, 0, ctx->stream>>>(f);
         SO_LAUNCH_CHECK();
         return SO_OK;

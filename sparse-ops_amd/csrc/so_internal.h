@@ -38,6 +38,7 @@ struct so_tuning {
     int wait_spins = -1;     // SPARSEOPS_WAIT_SPINS: most polls of a bounded wait on LDS progress counters (0: every wait gives up at once; tests)
     int norm_lanes = -1;     // SPARSEOPS_NORM_LANES: lanes of a row (1, 2, 4, 8) of the layer norm that holds all features, 0 forbids it and the gradient in one workgroup; more than whole_of has a kernel for: in parts
     int mxfp4_form = 0;      // SPARSEOPS_MXFP4_MATMUL: the tile of so_mxfp4_matmul, by its number in csrc/mxfp4_matmul.hip
+    int gated_form = 0;      // SPARSEOPS_GATED_TILE: the tile of so_gated and its gradient, by its number in csrc/gated.hip
     int conv_rbm = -1;       // SPARSEOPS_CONV_RBM: 0 forbids the row-block-merged kernel on plans that carry its streams, 1 asks for it against any other override
 };
 

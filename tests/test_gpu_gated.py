@@ -80,6 +80,23 @@ def test_rows_that_are_aligned_and_end_inside_a_group(ctx, m, n, B, type_):
         make(0, up(n))
 
 
+FORMS = ["gated-32x32", "gated-32x64", "gated-64x64", "gated-64x128", "gated-128x128", "gated-256x256"]
+
+
+@pytest.mark.parametrize("form", range(1, 7))
+@pytest.mark.parametrize("m,n,B", [(40, 24, 16), (70, 72, 40), (150, 264, 72), (300, 520, 264), (280, 1032, 328), (96, 4096, 48), (520, 2056, 40)])
+def test_every_tile(ctx, m, n, B, form):
+    """Each tile of the result on contractions of less than one step of its ring, a few, and many, with and without a last one that is not whole; both ways that operands go to LDS."""
+    rng = np.random.default_rng(form + m + n + B)
+    for type_ in TYPES:
+        with ctx.tuning(SPARSEOPS_GATED_TILE=form):
+            run_forward(ctx, rng, m, n, B, type_, "silu", pad=8, wpad=0)
+            assert ctx.last_kernel() == FORMS[min(form, 6 if type_ != "f32" else 5) - 1]
+            run_backward(ctx, rng, m, n, B, type_, "silu", pad=8, wpad=8)
+            run_forward(ctx, rng, m, n, B, type_, "gelu", pad=3, wpad=5)
+            run_backward(ctx, rng, m, n, B, type_, "gelu", pad=3, wpad=5)
+
+
 @pytest.mark.parametrize("act", ACTS)
 def test_forward_of_every_activation(ctx, act):
     rng = np.random.default_rng(5)
