@@ -20,17 +20,34 @@ __device__ __forceinline__ uint2 rows_of(const Shape &s, uint32_t p)
 }
 
 // cos and sin of pos * freq, times the amplitude.  The product is exact in fp64; of it the whole turns are taken off there, so that a position of 2^31 costs 2^-22 of a turn and one of 2^20 less
-// than fp32 can tell.
+// than fp32 can tell.  For results of 16 bits the vector unit's sine and cosine of what is left, which are off by some 2^-20 of 1, do.
+template <bool HALF>
 __device__ __forceinline__ float2 turn_of(int32_t pos, double turns, float amplitude)
 {
     const double t = (double)pos * turns;
+    const float left = (float)(t - rint(t));
     float c, s;
-    sincospif(2.0f * (float)(t - rint(t)), &s, &c);
+    if constexpr (HALF) {
+        c = __builtin_amdgcn_cosf(left);
+        s = __builtin_amdgcn_sinf(left);
+    } else {
+        sincospif(2.0f * left, &s, &c);
+    }
     return make_float2(amplitude * c, amplitude * s);
+}
+
+// 1 / sqrt(v), also where v is below the least normal number, which the vector unit takes for 0
+__device__ __forceinline__ float inverse_root(float v)
+{
+    const bool small = v < 0x1p-100f;
+    return __builtin_amdgcn_rsqf(small ? v * 0x1p100f : v) * (small ? 0x1p50f : 1.0f);
 }
 
 constexpr double kTurnsPerRadian = 0.15915494309189533577;
 
+// y = turn(gain * x * rstd), rstd = 1 / sqrt(mean(x^2) + eps) of a head's D features; turn takes (u, v) to (u cos - v sin, v cos + u sin).  One read and one write of every element: memory bounds
+// it.  32 + 8 heads of 128 x 8192 bf16, 168 MB, take 38.6 us or 4.4 TB/s (a layer norm of as many bytes runs at 3.9); one column 4.8 us, a launch.  With fp64 multiples and the library's sine for
+// every type it was 50 us, and with two pairs a thread and 256 threads, of 136 registers, 45.
 // What forward pass and gradient share: a workgroup of NT threads takes LC * V columns of `per` heads, one after the other; a thread PPT pairs of a head's features, for which it keeps the turns of its columns.
 template <class T, int LC, int PPT, int NT>
 struct Seat {
@@ -69,7 +86,7 @@ struct Seat {
             const bool turned = i < s.rot / 2u;
             const double f = turned ? (double)freq[i] * kTurnsPerRadian : 0.0;
 #pragma unroll
-            for (int e = 0; e < V; ++e) t[k][e] = turned ? turn_of(p[e], f, amplitude) : make_float2(1.0f, 0.0f);
+            for (int e = 0; e < V; ++e) t[k][e] = turned ? turn_of<sizeof(T) == 2>(p[e], f, amplitude) : make_float2(1.0f, 0.0f);
         }
     }
     __device__ __forceinline__ void load(const Shape &s, uint32_t head, const T *X, size_t ld, group (&x)[PPT][2]) const
@@ -117,7 +134,7 @@ void rotary_kernel(Shape s, const T *X, size_t ldx, const float *gain_q, const f
                 for (int e = 0; e < V; ++e) r[e] = fmaf((float)x[k][1][e], (float)x[k][1][e], fmaf((float)x[k][0][e], (float)x[k][0][e], r[e]));
             so_norm::sum_tile<NT, LC, V>(r, lds);
 #pragma unroll
-            for (int e = 0; e < V; ++e) r[e] = 1.0f / sqrtf(r[e] / (float)s.D + eps);
+            for (int e = 0; e < V; ++e) r[e] = inverse_root(fmaf(r[e], 1.0f / (float)s.D, eps));
             if (rstd && threadIdx.x < LC)
 #pragma unroll
                 for (int e = 0; e < V; ++e)
@@ -141,13 +158,16 @@ void rotary_kernel(Shape s, const T *X, size_t ldx, const float *gain_q, const f
     }
 }
 
-// With norms: dX, and of every workgroup its share of the gains' gradients, [tiles * groups][D].
+// With norms: h = turn^-1(dY); dX = rstd (gain h - n mean(gain h n)), n = x rstd, and of every workgroup its share of the gains' gradients sum(h n), [tiles * groups][D], which the kernel below adds
+// up in a fixed order.  24 + 8 heads of 96 x 4099 fp16, 75 MB: 30 us and 4.5 for the shares; with the next head in registers ahead, which leaves one workgroup a compute unit, 47, and with h
+// kept instead of turned back again after the sum, 38.
 template <class T, int LC, int PPT, int NT>
-__global__ __launch_bounds__(NT)
+__global__ __launch_bounds__(NT, PPT == 1 ? 4 : 1)
 void rotary_grad_kernel(Shape s, const T *X, size_t ldx, const T *dY, size_t ldd, const float *gain_q, const float *gain_k, const float *rstd, const int32_t *pos, const float *freq, float amplitude,
                         T *dX, size_t ldo, float *shares)
 {
     constexpr int V = so_elements<T>::V;
+    typedef typename so_elements<T>::plain group;
     __shared__ float lds[(NT / 64 + 1) * LC * V];
     const Seat<T, LC, PPT, NT> at(s, ldx);
     const uint32_t wide_d = so_group_wide_rows<T>(at.left, s.heads * s.D, ldd);
@@ -165,24 +185,26 @@ void rotary_grad_kernel(Shape s, const T *X, size_t ldx, const T *dY, size_t ldd
         if (gain && at.two[k]) g[k].y = gain[at.row[k].y];
     }
     for (uint32_t head = at.first; head < at.last; ++head) {
-        typename so_elements<T>::plain x[PPT][2], d[PPT][2];
+        group x[PPT][2], d[PPT][2];
         at.load(s, head, X, ldx, x);
         of_dy.load(s, head, dY, ldd, d);
-        float r[V], dot[V];
+        float r[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            r[e] = (uint32_t)e < at.left ? rstd[(size_t)head * s.B + at.c0 + e] : 0.0f;
-            dot[e] = 0.0f;
-        }
-        float a[PPT][V], b[PPT][V];
+        for (int e = 0; e < V; ++e) r[e] = (uint32_t)e < at.left ? rstd[(size_t)head * s.B + at.c0 + e] : 0.0f;
+        float dot[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) dot[e] = 0.0f;
+        // the gradients of the products, turned back
+        const auto back = [&](int k, int e) {
+            const float u = (float)d[k][0][e], v = (float)d[k][1][e];
+            return make_float2(fmaf(u, turn[k][e].x, v * turn[k][e].y), fmaf(v, turn[k][e].x, -(u * turn[k][e].y)));
+        };
 #pragma unroll
         for (int k = 0; k < PPT; ++k)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float u = (float)d[k][0][e], v = (float)d[k][1][e], c = turn[k][e].x, w = turn[k][e].y;
-                a[k][e] = fmaf(u, c, v * w);
-                b[k][e] = fmaf(v, c, -(u * w));
-                const float p = a[k][e] * ((float)x[k][0][e] * r[e]), q = b[k][e] * ((float)x[k][1][e] * r[e]);
+                const float2 y = back(k, e);
+                const float p = y.x * ((float)x[k][0][e] * r[e]), q = y.y * ((float)x[k][1][e] * r[e]);
                 if ((uint32_t)e < at.left) {
                     sum[k].x += p;
                     sum[k].y += q;
@@ -193,12 +215,14 @@ void rotary_grad_kernel(Shape s, const T *X, size_t ldx, const T *dY, size_t ldd
         so_norm::sum_tile<NT, LC, V>(dot, lds);
 #pragma unroll
         for (int k = 0; k < PPT; ++k) {
+            for (int i = 0; i < 2; ++i) so_group_afresh(x[k][i]), so_group_afresh(d[k][i]);      // converted again: the fp32 values would take 32 registers a pair
             float p[V], q[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float mean = dot[e] / (float)s.D;
-                p[e] = r[e] * fmaf(a[k][e], g[k].x, -(((float)x[k][0][e] * r[e]) * mean));
-                q[e] = r[e] * fmaf(b[k][e], g[k].y, -(((float)x[k][1][e] * r[e]) * mean));
+                const float2 y = back(k, e);
+                const float mean = dot[e] * (1.0f / (float)s.D);
+                p[e] = r[e] * fmaf(y.x, g[k].x, -(((float)x[k][0][e] * r[e]) * mean));
+                q[e] = r[e] * fmaf(y.y, g[k].y, -(((float)x[k][1][e] * r[e]) * mean));
             }
             if (at.has[k]) so_group_store(dX + (size_t)(head * s.D + at.row[k].x) * ldo + at.c0, at.left, p);
             if (at.two[k]) so_group_store(dX + (size_t)(head * s.D + at.row[k].y) * ldo + at.c0, at.left, q);
@@ -215,7 +239,7 @@ void rotary_grad_kernel(Shape s, const T *X, size_t ldx, const T *dY, size_t ldd
     }
 }
 
-// The shares of the queries' workgroups and of the keys' to one gradient each: 16 features a workgroup, 16 runs of shares.
+// The shares of the queries' workgroups and of the keys' to one gradient each: 16 features a workgroup, 16 runs of shares, eight of a run on their way at a time (one at a time: 25 us for 455).
 __global__ __launch_bounds__(256)
 void rotary_gains_kernel(uint32_t D, uint32_t shares_q, uint32_t shares, uint32_t blocks, const float *from, float *gain_q, float *gain_k)
 {
@@ -225,7 +249,13 @@ void rotary_gains_kernel(uint32_t D, uint32_t shares_q, uint32_t shares, uint32_
     const uint32_t d = blockIdx.x % blocks * 16u + threadIdx.x % 16u, run = threadIdx.x / 16u, end = query ? shares_q : shares;
     float s = 0.0f;
     if (d < D)
-        for (uint32_t p = (query ? 0u : shares_q) + run; p < end; p += 16u) s += from[(size_t)p * D + d];
+        for (uint32_t p = (query ? 0u : shares_q) + run; p < end; p += 128u) {
+            float v[8];                                                  // eight on their way at a time
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) v[i] = p + i * 16u < end ? from[(size_t)(p + i * 16u) * D + d] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[i];
+        }
     sums[run][threadIdx.x % 16u] = s;
     __syncthreads();
     if (run || d >= D || !out) return;
@@ -234,14 +264,14 @@ void rotary_gains_kernel(uint32_t D, uint32_t shares_q, uint32_t shares, uint32_
     out[d] = s;
 }
 
-// Lanes of a row and threads, and the pairs of a thread, 1, 2 or 4: 32 lanes down a head of up to 256 features, 128 of a larger one, 64 where a row is one group.
+// Lanes of a row and threads, and the pairs of a thread: 32 lanes down a head of up to 64 features, 64 of one of up to 256, 128 of a larger one, 64 where a row is one group.
 struct Cut { uint32_t lanes, threads, pairs; };
 Cut cut_of(int type, uint32_t D, uint32_t rot, uint32_t B)
 {
     const uint32_t V = 16u / (uint32_t)so_type_bytes(type), pairs = rot / 2u + (D - rot + 1u) / 2u;
     Cut c;
     c.lanes = B <= V ? 1 : pairs > 128 ? 4 : B <= 2 * V ? 2 : B <= 4 * V ? 4 : 8;
-    c.threads = c.lanes == 1 ? 64 : pairs > 128 ? 512 : 32 * c.lanes;
+    c.threads = c.lanes == 1 ? 64 : pairs > 128 ? 512 : (pairs > 32 ? 64 : 32) * c.lanes;
     const uint32_t each = so_ceil_div(pairs, c.threads / c.lanes);
     c.pairs = each <= 1 ? 1 : each <= 2 ? 2 : 4;
     return c;
@@ -251,9 +281,11 @@ Shape shape_of(const so_ctx *ctx, const Cut &c, int type, uint32_t heads_q, uint
 {
     Shape s = {heads_q, heads_q + heads_k, D, B, rot, layout == SO_ROTARY_PAIRS, 0, 1, 0, 0};
     s.tiles = so_ceil_div(B, c.lanes * (16u / (uint32_t)so_type_bytes(type)));
-    // as many heads a workgroup as leave every compute unit 2048 threads: the turns are worked out once for all of them
-    const uint64_t want = (uint64_t)ctx->compute_units * (2048u / c.threads);
-    s.per = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((uint64_t)s.tiles * s.heads / want, s.heads));
+    // The turns are worked out once for all heads of a workgroup, and the next head is on its way while one is turned: as many heads a workgroup as all there are, dealt to two workgroups of 512
+    // threads on every compute unit.  32 + 8 heads of 128 x 8192 bf16, 10 a workgroup: 38.6 us; 5: 43; 2: 45; 20: 45.  The gradient of 24 + 8 heads of 96 x 4099 fp16, 5 a workgroup: 33 us; 4: 37;
+    // 1: 43; 10: 39.
+    const uint64_t room = (uint64_t)ctx->compute_units * (1024u / c.threads);
+    s.per = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(((uint64_t)s.tiles * s.heads + room - 1u) / room, s.heads));
     s.groups_q = so_ceil_div(heads_q, s.per);
     s.groups = s.groups_q + so_ceil_div(heads_k, s.per);
     return s;
@@ -264,16 +296,24 @@ size_t share_bytes(const Shape &s) { return (size_t)s.tiles * s.groups * s.D * s
 template <class F>
 void for_cut(const Cut &c, F &&f)
 {
-    const auto with = [&](auto lanes, auto threads) {
-        if (c.pairs == 1) f(lanes, std::integral_constant<int, 1>(), threads);
-        else if (c.pairs == 2) f(lanes, std::integral_constant<int, 2>(), threads);
-        else f(lanes, std::integral_constant<int, 4>(), threads);
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    const auto with = [&](auto lanes) {
+        constexpr int N = decltype(lanes)::value;
+        const std::integral_constant<int, 64 * N> threads;
+        if (c.threads == 32 * N) f(lanes, one, std::integral_constant<int, 32 * N>());
+        else if (c.pairs == 1) f(lanes, one, threads);
+        else f(lanes, two, threads);
     };
-    if (c.lanes == 1) with(std::integral_constant<int, 1>(), std::integral_constant<int, 64>());
-    else if (c.lanes == 2) with(std::integral_constant<int, 2>(), std::integral_constant<int, 64>());
-    else if (c.threads == 512) f(std::integral_constant<int, 4>(), std::integral_constant<int, 2>(), std::integral_constant<int, 512>());
-    else if (c.lanes == 4) with(std::integral_constant<int, 4>(), std::integral_constant<int, 128>());
-    else with(std::integral_constant<int, 8>(), std::integral_constant<int, 256>());
+    if (c.lanes == 1) {
+        const std::integral_constant<int, 64> threads;
+        if (c.pairs == 1) f(one, one, threads);
+        else if (c.pairs == 2) f(one, two, threads);
+        else f(one, std::integral_constant<int, 4>(), threads);
+    } else if (c.lanes == 2) with(two);
+    else if (c.lanes == 8) with(std::integral_constant<int, 8>());
+    else if (c.threads == 512) f(std::integral_constant<int, 4>(), two, std::integral_constant<int, 512>());
+    else with(std::integral_constant<int, 4>());
 }
 
 so_status workspace(so_ctx *ctx, const char *who, size_t bytes)
