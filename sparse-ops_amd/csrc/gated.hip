@@ -11,12 +11,55 @@ using so_dense::Operand;
 
 constexpr int kThreads = 256;
 
+// A long contraction over few tiles of the result is dealt to workgroups piece by piece: each piece's sums go to the workspace as [piece][row][column], fp32, and are added up in order by a kernel of their own.
+struct Pieces {
+    float *to;                       // null: no pieces
+    uint32_t cuts, depth;            // of one product: how many, and of how many terms
+    size_t pitch;
+    __device__ __forceinline__ float *at(uint64_t row, uint64_t col) const { return to + row * pitch + col; }
+};
+
+// The piece of an operand that begins at k0, its rows along the contraction or across.
+template <class T, bool ACROSS>
+__device__ __forceinline__ Operand<T> piece_of(const Operand<T> &o, uint32_t k0, uint32_t depth)
+{
+    return {o.p + (ACROSS ? k0 * o.ld : k0), o.ld, o.own, min(depth, o.depth - k0)};
+}
+
+// V neighbouring sums of a row from its pieces, `between` rows apart.
+template <int V>
+__device__ __forceinline__ void join(const Pieces &p, uint32_t count, uint64_t between, uint64_t row, uint64_t col, float (&v)[V])
+{
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = 0.0f;
+    constexpr uint32_t AHEAD = 32 / V;
+    for (uint32_t i = 0; i < count; i += AHEAD) {
+        f32x4 w[AHEAD][V / 4];
+#pragma unroll
+        for (uint32_t j = 0; j < AHEAD; ++j)
+#pragma unroll
+            for (int e = 0; e < V; e += 4) w[j][e / 4] = *reinterpret_cast<const f32x4 *>(p.at(row + min(i + j, count - 1u) * between, col + e));
+#pragma unroll
+        for (uint32_t j = 0; j < AHEAD; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] += i + j < count ? w[j][e / 4][e % 4] : 0.0f;
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void keep(const Pieces &p, uint64_t row, uint64_t col, const float (&v)[V])
+{
+#pragma unroll
+    for (int e = 0; e < V; e += 4) *reinterpret_cast<f32x4 *>(p.at(row, col + e)) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+}
+
 template <class T> struct Forward {
     const T *Wg, *Wu, *X, *G0, *U0;
     T *H, *G, *U;
     size_t ldw, ldx, ld0, ldh, ldg;
     uint32_t m, n, B;
     int act;
+    Pieces pieces;
 };
 
 // The results of V neighbouring columns of a row from its two sums.
@@ -51,11 +94,36 @@ void gated_kernel(Forward<T> f, Grid grid)
     const auto spot = so_dense::spot_of(grid);
     if (spot.none) return;
     so_dense::Loop<T, TILE, false, true, true> loop;
-    const uint64_t i0 = (uint64_t)spot.m * (TILE::ROWS / 2), j0 = (uint64_t)spot.c * TILE::COLS;
-    loop.template add<DIRECT>(stage, {{f.Wg, f.ldw, f.m, f.n}, {f.Wu, f.ldw, f.m, f.n}}, i0, {f.X, f.ldx, f.B, f.n}, j0);
+    constexpr bool PIECES = TILE::ROWS < 256;                            // of the largest tile there are enough
+    const bool pieces = PIECES && f.pieces.to;
+    const uint32_t each = (f.m + TILE::ROWS / 2 - 1u) / (TILE::ROWS / 2), piece = pieces ? spot.m / each : 0u, k0 = piece * f.pieces.depth;
+    const uint64_t i0 = (uint64_t)(spot.m - piece * each) * (TILE::ROWS / 2), j0 = (uint64_t)spot.c * TILE::COLS;
+    const Operand<T> g = {f.Wg, f.ldw, f.m, f.n}, u = {f.Wu, f.ldw, f.m, f.n}, x = {f.X, f.ldx, f.B, f.n};
+    if constexpr (!PIECES) loop.template add<DIRECT>(stage, {g, u}, i0, x, j0);
+    else loop.template add<DIRECT>(stage, {piece_of<T, false>(g, k0, f.pieces.depth), piece_of<T, false>(u, k0, f.pieces.depth)}, i0, piece_of<T, true>(x, k0, f.pieces.depth), j0);
     __syncthreads();
     const uint64_t row0 = i0 + threadIdx.x / 64u / TILE::WC * (TILE::RT / 2 * 16);
-    loop.template out<2>(stage, [&](int i, uint32_t r, uint32_t c, float (&v)[2][so_elements<T>::V]) { finish(f, row0 + i * 16 + r, j0 + c, v[0], v[1]); });
+    loop.template out<2>(stage, [&](int i, uint32_t r, uint32_t c, float (&v)[2][so_elements<T>::V]) {
+        const uint64_t row = row0 + i * 16 + r, col = j0 + c;
+        if (!pieces) return finish(f, row, col, v[0], v[1]);
+        if (row >= f.m || col >= f.B) return;
+        keep(f.pieces, piece * 2u * (uint64_t)f.m + row, col, v[0]);
+        keep(f.pieces, (piece * 2u + 1u) * (uint64_t)f.m + row, col, v[1]);
+    });
+}
+
+// Both sums from their pieces, and what follows them.
+template <class T>
+__global__ __launch_bounds__(kThreads)
+void gated_join_kernel(Forward<T> f, uint32_t groups)
+{
+    constexpr int V = so_elements<T>::V;
+    const uint64_t at = (uint64_t)blockIdx.x * kThreads + threadIdx.x, row = at / groups, col = at % groups * V;
+    if (row >= f.m) return;
+    float g[V], u[V];
+    join(f.pieces, f.pieces.cuts, 2u * (uint64_t)f.m, row, col, g);
+    join(f.pieces, f.pieces.cuts, 2u * (uint64_t)f.m, row + f.m, col, u);
+    finish(f, row, col, g, u);
 }
 
 // One column: a wave takes R rows of both projections, 64 lanes a group of 16 bytes each, and holds a panel of kPanel groups a lane of X in registers for them.
@@ -197,6 +265,7 @@ template <class T> struct Product {
     T *Y, *Y2;
     size_t ldy;
     uint32_t rows, cols, terms;      // of one part; products to add
+    Pieces pieces;                   // of either product in turn
 };
 
 template <class T, class TILE, bool AX, bool BX, bool DIRECT>
@@ -206,17 +275,39 @@ void product_kernel(Product<T> p, Grid grid)
     extern __shared__ char stage[];
     const auto spot = so_dense::spot_of(grid);
     if (spot.none) return;
-    const uint32_t each = (p.rows + TILE::ROWS - 1u) / TILE::ROWS, second = spot.m >= each ? 1u : 0u;
+    const uint32_t each = (p.rows + TILE::ROWS - 1u) / TILE::ROWS, tiles = p.Y2 ? 2u * each : each;
+    constexpr bool PIECES = TILE::ROWS < 256;                            // of the largest tile there are enough
+    const bool pieces = PIECES && p.pieces.to;
+    const uint32_t piece = pieces ? spot.m / tiles : 0u, m = spot.m - piece * tiles, second = m >= each ? 1u : 0u;
     so_dense::Loop<T, TILE, AX, BX, false> loop;
-    const uint64_t i0 = (uint64_t)(spot.m - second * each) * TILE::ROWS, j0 = (uint64_t)spot.c * TILE::COLS;
-    for (uint32_t t = 0; t < p.terms; ++t) loop.template add<DIRECT>(stage, {p.A[second + t]}, i0, p.B[second + t], j0);
+    const uint64_t i0 = (uint64_t)(m - second * each) * TILE::ROWS, j0 = (uint64_t)spot.c * TILE::COLS;
+    const uint32_t term = pieces ? piece / p.pieces.cuts : 0u, k0 = (piece - term * p.pieces.cuts) * p.pieces.depth;
+    for (uint32_t t = term; t < (pieces ? term + 1u : p.terms); ++t) {
+        if constexpr (PIECES) loop.template add<DIRECT>(stage, {piece_of<T, AX>(p.A[second + t], k0, p.pieces.depth)}, i0, piece_of<T, BX>(p.B[second + t], k0, p.pieces.depth), j0);
+        else loop.template add<DIRECT>(stage, {p.A[second + t]}, i0, p.B[second + t], j0);
+    }
     __syncthreads();
     T *Y = second ? p.Y2 : p.Y;
-    const uint64_t row0 = i0 + threadIdx.x / 64u / TILE::WC * (TILE::RT * 16);
+    const uint64_t row0 = i0 + threadIdx.x / 64u / TILE::WC * (TILE::RT * 16), kept = (tiles == each ? piece : 2u * piece + second) * (uint64_t)p.rows;
     loop.template out<1>(stage, [&](int i, uint32_t r, uint32_t c, float (&v)[1][so_elements<T>::V]) {
         const uint64_t row = row0 + i * 16 + r, col = j0 + c;
-        if (row < p.rows && col < p.cols) so_group_store(Y + row * p.ldy + col, (uint32_t)min((uint64_t)so_elements<T>::V, p.cols - col), v[0]);
+        if (row >= p.rows || col >= p.cols) return;
+        if (pieces) keep(p.pieces, kept + row, col, v[0]);
+        else so_group_store(Y + row * p.ldy + col, (uint32_t)min((uint64_t)so_elements<T>::V, p.cols - col), v[0]);
     });
+}
+
+template <class T>
+__global__ __launch_bounds__(kThreads)
+void product_join_kernel(Product<T> p, uint32_t groups, uint32_t parts)
+{
+    constexpr int V = so_elements<T>::V;
+    const uint64_t at = (uint64_t)blockIdx.x * kThreads + threadIdx.x, row = at / groups, col = at % groups * V;
+    if (row >= (uint64_t)parts * p.rows) return;
+    float v[V];
+    join(p.pieces, p.terms * p.pieces.cuts, (uint64_t)parts * p.rows, row, col, v);
+    T *Y = row >= p.rows ? p.Y2 + (row - p.rows) * p.ldy : p.Y + row * p.ldy;
+    so_group_store(Y + col, (uint32_t)min((uint64_t)V, p.cols - col), v);
 }
 
 // Tiles, by rows and columns of the result (of both projections together in the forward pass).
@@ -227,33 +318,71 @@ typedef so_dense::Tile<2, 2, 2, 2, 128, 4> T64x64;
 typedef so_dense::Tile<2, 1, 1, 4, 256, 3, true> T32x64;
 typedef so_dense::Tile<2, 1, 1, 2, 256, 4, true> T32x32;
 
-struct Form { uint32_t rows, cols; const char *name; };
-constexpr Form kForms[] = {{32, 32, "gated-32x32"}, {32, 64, "gated-32x64"}, {64, 64, "gated-64x64"}, {64, 128, "gated-64x128"}, {128, 128, "gated-128x128"}, {256, 256, "gated-256x256"}};
+// A KiB of the contraction of one tile on every compute unit, and of one more tile, in us, for elements of 2 and of 4 bytes: operands past the registers, both of them across the contraction (dX's), and by way of the
+// registers (two tiles only).  Measured with 256, 512, 768 and 1024 tiles of each form and contractions of 4 and 8 KiB: 64 x 128 in 16 bits, say, takes 2.8, 4.7, 7.6 and 9.6 us a KiB.  A turn
+// of tiles takes 1.5 us besides, and a unit stores its results at 20 bytes a ns.
+struct Rate { float first, other; };
+struct Form { uint32_t rows, cols; const char *name; Rate along[2], across[2], any[2]; };
+constexpr Form kForms[] = {
+    {32, 32, "gated-32x32", {{1.4f, 1.4f}, {2.6f, 2.1f}}, {{1.1f, 1.2f}, {2.4f, 2.2f}}, {}},
+    {32, 64, "gated-32x64", {{1.6f, 1.4f}, {2.8f, 2.1f}}, {{1.6f, 1.2f}, {2.7f, 2.4f}}, {}},
+    {64, 64, "gated-64x64", {{1.9f, 1.4f}, {4.6f, 3.9f}}, {{2.3f, 1.3f}, {4.8f, 4.1f}}, {{3.2f, 1.2f}, {5.7f, 3.7f}}},
+    {64, 128, "gated-64x128", {{2.8f, 2.3f}, {9.4f, 7.8f}}, {{3.6f, 2.1f}, {10.5f, 8.2f}}, {}},
+    {128, 128, "gated-128x128", {{5.7f, 4.6f}, {18.0f, 15.5f}}, {{4.8f, 3.2f}, {16.2f, 15.1f}}, {{6.5f, 4.2f}, {18.8f, 14.5f}}},
+    {256, 256, "gated-256x256", {{13.0f, 13.0f}, {}}, {{11.5f, 11.6f}, {}}, {}},
+};
 constexpr int kFormCount = 6;
 
-// The largest tile that gives every compute unit a workgroup, not half of whose columns would do: a larger one asks the caches for less, a smaller one leaves none idle.  From a sweep (bf16 forward, us, this form /
-// its neighbours): 8192 x 4096 (m x n) at B = 24 32 x 32 27 / 28, 64 64 x 64 32 / 33 and 37, 128 64 x 128 39 / 43 and 53; 4096 x 4096 at 24 32 x 32 15.8 / 19, 64 32 x 64 19.8 / 27 and 24, 256
-// 64 x 128 33 / 36 and 51; 2048 x 2048 at 128 32 x 64 10.5 / 11.4 and 11.5; 2048 x 1024 at 64 32 x 32 6.3 / 6.8.  fp32 has no use for the largest: its products take eight times as long.
-int choose_form(const so_ctx *ctx, int most, uint64_t rows, uint64_t cols)
+// How a result of `rows` x `cols` is made of `terms` products of `depth` each: the tile, and in how many pieces; what takes least by the rates above.  Not half of a tile's
+// columns would do: fewer of the weights' rows a workgroup keep more of them on their way (24 columns of 8192 x 4096 fp16: 32 x 32 27 us, 64 x 64 33).  The pieces' sums are written and read at 4 TB/s, by a launch of 3 us.
+struct Plan {
+    bool direct;
+    int form;
+    uint32_t cuts, depth;
+    size_t pitch, bytes;             // of the pieces in the workspace, 0: none
+    Pieces pieces(void *at) const { return {bytes ? (float *)at : nullptr, cuts, depth, pitch}; }
+};
+Plan plan_of(const so_ctx *ctx, int type, bool direct, uint64_t rows, uint32_t cols, uint32_t terms, uint32_t depth)
 {
-    if (ctx->tune.gated_form >= 1 && ctx->tune.gated_form <= kFormCount) return std::min(ctx->tune.gated_form - 1, most);
-    const auto tiles = [&](int f) { return (uint64_t)so_ceil_div(rows, kForms[f].rows) * so_ceil_div(cols, kForms[f].cols); };
-    for (int f = most; f > 0; --f)
-        if (tiles(f) >= (uint64_t)ctx->compute_units && cols > kForms[f].cols / 2) return f;
-    return 0;
+    Plan p = {direct, 2, 1, depth, (cols + 7u) / 8u * (size_t)8, 0};
+    const uint32_t size = (uint32_t)so_type_bytes(type), units = (uint32_t)ctx->compute_units;
+    const float length = (float)terms * (float)depth * (float)size / 1024.0f;
+    const int forced = ctx->tune.gated_form < 1 || ctx->tune.gated_form > kFormCount ? -1 : std::min(ctx->tune.gated_form - 1, size == 4 ? 4 : 5);
+    uint32_t pieces = 1;
+    float least = INFINITY;
+    for (int f = 0; f < kFormCount; ++f) {
+        const Rate rate = (!direct ? kForms[f].any : terms == 2 ? kForms[f].across : kForms[f].along)[size / 4u];
+        if (rate.first == 0.0f || (direct && (forced >= 0 ? f != forced : f && cols <= kForms[f].cols / 2))) continue;
+        const uint64_t tiles = (uint64_t)so_ceil_div(rows, kForms[f].rows) * so_ceil_div(cols, kForms[f].cols);
+        // pieces of a KiB at least, as long as there are fewer than three for every unit
+        for (uint32_t n = 1; n <= 32 && (n == 1 || ((float)n <= length && tiles * n < 3ull * units && f < 5)); n += n < terms ? terms - n : terms) {
+            const float turns = (float)((tiles * n + units - 1) / units);
+            const float results = (float)(kForms[f].rows * kForms[f].cols) * (n > 1 ? 4.0f : (float)size);
+            const float time = (rate.first + (turns - 1.0f) * rate.other) * length / (float)n + turns * (1.5f + results / 20000.0f) + (n > 1 ? 3.0f + (float)n * (0.25f + (float)rows * (float)p.pitch * 2e-6f) : 0.0f);
+            if (time < least) {
+                least = time;
+                p.form = f;
+                pieces = n;
+            }
+        }
+    }
+    if (pieces == 1) return p;
+    p.depth = so_ceil_div(so_ceil_div(depth, pieces / terms), 256u / size) * (256u / size);      // whole steps of the smallest tile
+    p.cuts = so_ceil_div(depth, p.depth);
+    p.bytes = (uint64_t)p.cuts * terms * rows * p.pitch * sizeof(float);
+    return p;
 }
 
-// f(a tile, whether operands go past the registers).  By way of them only two sizes, as large as they go.
+// f(a tile, whether operands go past the registers)
 template <class T, class F>
-so_status for_tile(so_ctx *ctx, uint64_t rows, uint64_t cols, bool direct, F &&f)
+so_status for_tile(so_ctx *ctx, const Plan &p, F &&f)
 {
-    const int form = choose_form(ctx, direct ? (sizeof(T) == 2 ? 5 : 4) : 4, rows, cols);
-    ctx->last_kernel = kForms[form].name;
-    if (!direct) {
-        ctx->last_kernel = form == 4 ? "gated-128x128-any" : "gated-64x64-any";
-        return form == 4 ? f(T128x128(), std::false_type()) : f(T64x64(), std::false_type());
+    ctx->last_kernel = kForms[p.form].name;
+    if (!p.direct) {
+        ctx->last_kernel = p.form == 4 ? "gated-128x128-any" : "gated-64x64-any";
+        return p.form == 4 ? f(T128x128(), std::false_type()) : f(T64x64(), std::false_type());
     }
-    switch (form) {
+    switch (p.form) {
     case 0: return f(T32x32(), std::true_type());
     case 1: return f(T32x64(), std::true_type());
     case 2: return f(T64x64(), std::true_type());
@@ -276,18 +405,6 @@ so_status launch_tiles(so_ctx *ctx, const char *who, Kernel kernel, const Arg &a
     return SO_OK;
 }
 
-template <class T, bool AX, bool BX>
-so_status product(so_ctx *ctx, const Product<T> &p)
-{
-    const uint32_t parts = p.Y2 ? 2 : 1;
-    bool direct = true;
-    for (uint32_t i = 0; i < std::max(parts, p.terms); ++i) direct = direct && p.A[i].direct() && p.B[i].direct();
-    return for_tile<T>(ctx, (uint64_t)parts * p.rows, p.cols, direct, [&](auto t, auto past) {
-        typedef decltype(t) TILE;
-        return launch_tiles<TILE>(ctx, "so_gated_grad", product_kernel<T, TILE, AX, BX, decltype(past)::value>, p, (uint64_t)parts * so_ceil_div(p.rows, TILE::ROWS), so_ceil_div(p.cols, TILE::COLS));
-    });
-}
-
 so_status workspace(so_ctx *ctx, const char *who, size_t bytes)
 {
     SO_REQUIRE(!ctx->capturing || (ctx->mm_part && ctx->mm_part->bytes >= bytes),
@@ -298,8 +415,27 @@ so_status workspace(so_ctx *ctx, const char *who, size_t bytes)
 // Bytes of a matrix in the workspace, its rows at multiples of 16 bytes.
 size_t stride_of(uint32_t cols) { return (cols + 7u) / 8u * (size_t)8; }
 size_t bytes_of(int type, uint32_t rows, uint32_t cols) { return rows * stride_of(cols) * so_type_bytes(type); }
+template <class T> bool direct_there(uint32_t cols) { return Operand<T>{nullptr, stride_of(cols), 0, 0}.direct(); }
 
 template <class T> uint64_t blocks_of(uint32_t rows, uint32_t groups) { return ((uint64_t)rows * groups + kThreads - 1) / kThreads; }
+
+template <class T, bool AX, bool BX>
+so_status product(so_ctx *ctx, const Product<T> &p, const Plan &plan)
+{
+    const uint32_t parts = p.Y2 ? 2 : 1;
+    const so_status status = for_tile<T>(ctx, plan, [&](auto t, auto past) {
+        typedef decltype(t) TILE;
+        return launch_tiles<TILE>(ctx, "so_gated_grad", product_kernel<T, TILE, AX, BX, decltype(past)::value>, p,
+                                  (uint64_t)(plan.bytes ? p.terms * plan.cuts : 1u) * parts * so_ceil_div(p.rows, TILE::ROWS), so_ceil_div(p.cols, TILE::COLS));
+    });
+    if (status != SO_OK || !plan.bytes) return status;
+    const uint32_t groups = so_ceil_div(p.cols, so_elements<T>::V);
+    const uint64_t blocks = ((uint64_t)parts * p.rows * groups + kThreads - 1) / kThreads;
+    SO_REQUIRE(so_grid_fits(blocks, kThreads), "so_gated_grad: the result is too large for one launch");
+    product_join_kernel<T><<<(uint32_t)blocks, kThreads, 0, ctx->stream>>>(p, groups, parts);
+    SO_LAUNCH_CHECK();
+    return SO_OK;
+}
 
 // m in the workspace at `to`, aligned.
 template <class T>
@@ -341,16 +477,28 @@ so_status forward(so_ctx *ctx, int type, Forward<T> f)
     }
     const Operand<T> g = {f.Wg, f.ldw, f.m, f.n}, u = {f.Wu, f.ldw, f.m, f.n};
     Operand<T> x = {f.X, f.ldx, f.B, f.n};
-    if (g.direct() && u.direct() && !x.direct()) {
-        if (const so_status s = workspace(ctx, "so_gated", bytes_of(type, f.n, f.B)); s != SO_OK) return s;
+    const bool align = g.direct() && u.direct() && !x.direct();
+    const Plan plan = plan_of(ctx, type, g.direct() && u.direct() && (align ? direct_there<T>(f.B) : x.direct()), 2 * (uint64_t)f.m, f.B, 1, f.n);
+    const size_t aligned = align ? bytes_of(type, f.n, f.B) : 0;
+    if (align || plan.bytes)
+        if (const so_status s = workspace(ctx, "so_gated", aligned + plan.bytes); s != SO_OK) return s;
+    if (align) {
         if (const so_status s = align_rows(ctx, "so_gated", &x, f.n, f.B, ctx->mm_part->p); s != SO_OK) return s;
         f.X = x.p;
         f.ldx = x.ld;
     }
-    return for_tile<T>(ctx, 2 * (uint64_t)f.m, f.B, g.direct() && u.direct() && x.direct(), [&](auto t, auto direct) {
+    f.pieces = plan.pieces(plan.bytes ? (char *)ctx->mm_part->p + aligned : nullptr);
+    const so_status status = for_tile<T>(ctx, plan, [&](auto t, auto past) {
         typedef decltype(t) TILE;
-        return launch_tiles<TILE>(ctx, "so_gated", gated_kernel<T, TILE, decltype(direct)::value>, f, so_ceil_div(f.m, TILE::ROWS / 2), so_ceil_div(f.B, TILE::COLS));
+        return launch_tiles<TILE>(ctx, "so_gated", gated_kernel<T, TILE, decltype(past)::value>, f, (uint64_t)plan.cuts * so_ceil_div(f.m, TILE::ROWS / 2), so_ceil_div(f.B, TILE::COLS));
     });
+    if (status != SO_OK || !plan.bytes) return status;
+    const uint32_t groups = so_ceil_div(f.B, so_elements<T>::V);
+    const uint64_t blocks = blocks_of<T>(f.m, groups);
+    SO_REQUIRE(so_grid_fits(blocks, kThreads), "so_gated: %u x %u is too large for one launch", f.m, f.B);
+    gated_join_kernel<T><<<(uint32_t)blocks, kThreads, 0, ctx->stream>>>(f, groups);
+    SO_LAUNCH_CHECK();
+    return SO_OK;
 }
 
 // The three gradients from dG and dU, either of which may have to go to the caller too.
@@ -365,25 +513,32 @@ so_status backward(so_ctx *ctx, int type, Slopes<T> s, uint32_t n, const Operand
     const bool weights = r.dWg || r.dWu, products = r.dX || weights;
     so_status status = SO_OK;
     Operand<T> d[2] = {{s.to[0].g, s.to[0].ld, B, m}, {s.to[0].u, s.to[0].ld, B, m}};
+    const uint32_t parts = r.dWg && r.dWu ? 2u : 1u;
+    const bool to_workspace = products && !(s.to[0].g && s.to[0].u && d[0].direct() && d[1].direct()), align = weights && !x.direct();
+    const bool direct = to_workspace ? direct_there<T>(B) : d[0].direct() && d[1].direct();
+    const Plan dx = plan_of(ctx, type, direct && W[0].direct() && W[1].direct(), n, B, 2, m);
+    const Plan dw = plan_of(ctx, type, direct && (align ? direct_there<T>(B) : x.direct()), (uint64_t)parts * m, n, 1, B);
+    char *pieces = nullptr;
     if (m && B) {
-        const bool to_workspace = products && !(s.to[0].g && s.to[0].u && d[0].direct() && d[1].direct()), align = weights && !x.direct();
-        if (to_workspace || align) {
-            const size_t each = bytes_of(type, m, B);
-            if ((status = workspace(ctx, "so_gated_grad", 2 * each + bytes_of(type, n, B))) != SO_OK) return status;
+        const size_t each = to_workspace ? bytes_of(type, m, B) : 0, aligned = align ? bytes_of(type, n, B) : 0;
+        const size_t bytes = 2 * each + aligned + std::max(r.dX ? dx.bytes : 0, weights ? dw.bytes : 0);
+        if (bytes) {
+            if ((status = workspace(ctx, "so_gated_grad", bytes)) != SO_OK) return status;
             char *at = (char *)ctx->mm_part->p;
             if (to_workspace) {
                 s.to[1] = {(T *)at, (T *)(at + each), stride_of(B)};
                 for (int i = 0; i < 2; ++i) d[i] = {(const T *)(at + i * each), stride_of(B), B, m};
             }
             if (align && (status = align_rows(ctx, "so_gated_grad", &x, n, B, at + 2 * each)) != SO_OK) return status;
+            pieces = at + 2 * each + aligned;
         }
         if ((status = slopes(ctx, s)) != SO_OK) return status;
     }
-    if (r.dX && B) status = product<T, true, true>(ctx, {{W[0], W[1]}, {d[0], d[1]}, (T *)r.dX, nullptr, r.ldx, n, B, 2});
+    if (r.dX && B) status = product<T, true, true>(ctx, {{W[0], W[1]}, {d[0], d[1]}, (T *)r.dX, nullptr, r.ldx, n, B, 2, dx.pieces(pieces)}, dx);
     if (status != SO_OK || !weights || !m) return status;
     const Operand<T> along = {x.p, x.ld, n, B}, g = {d[0].p, d[0].ld, m, B}, u = {d[1].p, d[1].ld, m, B};
-    if (r.dWg && r.dWu) return product<T, false, false>(ctx, {{g, u}, {along, along}, (T *)r.dWg, (T *)r.dWu, r.ldw, m, n, 1});
-    return product<T, false, false>(ctx, {{r.dWg ? g : u, u}, {along, along}, (T *)(r.dWg ? r.dWg : r.dWu), nullptr, r.ldw, m, n, 1});
+    if (parts == 2) return product<T, false, false>(ctx, {{g, u}, {along, along}, (T *)r.dWg, (T *)r.dWu, r.ldw, m, n, 1, dw.pieces(pieces)}, dw);
+    return product<T, false, false>(ctx, {{r.dWg ? g : u, u}, {along, along}, (T *)(r.dWg ? r.dWg : r.dWu), nullptr, r.ldw, m, n, 1, dw.pieces(pieces)}, dw);
 }
 
 } // namespace
@@ -396,7 +551,13 @@ extern "C" so_status so_gated_reserve(so_ctx *ctx, int type, uint32_t m, uint32_
     if (m == 0 || B == 0) return SO_OK;
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
-    return workspace(ctx, "so_gated_reserve", 2 * bytes_of(type, m, B) + bytes_of(type, n, B));
+    size_t pieces = 0;
+    for (const bool direct : {false, true}) {
+        pieces = std::max(pieces, plan_of(ctx, type, direct, 2 * (uint64_t)m, B, 1, n).bytes);
+        pieces = std::max(pieces, plan_of(ctx, type, direct, n, B, 2, m).bytes);
+        for (const uint64_t rows : {(uint64_t)m, 2 * (uint64_t)m}) pieces = std::max(pieces, plan_of(ctx, type, direct, rows, n, 1, B).bytes);
+    }
+    return workspace(ctx, "so_gated_reserve", 2 * bytes_of(type, m, B) + bytes_of(type, n, B) + pieces);
 }
 
 extern "C" so_status so_gated(so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t B, const void *dWg, const void *dWu, size_t w_stride, const void *dX, size_t x_stride, int act,
