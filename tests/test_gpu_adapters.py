@@ -269,3 +269,40 @@ def test_a_workspace_that_must_grow_is_refused_while_recording():
         assert np.all(Y.download() == 64.0 * 64.0 + 1.0)
     finally:
         ctx.close()
+
+
+# a last tile of columns of every kind, ranks that end inside a run of products and a group, adapters and rows to the end of their arrays
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("m,n,C,count,rank", [(70, 40, 256, 3, 1), (33, 72, 257, 4, 3), (100, 130, 320, 5, 10), (17, 64, 383, 2, 33), (65, 33, 449, 3, 100), (40, 200, 300, 6, 4), (130, 24, 511, 2, 256),
+                                              (3, 5, 290, 2, 7), (1, 1, 260, 1, 1)])
+def test_many_columns(ctx, m, n, C, count, rank, type_):
+    rng = np.random.default_rng(C + rank)
+    A, B, scale, X, base = problem(rng, m, n, C, count, rank, type_)
+    for i, (pad, shift) in enumerate(PLACES):
+        for which in (requests(rng, C, count), rng.integers(-1, count + 1, C).astype(np.int32), np.full(C, count - 1, np.int32)):
+            check(run(ctx, A, B, scale if i else None, which, X, base if i != 1 else None, type_, pad, shift, in_place=i == 2), A, B, scale if i else None, which, X, base if i != 1 else None, type_)
+
+
+@pytest.mark.parametrize("type_", TYPES)
+def test_sixty_four_adapters_in_every_tile_of_many_columns(ctx, type_):
+    rng = np.random.default_rng(12)
+    m, n, C, count, rank = 90, 100, 330, 64, 6
+    A, B, scale, X, base = problem(rng, m, n, C, count, rank, type_)
+    which = np.concatenate([rng.permutation(count) for _ in range(6)])[:C].astype(np.int32)
+    check(run(ctx, A, B, scale, which, X, base, type_), A, B, scale, which, X, base, type_)
+
+
+@pytest.mark.parametrize("type_", TYPES)
+def test_a_column_of_many_does_not_depend_on_the_others(ctx, type_):
+    rng = np.random.default_rng(13)
+    m, n, C, count, rank = 70, 140, 300, 6, 9
+    A, B, scale, X, base = problem(rng, m, n, C, count, rank, type_)
+    which = rng.integers(0, count - 1, C).astype(np.int32)
+    mine = rng.random(C) < 0.4
+    first = run(ctx, A, B, scale, which, X, base, type_)
+    A2, B2, X2, base2, which2 = A.copy(), B.copy(), X.copy(), base.copy(), which.copy()
+    which2[~mine] = rng.integers(-1, count + 1, int((~mine).sum()))
+    A2[count - 1], B2[count - 1] = np.nan, np.inf
+    X2[:, ~mine], base2[:, ~mine] = rng.choice([np.nan, np.inf, -np.inf, 1.0], (n, int((~mine).sum()))), np.nan
+    second = run(ctx, A2, B2, scale, which2, X2, base2, type_)
+    assert np.array_equal(first[:, mine], second[:, mine])

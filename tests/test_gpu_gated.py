@@ -424,3 +424,40 @@ def test_two_contexts_at_once():
     finally:
         for ctx in contexts:
             ctx.close()
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("m,n,B", [(24, 6000, 40), (16, 9001, 2), (2500, 33, 20), (33, 50, 5000), (30, 40, 3001), (700, 16, 9), (12, 700, 70)])
+def test_long_contractions_over_few_tiles(ctx, m, n, B, type_):
+    """A result of few tiles is made in pieces of its contraction, of n, m or B terms, which another kernel adds up: twice with the same bits."""
+    rng = np.random.default_rng(m + n + B + 2)
+    for pad, shift, wpad in ((0, 0, 0), (3, 1, 5), (8 - B % 8, 0, 8 - n % 8)):
+        run_forward(ctx, rng, m, n, B, type_, "silu", pad, shift, wpad)
+        run_backward(ctx, rng, m, n, B, type_, "gelu_tanh", pad, shift, wpad)
+    a = Arrays(ctx, type_)
+    Wg, Wu, X, D = (a.put(v)[0] for v in (weights(rng, type_, m, n), weights(rng, type_, m, n), draw(rng, type_, n, B), draw(rng, type_, m, B)))
+    outs = [a.put(np.zeros(s))[0] for s in ((m, B), (m, B), (m, B), (n, B), (m, n), (m, n))]
+    seen = []
+    for _ in range(2):
+        ctx.gated(Wg, Wu, m, n, X, B, "silu", *outs[:3], type=type_)
+        ctx.gated_grad(Wg, Wu, m, n, X, B, "silu", outs[1], outs[2], D, *outs[3:], type=type_)
+        seen.append([o.download().view(np.uint8).copy() for o in outs])
+    for first, second in zip(*seen):
+        assert np.array_equal(first, second)
+    a.free()
+
+
+@pytest.mark.parametrize("type_", TYPES)
+def test_what_is_not_a_number_stays_where_it_is_in_pieces(ctx, type_):
+    rng = np.random.default_rng(18)
+    m, n, B = 40, 5000, 30
+    Wg, Wu, X = weights(rng, type_, m, n), weights(rng, type_, m, n), draw(rng, type_, n, B)
+    Wg[3, 4999], Wu[39, 0], X[2500, 7] = np.nan, np.inf, np.nan
+    a = Arrays(ctx, type_)
+    outs = [a.put(np.zeros((m, B)), 1)[0] for _ in range(3)]
+    ctx.gated(a.put(Wg)[0], a.put(Wu)[0], m, n, a.put(X)[0], B, "silu", *outs, type=type_, h_stride=B + 1, g_stride=B + 1)
+    bad = np.zeros((m, B), bool)
+    bad[3], bad[39], bad[:, 7] = True, True, True
+    H = fetch(outs[0], m, B, type_, 1)[0]
+    assert np.array_equal(~np.isfinite(H), bad)
+    a.free()
