@@ -9,6 +9,8 @@ struct Shape {
     uint32_t heads_q, heads, D, B, rot;
     int pairs;                          // SO_ROTARY_PAIRS
     uint32_t tiles, per, groups_q, groups;      // tiles of columns; heads of a workgroup; groups of them, first the queries'
+    uint32_t strip;                             // tiles of an XCD, 0: as they come
+    uint32_t blocks() const { return (strip ? 8u * strip : tiles) * groups; }
 };
 
 // The rows of a head that a thread holds: pair p is two features that are turned together, or two neighbours of those behind them.
@@ -53,14 +55,17 @@ template <class T, int LC, int PPT, int NT>
 struct Seat {
     static constexpr int V = so_elements<T>::V, RL = NT / LC;
     typedef typename so_elements<T>::plain group;
-    uint32_t tile, c0, left, first, last, wide;     // its columns; heads first .. last - 1
+    uint32_t at, tile, c0, left, first, last, wide; // its number; columns; heads first .. last - 1
     bool query;
     uint2 row[PPT];                                 // inside a head
     bool has[PPT], two[PPT];
     __device__ __forceinline__ Seat(const Shape &s, size_t ld)
     {
-        tile = blockIdx.x % s.tiles;
-        const uint32_t g = blockIdx.x / s.tiles;
+        // Workgroups go round-robin to the 8 XCDs.  With strips neighbouring tiles, which share the lines of memory that rows' tiles end in, are on the same one: the gradient of 24 + 8 heads of 96 x 4099 fp16 with neighbours on
+        // different ones reads 98 MB instead of 50 and takes 30.6 us instead of 26.8.
+        const uint32_t in = s.strip ? blockIdx.x / 8u : blockIdx.x, wide_of = s.strip ? s.strip : s.tiles, g = in / wide_of;
+        tile = in % wide_of + (s.strip ? blockIdx.x % 8u * s.strip : 0u);
+        at = g * s.tiles + tile;
         query = g < s.groups_q;
         first = query ? g * s.per : s.heads_q + (g - s.groups_q) * s.per;
         last = min(first + s.per, query ? s.heads_q : s.heads);
@@ -110,6 +115,7 @@ void rotary_kernel(Shape s, const T *X, size_t ldx, const float *gain_q, const f
     constexpr int V = so_elements<T>::V;
     __shared__ float lds[(NT / 64 + 1) * LC * V];
     const Seat<T, LC, PPT, NT> at(s, ldx);
+    if (at.tile >= s.tiles) return;
     typename so_elements<T>::plain x[PPT][2], next[PPT][2];
     at.load(s, at.first, X, ldx, x);
     float2 turn[PPT][V];
@@ -170,6 +176,7 @@ void rotary_grad_kernel(Shape s, const T *X, size_t ldx, const T *dY, size_t ldd
     typedef typename so_elements<T>::plain group;
     __shared__ float lds[(NT / 64 + 1) * LC * V];
     const Seat<T, LC, PPT, NT> at(s, ldx);
+    if (at.tile >= s.tiles) return;
     const uint32_t wide_d = so_group_wide_rows<T>(at.left, s.heads * s.D, ldd);
     Seat<T, LC, PPT, NT> of_dy = at;
     of_dy.wide = wide_d;
@@ -238,8 +245,8 @@ void rotary_grad_kernel(Shape s, const T *X, size_t ldx, const T *dY, size_t ldd
     for (int k = 0; k < PPT; ++k) {
         const float p = so_norm::sum_lanes<LC>(sum[k].x), q = so_norm::sum_lanes<LC>(sum[k].y);
         if (threadIdx.x % LC == 0) {                                 // the first of a row's lanes: its columns exist where any do
-            if (at.has[k]) shares[(size_t)blockIdx.x * s.D + at.row[k].x] = p;
-            if (at.two[k]) shares[(size_t)blockIdx.x * s.D + at.row[k].y] = q;
+            if (at.has[k]) shares[(size_t)at.at * s.D + at.row[k].x] = p;
+            if (at.two[k]) shares[(size_t)at.at * s.D + at.row[k].y] = q;
         }
     }
 }
@@ -284,7 +291,7 @@ Cut cut_of(int type, uint32_t D, uint32_t rot, uint32_t B)
 
 Shape shape_of(const so_ctx *ctx, const Cut &c, int type, uint32_t heads_q, uint32_t heads_k, uint32_t D, uint32_t B, uint32_t rot, int layout)
 {
-    Shape s = {heads_q, heads_q + heads_k, D, B, rot, layout == SO_ROTARY_PAIRS, 0, 1, 0, 0};
+    Shape s = {heads_q, heads_q + heads_k, D, B, rot, layout == SO_ROTARY_PAIRS, 0, 1, 0, 0, 0};
     s.tiles = so_ceil_div(B, c.lanes * (16u / (uint32_t)so_type_bytes(type)));
     // The turns are worked out once for all heads of a workgroup, and the next head is on its way while one is turned: as many heads a workgroup as all there are, dealt to two workgroups of 512
     // threads on every compute unit.  32 + 8 heads of 128 x 8192 bf16, 10 a workgroup: 38.6 us; 5: 43; 2: 45; 20: 45.  The gradient of 24 + 8 heads of 96 x 4099 fp16, 5 a workgroup: 33 us (now 30.6); 4: 37;
@@ -294,6 +301,15 @@ Shape shape_of(const so_ctx *ctx, const Cut &c, int type, uint32_t heads_q, uint
     s.groups_q = so_ceil_div(heads_q, s.per);
     s.groups = s.groups_q + so_ceil_div(heads_k, s.per);
     return s;
+}
+
+// Of many tiles each XCD gets a strip, where rows do not all begin at a line of memory of 128 bytes; where they do, as they come: 38.6 us of rotary positions of 32 + 8 heads of 128 x 8192 bf16, in strips 40.7.
+void place(Shape &s, int type, std::initializer_list<const void *> arrays, std::initializer_list<size_t> strides)
+{
+    uint64_t bits = 0;
+    for (const void *p : arrays) bits |= (uintptr_t)p;
+    for (const size_t n : strides) bits |= n * so_type_bytes(type);
+    s.strip = bits % 128 && s.tiles >= 64 ? so_ceil_div(s.tiles, 8) : 0;      // fewer would not go to the XCDs evenly
 }
 
 size_t share_bytes(const Shape &s) { return (size_t)s.tiles * s.groups * s.D * sizeof(float); }
@@ -328,7 +344,7 @@ so_status workspace(so_ctx *ctx, const char *who, size_t bytes)
     return so_matmul_workspace(ctx, bytes, 4);
 }
 
-bool launch_fits(const Shape &s, const Cut &c) { return so_grid_fits((uint64_t)s.tiles * s.groups, c.threads) && (uint64_t)s.heads * s.D < (1ull << 32); }
+bool launch_fits(const Shape &s, const Cut &c) { return so_grid_fits(((uint64_t)s.tiles + 7) * s.groups, c.threads) && (uint64_t)s.heads * s.D < (1ull << 32); }
 
 } // namespace
 
@@ -367,14 +383,15 @@ extern "C" so_status so_head_rotary(so_ctx *ctx, int type, uint32_t heads_q, uin
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
     const Cut c = cut_of(type, D, rot, B);
-    const Shape s = shape_of(ctx, c, type, heads_q, heads_k, D, B, rot, layout);
+    Shape s = shape_of(ctx, c, type, heads_q, heads_k, D, B, rot, layout);
+    place(s, type, {dX, dY}, {x_stride, y_stride});
     SO_REQUIRE(launch_fits(s, c), "so_head_rotary: %u x %u is too large for one launch", s.heads * D, B);
     so_for_type(type, [&](auto t) {
         using T = decltype(t);
         for_cut(c, [&](auto lanes, auto pairs, auto threads) {
             constexpr int LC = decltype(lanes)::value, PPT = decltype(pairs)::value, NT = decltype(threads)::value;
             const auto kernel = norm ? rotary_kernel<T, LC, PPT, NT, true> : rotary_kernel<T, LC, PPT, NT, false>;
-            kernel<<<s.tiles * s.groups, NT, 0, ctx->stream>>>(s, (const T *)dX, x_stride, dGainQ, dGainK, eps, dPos, dFreq, amplitude, 1.0f, (T *)dY, y_stride, dRstd);
+            kernel<<<s.blocks(), NT, 0, ctx->stream>>>(s, (const T *)dX, x_stride, dGainQ, dGainK, eps, dPos, dFreq, amplitude, 1.0f, (T *)dY, y_stride, dRstd);
         });
     });
     SO_LAUNCH_CHECK();
@@ -406,7 +423,8 @@ extern "C" so_status so_head_rotary_grad(so_ctx *ctx, int type, uint32_t heads_q
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
     const Cut c = cut_of(type, D, rot, std::max(B, 1u));
-    const Shape s = shape_of(ctx, c, type, heads_q, heads_k, D, B, rot, layout);
+    Shape s = shape_of(ctx, c, type, heads_q, heads_k, D, B, rot, layout);
+    place(s, type, {norm ? dX : nullptr, dDy, dDx}, {norm ? x_stride : 0, dy_stride, dDx ? dx_stride : 0});
     SO_REQUIRE(launch_fits(s, c), "so_head_rotary_grad: %u x %u is too large for one launch", s.heads * D, B);
     float *shares = nullptr;
     if (gains && any) {
@@ -419,10 +437,10 @@ extern "C" so_status so_head_rotary_grad(so_ctx *ctx, int type, uint32_t heads_q
             for_cut(c, [&](auto lanes, auto pairs, auto threads) {
                 constexpr int LC = decltype(lanes)::value, PPT = decltype(pairs)::value, NT = decltype(threads)::value;
                 if (norm)
-                    rotary_grad_kernel<T, LC, PPT, NT><<<s.tiles * s.groups, NT, 0, ctx->stream>>>(s, (const T *)dX, x_stride, (const T *)dDy, dy_stride, dGainQ, dGainK, dRstd, dPos, dFreq,
+                    rotary_grad_kernel<T, LC, PPT, NT><<<s.blocks(), NT, 0, ctx->stream>>>(s, (const T *)dX, x_stride, (const T *)dDy, dy_stride, dGainQ, dGainK, dRstd, dPos, dFreq,
                                                                                                      amplitude, (T *)dDx, dx_stride, shares);
                 else
-                    rotary_kernel<T, LC, PPT, NT, false><<<s.tiles * s.groups, NT, 0, ctx->stream>>>(s, (const T *)dDy, dy_stride, nullptr, nullptr, 0.0f, dPos, dFreq, amplitude, -1.0f, (T *)dDx,
+                    rotary_kernel<T, LC, PPT, NT, false><<<s.blocks(), NT, 0, ctx->stream>>>(s, (const T *)dDy, dy_stride, nullptr, nullptr, 0.0f, dPos, dFreq, amplitude, -1.0f, (T *)dDx,
                                                                                                        dx_stride, nullptr);
             });
         });

@@ -343,3 +343,12 @@ def test_recorded_ahead_of_the_first_launch(type_, q, k, D, rot, B):
         ctx.graph_free(graph)
     finally:
         ctx.close()
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("q,k,D,rot,B", [(3, 2, 32, 32, 4161), (1, 1, 16, 8, 8300), (2, 0, 130, 20, 4200), (0, 1, 300, 300, 4100)])
+def test_many_tiles_of_columns(ctx, q, k, D, rot, B, type_):
+    rng = np.random.default_rng(B + D)
+    for pad, shift in ((0, 0), (3, 1), (128 - B % 64, 0)):
+        run_forward(ctx, rng, q, k, D, rot, B, type_, "halves", pad != 3, pad=pad, shift=shift)
+        run_backward(ctx, rng, q, k, D, rot, B, type_, "pairs", pad != 3, pad=pad, shift=shift, in_place=(None, "X", "dY")[pad % 3])
