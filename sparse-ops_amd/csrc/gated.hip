@@ -367,7 +367,8 @@ Plan plan_of(const so_ctx *ctx, int type, bool direct, uint64_t rows, uint32_t c
         }
     }
     if (pieces == 1) return p;
-    p.depth = so_ceil_div(so_ceil_div(depth, pieces / terms), 256u / size) * (256u / size);      // whole steps of the smallest tile
+    const uint64_t step = 256u / size;                                   // whole steps of the smallest tile
+    p.depth = (uint32_t)std::min<uint64_t>(so_ceil_div(so_ceil_div(depth, pieces / terms), step) * step, depth);
     p.cuts = so_ceil_div(depth, p.depth);
     p.bytes = (uint64_t)p.cuts * terms * rows * p.pitch * sizeof(float);
     return p;
@@ -477,8 +478,8 @@ so_status forward(so_ctx *ctx, int type, Forward<T> f)
     }
     const Operand<T> g = {f.Wg, f.ldw, f.m, f.n}, u = {f.Wu, f.ldw, f.m, f.n};
     Operand<T> x = {f.X, f.ldx, f.B, f.n};
-    const bool align = g.direct() && u.direct() && !x.direct();
-    const Plan plan = plan_of(ctx, type, g.direct() && u.direct() && (align ? direct_there<T>(f.B) : x.direct()), 2 * (uint64_t)f.m, f.B, 1, f.n);
+    const bool align = g.direct() && u.direct() && !x.direct() && direct_there<T>(f.B);
+    const Plan plan = plan_of(ctx, type, g.direct() && u.direct() && (align || x.direct()), 2 * (uint64_t)f.m, f.B, 1, f.n);
     const size_t aligned = align ? bytes_of(type, f.n, f.B) : 0;
     if (align || plan.bytes)
         if (const so_status s = workspace(ctx, "so_gated", aligned + plan.bytes); s != SO_OK) return s;
@@ -514,10 +515,10 @@ so_status backward(so_ctx *ctx, int type, Slopes<T> s, uint32_t n, const Operand
     so_status status = SO_OK;
     Operand<T> d[2] = {{s.to[0].g, s.to[0].ld, B, m}, {s.to[0].u, s.to[0].ld, B, m}};
     const uint32_t parts = r.dWg && r.dWu ? 2u : 1u;
-    const bool to_workspace = products && !(s.to[0].g && s.to[0].u && d[0].direct() && d[1].direct()), align = weights && !x.direct();
+    const bool to_workspace = products && !(s.to[0].g && s.to[0].u && d[0].direct() && d[1].direct()), align = weights && !x.direct() && direct_there<T>(B);
     const bool direct = to_workspace ? direct_there<T>(B) : d[0].direct() && d[1].direct();
     const Plan dx = plan_of(ctx, type, direct && W[0].direct() && W[1].direct(), n, B, 2, m);
-    const Plan dw = plan_of(ctx, type, direct && (align ? direct_there<T>(B) : x.direct()), (uint64_t)parts * m, n, 1, B);
+    const Plan dw = plan_of(ctx, type, direct && (align || x.direct()), (uint64_t)parts * m, n, 1, B);
     char *pieces = nullptr;
     if (m && B) {
         const size_t each = to_workspace ? bytes_of(type, m, B) : 0, aligned = align ? bytes_of(type, n, B) : 0;

@@ -461,3 +461,31 @@ def test_what_is_not_a_number_stays_where_it_is_in_pieces(ctx, type_):
     H = fetch(outs[0], m, B, type_, 1)[0]
     assert np.array_equal(~np.isfinite(H), bad)
     a.free()
+
+
+@pytest.mark.parametrize("type_", TYPES)
+def test_millions_of_columns(ctx, type_):
+    """Rows so long that offsets inside a tile pass 31 bits.  All but 1000 columns of dH are zero, and adding a zero is exact: the weights' gradients are sums of 1000 terms."""
+    rng = np.random.default_rng(20)
+    m, n, B = 3, 2, 4_300_001
+    Wg, Wu, X = weights(rng, type_, m, n), weights(rng, type_, m, n), draw(rng, type_, n, B)
+    dH = np.zeros((m, B))
+    some = np.unique(np.append(rng.integers(0, B, 1000), [0, B - 1]))
+    dH[:, some] = draw(rng, type_, m, some.size)
+    a = Arrays(ctx, type_)
+    dWg, dWu, dX, dDh = (a.put(v)[0] for v in (Wg, Wu, X, dH))
+    H, G, S, gX, gWg, gWu = (a.put(np.zeros(s))[0] for s in ((m, B), (m, B), (m, B), (n, B), (m, n), (m, n)))
+    ctx.gated(dWg, dWu, m, n, dX, B, "silu", H, G, S, type=type_)
+    ctx.gated_grad(dWg, dWu, m, n, dX, B, "silu", G, S, dDh, gX, gWg, gWu, type=type_)
+    want = forward(Wg, Wu, X, "silu", type_)
+    check(fetch(H, m, B, type_)[0], want["H"])
+    vG, vS = fetch(G, m, B, type_)[0], fetch(S, m, B, type_)[0]
+    got = fetch(gX, n, B, type_)[0]
+    rest = np.ones(B, bool)
+    rest[some] = False
+    assert not got[:, rest].any()
+    back = backward(Wg, Wu, X[:, some], "silu", vG[:, some], vS[:, some], dH[:, some], type_)
+    check(got[:, some], back["dX"])
+    check(fetch(gWg, m, n, type_)[0], back["dWg"])
+    check(fetch(gWu, m, n, type_)[0], back["dWu"])
+    a.free()
