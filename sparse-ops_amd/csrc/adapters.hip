@@ -58,6 +58,19 @@ struct Which {
 struct Cut {
     uint32_t tiles, turns, parts, depth, rows, row_groups, padded;
     bool few;                // columns
+    uint32_t strip;          // tiles of an XCD, 0: as they come
+    uint32_t blocks(uint32_t each) const { return (strip ? 8u * strip : tiles) * each; }
+};
+
+// Which tile of columns a workgroup takes, and which of the tile's workgroups it is.  Workgroups go round-robin to the 8 XCDs; in strips neighbouring tiles are on the same one.
+struct Spot {
+    uint32_t tile, other;
+    __device__ __forceinline__ Spot(const Cut &c)
+    {
+        const uint32_t in = c.strip ? blockIdx.x / 8u : blockIdx.x, w = c.strip ? c.strip : c.tiles;
+        other = in / w;
+        tile = in % w + (c.strip ? blockIdx.x % 8u * c.strip : 0u);
+    }
 };
 
 template <class T> struct Call {
@@ -85,13 +98,15 @@ void adapters_in_kernel(Call<T> f)
 {
     extern __shared__ char stage[];
     fetch_arguments(f);
-    const uint32_t tile = blockIdx.x % f.cut.tiles, part = blockIdx.x / f.cut.tiles % f.cut.parts;
-    const uint64_t j0 = (uint64_t)tile * kCols;
+    const Spot spot(f.cut);
+    if (spot.tile >= f.cut.tiles) return;
+    const uint32_t part = spot.other % f.cut.parts;
+    const uint64_t j0 = (uint64_t)spot.tile * kCols;
     const size_t k0 = (size_t)part * f.cut.depth;
     const uint32_t depth = (uint32_t)min((size_t)f.cut.depth, f.n - k0), lane = threadIdx.x % 64u;
     const Which which(f.which, j0, j0, f.C, f.count, reinterpret_cast<uint64_t *>(stage));      // the ring comes later
     // a tile's second adapters first: few tiles have one, and they are not to begin when all others end
-    for (uint32_t i = f.cut.turns - 1u - blockIdx.x / f.cut.tiles / f.cut.parts; i < which.adapters(); i += f.cut.turns) {
+    for (uint32_t i = f.cut.turns - 1u - spot.other / f.cut.parts; i < which.adapters(); i += f.cut.turns) {
         const Which::Turn at = which.turn(i);
         for (uint32_t r0 = 0; r0 < f.rank; r0 += TILE::ROWS) {
             so_dense::Loop<T, TILE, false, true, false> loop;
@@ -319,7 +334,9 @@ void adapters_out_kernel(Call<T> f)
     typedef typename Shared::group_anywhere group_anywhere;
     extern __shared__ char lds[];
     fetch_arguments(f);
-    const uint32_t tile = blockIdx.x % f.cut.tiles, part = blockIdx.x / f.cut.tiles, lane = threadIdx.x % 64u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), l = lane % 16u, g = lane / 16u;
+    const Spot spot(f.cut);
+    if (spot.tile >= f.cut.tiles) return;
+    const uint32_t tile = spot.tile, part = spot.other, lane = threadIdx.x % 64u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u), l = lane % 16u, g = lane / 16u;
     // The last tile's columns end at C.  Those that the tile before it has too are written by both, the same bits, or, in place, where that would add twice, by that one alone.
     const uint64_t j0 = min((uint64_t)tile * kCols, (uint64_t)f.C - kCols), row_begin = (uint64_t)part * f.cut.rows, row_end = min(row_begin + f.cut.rows, (uint64_t)f.m);
     Shared at(f, lds);
@@ -481,7 +498,7 @@ Cut cut_of(const so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t C, uint
 {
     const uint32_t step = (rank <= 16 ? 256u : 128u) / (uint32_t)so_type_bytes(type);      // of the first launch
     const uint64_t cus = (uint64_t)ctx->compute_units;
-    Cut c;
+    Cut c = {};
     c.tiles = so_ceil_div(C, kCols);
     // a tile may have as many adapters as columns, and a workgroup without one ends at once; where a request ends and the next begins a tile has two
     c.turns = (uint32_t)std::min<uint64_t>(std::min(C, kCols), std::max<uint64_t>(2, cus / 2 / c.tiles));
@@ -501,13 +518,13 @@ Cut cut_of(const so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t C, uint
 
 // Of the workspace: A x, and behind it a group of B's where that has no more.
 size_t low_floats(const Cut &c, uint32_t C) { return (size_t)c.parts * C * c.padded; }
-size_t bytes_of(const Cut &c, uint32_t C) { return low_floats(c, C) * sizeof(float) + 32; }
+size_t bytes_of(const Cut &c, uint32_t C) { return low_floats(c, C) * sizeof(float) + 16; }
 
 // All of B, less than a group of 16 bytes, as one.
 template <class T>
 __global__ void adapters_small_kernel(const T *B, uint32_t entries, T *to)
 {
-    if (threadIdx.x < 16u) to[threadIdx.x] = threadIdx.x < entries ? B[threadIdx.x] : (T)0.0f;
+    if (threadIdx.x < so_elements<T>::V) to[threadIdx.x] = threadIdx.x < entries ? B[threadIdx.x] : (T)0.0f;
 }
 
 so_status workspace(so_ctx *ctx, const char *who, size_t bytes)
@@ -522,7 +539,7 @@ so_status launch_in(so_ctx *ctx, const Call<T> &f, bool direct)
 {
     const auto kernel = direct ? adapters_in_kernel<T, TILE, true> : adapters_in_kernel<T, TILE, false>;
     SO_HIP(so_allow_big_lds(ctx, (const void *)kernel));
-    kernel<<<f.cut.tiles * f.cut.parts * f.cut.turns, kThreads, TILE::lds, ctx->stream>>>(f);
+    kernel<<<f.cut.blocks(f.cut.parts * f.cut.turns), kThreads, TILE::lds, ctx->stream>>>(f);
     SO_LAUNCH_CHECK();
     return SO_OK;
 }
@@ -530,7 +547,11 @@ so_status launch_in(so_ctx *ctx, const Call<T> &f, bool direct)
 template <class T>
 so_status run(so_ctx *ctx, Call<T> f)
 {
-    const uint64_t in = (uint64_t)f.cut.tiles * f.cut.parts * f.cut.turns, out = (uint64_t)f.cut.tiles * f.cut.row_groups;
+    // Of many tiles each XCD gets a strip where rows do not all begin at a line of memory of 128 bytes: tiles side by side share their last lines.  4096 x 4096, rank 16
+    // bf16, 5003 columns: 52.6 us, as they come 58.6; 8192 in rows of 8200: 48.6 and 52.9.
+    const uint64_t bits = (uintptr_t)f.X | (uintptr_t)f.base | (uintptr_t)f.Y | (f.ldx | f.ldb | f.ldy) * sizeof(T);
+    f.cut.strip = bits % 128 && f.cut.tiles >= 64 ? so_ceil_div(f.cut.tiles, 8) : 0;      // fewer would not go to the XCDs evenly
+    const uint64_t most = (uint64_t)f.cut.tiles + 7, in = most * f.cut.parts * f.cut.turns, out = most * f.cut.row_groups;
     SO_REQUIRE(so_grid_fits(std::max(in, out), kThreads), "so_adapters: %u x %u is too large for one launch", f.m, f.C);
     if (const uint64_t entries = (uint64_t)f.m * f.rank * f.count; entries > 0 && (uint64_t)f.m * f.rank < 8 && entries < (uint64_t)so_elements<T>::V) {
         T *to = (T *)(f.low + low_floats(f.cut, f.C));
@@ -549,7 +570,7 @@ so_status run(so_ctx *ctx, Call<T> f)
     const uint32_t bytes = Tile64<T>::lds(f.cut.padded / 16) + (f.cut.few ? 16u * kResultPitch * 4u : 0u);
     const auto launch = [&](auto kernel) {
         const hipError_t e = bytes > 40 * 1024 ? so_allow_big_lds(ctx, (const void *)kernel) : hipSuccess;
-        if (e == hipSuccess) kernel<<<(uint32_t)out, kThreads, bytes, ctx->stream>>>(f);
+        if (e == hipSuccess) kernel<<<f.cut.blocks(f.cut.row_groups), kThreads, bytes, ctx->stream>>>(f);
         return e;
     };
     const auto with = [&](auto rc) {
