@@ -225,9 +225,10 @@ so_status so_matmul(so_ctx *ctx, const so_ellpack *E, const float *dX, uint32_t 
  * connected layer -- the reference's documented way to get its allocation-free run(), README.md:146).
  * No counterpart in the reference. */
 so_status so_matmul_reserve(so_ctx *ctx, const so_ellpack *E, uint32_t C);
-/* Which kernel the context's last so_matmul, so_mxfp4_matmul, so_conv2d, so_conv2d_pair or encode launched, for tests and tuning.  so_matmul: "merged", "quad", "planes", "narrow",
+/* Which kernel the context's last so_matmul, so_mxfp4_matmul, so_gated, so_gated_grad, so_conv2d, so_conv2d_pair or encode launched, for tests and tuning.  so_matmul: "merged", "quad", "planes", "narrow",
  * "slabs" (the quad-union copy with X in LDS a part at a time) and "vector" (on handles with the RBM layout), "tiled", "columns", "shared", "row"; so_conv2d: "columns",
- * "merged-window", "window", "gather"; so_mxfp4_matmul: "mx-" and its tile of the output; so_conv2d_pair: "columns-pair", "window-pair", or so_conv2d's for its second convolution where it makes two launches; encode:
+ * "merged-window", "window", "gather"; so_mxfp4_matmul: "mx-" and its tile of the output; so_gated: "gated-token" for one column, else "gated-" and the
+ * tile of both projections, with "-any" where operands' rows do not all begin at multiples of 16 bytes; so_gated_grad: its last product's, likewise; so_conv2d_pair: "columns-pair", "window-pair", or so_conv2d's for its second convolution where it makes two launches; encode:
  * "encode-once", "encode-twice", "encode-spared" (twice, since an earlier one-read encode gave up waiting); "" before the first.  A static string.  No counterpart in
  * the reference. */
 const char *so_last_kernel(const so_ctx *ctx);
