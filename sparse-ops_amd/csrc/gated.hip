@@ -121,11 +121,11 @@ __global__ __launch_bounds__(kThreads)
 void gated_join_kernel(Forward<T> f, uint32_t groups)
 {
     constexpr int V = so_elements<T>::V;
-    const uint64_t at = (uint64_t)blockIdx.x * kThreads + threadIdx.x, row = at / groups, col = at % groups * V;
+    const uint32_t at = blockIdx.x * kThreads + threadIdx.x, row = at / groups, col = at % groups * V;      // a launch has fewer than 2^32 threads
     if (row >= f.m) return;
     float g[V], u[V];
     join(f.pieces, f.pieces.cuts, 2u * (uint64_t)f.m, row, col, g);
-    join(f.pieces, f.pieces.cuts, 2u * (uint64_t)f.m, row + f.m, col, u);
+    join(f.pieces, f.pieces.cuts, 2u * (uint64_t)f.m, (uint64_t)row + f.m, col, u);
     finish(f, row, col, g, u);
 }
 
@@ -213,9 +213,32 @@ void gated_token_kernel(Forward<T> f)
     f.H[row * f.ldh] = (T)mine[0];
 }
 
+// A matrix with its rows at multiples of 16 bytes: 1003 x 331 fp16 in 2.2 us, where a product that takes it as it lies, through registers, takes half as long again.
+template <class T> struct Rows {
+    const T *X;
+    size_t ldx;
+    uint32_t rows, cols, groups, blocks;     // groups of a row; workgroups, 0: nothing to do
+    T *Y;
+    size_t ldy;
+    __device__ __forceinline__ void copy(uint32_t at) const
+    {
+        constexpr int V = so_elements<T>::V;
+        const uint32_t row = at / groups, col = at % groups * V;
+        if (row >= rows) return;
+        const auto v = so_group_load(X + row * ldx + col, min((uint32_t)V, cols - col));
+        *reinterpret_cast<typename so_elements<T>::vec *>(Y + row * ldy + col) = v;      // zeros behind the row's end
+    }
+};
+template <class T>
+__global__ __launch_bounds__(kThreads)
+void align_rows_kernel(Rows<T> x)
+{
+    x.copy(blockIdx.x * kThreads + threadIdx.x);
+}
+
 // The gradients of the two sums, to either or both of two places (the caller's and the products').  A thread takes a group of 16 bytes of a row; groups of whole rows follow one another.  It reads what it
 // needs before it writes, so that the caller's may be the inputs.  In 16 bits both are rounded to the type, since the products take operands of it: half a step of each term, where fp32 gradients as two numbers each
-// would double the products.  Bound by memory: 8192 x 4096 bf16, 335 MB, 54 us or 6.2 TB/s.
+// would double the products.  The first workgroups align X for the products, where that is to be done.  Bound by memory: 8192 x 4096 bf16, 335 MB, 54 us or 6.2 TB/s.
 template <class T> struct Place {
     T *g, *u;
     size_t ld;
@@ -229,12 +252,13 @@ template <class T> struct Slopes {
 };
 template <class T>
 __global__ __launch_bounds__(kThreads)
-void gated_slopes_kernel(Slopes<T> s)
+void gated_slopes_kernel(Slopes<T> s, Rows<T> x)
 {
     constexpr int V = so_elements<T>::V;
-    const uint64_t at = (uint64_t)blockIdx.x * kThreads + threadIdx.x, row = at / s.groups, col = at % s.groups * V;
+    if (blockIdx.x < x.blocks) return x.copy(blockIdx.x * kThreads + threadIdx.x);
+    const uint32_t at = (blockIdx.x - x.blocks) * kThreads + threadIdx.x, row = at / s.groups, col = at % s.groups * V;
     if (row >= s.m) return;
-    const uint32_t left = (uint32_t)min((uint64_t)V, s.B - col);
+    const uint32_t left = min((uint32_t)V, s.B - col);
     const auto gv = so_group_load(s.G + row * s.ldg + col, left), uv = so_group_load(s.U + row * s.ldg + col, left), hv = so_group_load(s.dH + row * s.ldh + col, left);
     float g[V], u[V];
     so_gate::with_slope<sizeof(T) == 2>(s.act, [&](auto both) {
@@ -250,18 +274,6 @@ void gated_slopes_kernel(Slopes<T> s)
         if (s.to[i].g) so_group_store(s.to[i].g + row * s.to[i].ld + col, left, g);
         if (s.to[i].u) so_group_store(s.to[i].u + row * s.to[i].ld + col, left, u);
     }
-}
-
-// A matrix with its rows at multiples of 16 bytes: 1003 x 331 fp16 in 2.2 us, where a product that takes it as it lies, through registers, takes half as long again.
-template <class T>
-__global__ __launch_bounds__(kThreads)
-void align_rows_kernel(const T *X, size_t ldx, uint32_t rows, uint32_t cols, uint32_t groups, T *Y, size_t ldy)
-{
-    constexpr int V = so_elements<T>::V;
-    const uint64_t at = (uint64_t)blockIdx.x * kThreads + threadIdx.x, row = at / groups, col = at % groups * V;
-    if (row >= rows) return;
-    const auto v = so_group_load(X + row * ldx + col, (uint32_t)min((uint64_t)V, cols - col));
-    *reinterpret_cast<typename so_elements<T>::vec *>(Y + row * ldy + col) = v;      // zeros behind the row's end
 }
 
 // Y = A[0] B[0] + A[1] B[1], or either's rows one after the other where the result has two parts (Y2 is not null).  The three gradients of 8192 x 4096 x
@@ -308,12 +320,12 @@ __global__ __launch_bounds__(kThreads)
 void product_join_kernel(Product<T> p, uint32_t groups, uint32_t parts)
 {
     constexpr int V = so_elements<T>::V;
-    const uint64_t at = (uint64_t)blockIdx.x * kThreads + threadIdx.x, row = at / groups, col = at % groups * V;
+    const uint32_t at = blockIdx.x * kThreads + threadIdx.x, row = at / groups, col = at % groups * V;
     if (row >= (uint64_t)parts * p.rows) return;
     float v[V];
     join(p.pieces, p.terms * p.pieces.cuts, (uint64_t)parts * p.rows, row, col, v);
     T *Y = row >= p.rows ? p.Y2 + (row - p.rows) * p.ldy : p.Y + row * p.ldy;
-    so_group_store(Y + col, (uint32_t)min((uint64_t)V, p.cols - col), v);
+    so_group_store(Y + col, min((uint32_t)V, p.cols - col), v);
 }
 
 // Tiles, by rows and columns of the result (of both projections together in the forward pass).
@@ -444,27 +456,25 @@ so_status product(so_ctx *ctx, const Product<T> &p, const Plan &plan)
     return SO_OK;
 }
 
-// m in the workspace at `to`, aligned.
+// *m as what it is in the workspace at `to`, aligned; -> what makes it that.
 template <class T>
-so_status align_rows(so_ctx *ctx, const char *who, Operand<T> *m, uint32_t rows, uint32_t cols, void *to)
+Rows<T> align_rows(Operand<T> *m, uint32_t rows, uint32_t cols, void *to)
 {
     const uint32_t groups = so_ceil_div(cols, so_elements<T>::V);
-    const uint64_t blocks = blocks_of<T>(rows, groups);
-    SO_REQUIRE(so_grid_fits(blocks, kThreads), "%s: %u x %u is too large for one launch", who, rows, cols);
-    align_rows_kernel<T><<<(uint32_t)blocks, kThreads, 0, ctx->stream>>>(m->p, m->ld, rows, cols, groups, (T *)to, stride_of(cols));
-    SO_LAUNCH_CHECK();
+    const Rows<T> r = {m->p, m->ld, rows, cols, groups, (uint32_t)blocks_of<T>(rows, groups), (T *)to, stride_of(cols)};
     m->p = (const T *)to;
     m->ld = stride_of(cols);
-    return SO_OK;
+    return r;
 }
+template <class T> bool align_fits(uint32_t rows, uint32_t cols) { return so_grid_fits(blocks_of<T>(rows, so_ceil_div(cols, so_elements<T>::V)), kThreads); }
 
 template <class T>
-so_status slopes(so_ctx *ctx, Slopes<T> s)
+so_status slopes(so_ctx *ctx, Slopes<T> s, const Rows<T> &x)
 {
     s.groups = so_ceil_div(s.B, so_elements<T>::V);
     const uint64_t blocks = blocks_of<T>(s.m, s.groups);
-    SO_REQUIRE(so_grid_fits(blocks, kThreads), "so_gated_grad: %u x %u is too large for one launch", s.m, s.B);
-    gated_slopes_kernel<T><<<(uint32_t)blocks, kThreads, 0, ctx->stream>>>(s);
+    SO_REQUIRE(so_grid_fits(blocks + x.blocks, kThreads), "so_gated_grad: %u x %u is too large for one launch", s.m, s.B);
+    gated_slopes_kernel<T><<<(uint32_t)blocks + x.blocks, kThreads, 0, ctx->stream>>>(s, x);
     SO_LAUNCH_CHECK();
     return SO_OK;
 }
@@ -490,7 +500,10 @@ so_status forward(so_ctx *ctx, int type, Forward<T> f)
     if (align || plan.bytes)
         if (const so_status s = workspace(ctx, "so_gated", aligned + plan.bytes); s != SO_OK) return s;
     if (align) {
-        if (const so_status s = align_rows(ctx, "so_gated", &x, f.n, f.B, ctx->mm_part->p); s != SO_OK) return s;
+        SO_REQUIRE(align_fits<T>(f.n, f.B), "so_gated: %u x %u is too large for one launch", f.n, f.B);
+        const Rows<T> r = align_rows(&x, f.n, f.B, ctx->mm_part->p);
+        align_rows_kernel<T><<<r.blocks, kThreads, 0, ctx->stream>>>(r);
+        SO_LAUNCH_CHECK();
         f.X = x.p;
         f.ldx = x.ld;
     }
@@ -526,6 +539,7 @@ so_status backward(so_ctx *ctx, int type, Slopes<T> s, uint32_t n, const Operand
     const Plan dx = plan_of(ctx, type, direct && W[0].direct() && W[1].direct(), n, B, 2, m);
     const Plan dw = plan_of(ctx, type, direct && (align || x.direct()), (uint64_t)parts * m, n, 1, B);
     char *pieces = nullptr;
+    Rows<T> rows = {};
     if (m && B) {
         const size_t each = to_workspace ? bytes_of(type, m, B) : 0, aligned = align ? bytes_of(type, n, B) : 0;
         const size_t bytes = 2 * each + aligned + std::max(r.dX ? dx.bytes : 0, weights ? dw.bytes : 0);
@@ -536,10 +550,11 @@ so_status backward(so_ctx *ctx, int type, Slopes<T> s, uint32_t n, const Operand
                 s.to[1] = {(T *)at, (T *)(at + each), stride_of(B)};
                 for (int i = 0; i < 2; ++i) d[i] = {(const T *)(at + i * each), stride_of(B), B, m};
             }
-            if (align && (status = align_rows(ctx, "so_gated_grad", &x, n, B, at + 2 * each)) != SO_OK) return status;
+            SO_REQUIRE(!align || align_fits<T>(n, B), "so_gated_grad: %u x %u is too large for one launch", n, B);
+            if (align) rows = align_rows(&x, n, B, at + 2 * each);
             pieces = at + 2 * each + aligned;
         }
-        if ((status = slopes(ctx, s)) != SO_OK) return status;
+        if ((status = slopes(ctx, s, rows)) != SO_OK) return status;
     }
     if (r.dX && B) status = product<T, true, true>(ctx, {{W[0], W[1]}, {d[0], d[1]}, (T *)r.dX, nullptr, r.ldx, n, B, 2, dx.pieces(pieces)}, dx);
     if (status != SO_OK || !weights || !m) return status;

@@ -274,7 +274,7 @@ def test_a_workspace_that_must_grow_is_refused_while_recording():
 # a last tile of columns of every kind, ranks that end inside a run of products and a group, adapters and rows to the end of their arrays
 @pytest.mark.parametrize("type_", TYPES)
 @pytest.mark.parametrize("m,n,C,count,rank", [(70, 40, 256, 3, 1), (33, 72, 257, 4, 3), (100, 130, 320, 5, 10), (17, 64, 383, 2, 33), (65, 33, 449, 3, 100), (40, 200, 300, 6, 4), (130, 24, 511, 2, 256),
-                                              (3, 5, 290, 2, 7), (1, 1, 260, 1, 1)])
+                                              (3, 5, 290, 2, 7), (1, 1, 260, 1, 1), (40, 48, 4161, 5, 6), (20, 33, 4500, 3, 17), (70, 24, 8192, 4, 16)])
 def test_many_columns(ctx, m, n, C, count, rank, type_):
     rng = np.random.default_rng(C + rank)
     A, B, scale, X, base = problem(rng, m, n, C, count, rank, type_)
