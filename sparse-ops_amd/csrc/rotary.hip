@@ -165,7 +165,7 @@ void rotary_kernel(Shape s, const T *X, size_t ldx, const float *gain_q, const f
 }
 
 // With norms: h = turn^-1(dY); dX = rstd (gain h - n mean(gain h n)), n = x rstd, and of every workgroup its share of the gains' gradients sum(h n), [tiles * groups][D], which the kernel below adds
-// up in a fixed order.  24 + 8 heads of 96 x 4099 fp16, 75 MB: 28 us and 4.5 for the shares; with the next head in registers ahead, which leaves one workgroup a compute unit, 47, and with h
+// up in a fixed order.  24 + 8 heads of 96 x 4099 fp16, 75 MB: 25.5 us and 4.5 for the shares; with the next head in registers ahead, which leaves one workgroup a compute unit, 47, and with h
 // kept instead of turned back again after the sum, 38.
 template <class T, int LC, int PPT, int NT>
 __global__ __launch_bounds__(NT, PPT == 1 ? 4 : 1)
@@ -294,7 +294,7 @@ Shape shape_of(const so_ctx *ctx, const Cut &c, int type, uint32_t heads_q, uint
     Shape s = {heads_q, heads_q + heads_k, D, B, rot, layout == SO_ROTARY_PAIRS, 0, 1, 0, 0, 0};
     s.tiles = so_ceil_div(B, c.lanes * (16u / (uint32_t)so_type_bytes(type)));
     // The turns are worked out once for all heads of a workgroup, and the next head is on its way while one is turned: as many heads a workgroup as all there are, dealt to two workgroups of 512
-    // threads on every compute unit.  32 + 8 heads of 128 x 8192 bf16, 10 a workgroup: 38.6 us; 5: 43; 2: 45; 20: 45.  The gradient of 24 + 8 heads of 96 x 4099 fp16, 5 a workgroup: 33 us (now 30.6); 4: 37;
+    // threads on every compute unit.  32 + 8 heads of 128 x 8192 bf16, 10 a workgroup: 38.6 us; 5: 43; 2: 45; 20: 45.  The gradient of 24 + 8 heads of 96 x 4099 fp16, 5 a workgroup: 33 us (27.7 with strips); 4: 37;
     // 1: 43; 10: 39.
     const uint64_t room = (uint64_t)ctx->compute_units * (1024u / c.threads);
     s.per = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(((uint64_t)s.tiles * s.heads + room - 1u) / room, s.heads));
