@@ -200,7 +200,7 @@ struct Tile64 {
 #pragma unroll
             for (int e = 0; e < V / 4; ++e) a.s[i][e] = part + i < f.cut.parts ? *reinterpret_cast<const f32x4 *>(from + (part + i) * step + e * 4) : f32x4{};
     }
-    template <int N>
+    template <int HOLD, int N>
     __device__ __forceinline__ void gather(uint64_t j0, const Sums<N> &first) const
     {
         const uint32_t lane = threadIdx.x % 64u, wave = threadIdx.x / 64u, l = lane % 16u, g = lane / 16u, col = column(wave, l);
@@ -246,20 +246,36 @@ struct Tile64 {
             }
             operand[(wave * runs + run) * 64u + lane] = r;
         };
-        float v[V];
         if constexpr (SHIFTED) {
-            float largest = 0.0f;
-            for (uint32_t run = 0; run < runs; ++run) {
+            // the first HOLD runs stay in registers between the two passes
+            float held[HOLD][V], v[V], largest = 0.0f;
+#pragma unroll
+            for (uint32_t run = 0; run < HOLD; ++run)
+                if (run < runs) {
+                    low(run, held[run]);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) largest = fmaxf(largest, fabsf(held[run][e]));
+                }
+            for (uint32_t run = HOLD; run < runs; ++run) {
                 low(run, v);
 #pragma unroll
                 for (int e = 0; e < V; ++e) largest = fmaxf(largest, fabsf(v[e]));
             }
             choose(largest);
             if (g == 0) factor[col] = out;
-        }
-        for (uint32_t run = 0; run < runs; ++run) {
-            if (!SHIFTED || runs > 1u) low(run, v);
-            put(run, v);
+#pragma unroll
+            for (uint32_t run = 0; run < HOLD; ++run)
+                if (run < runs) put(run, held[run]);
+            for (uint32_t run = HOLD; run < runs; ++run) {
+                low(run, v);
+                put(run, v);
+            }
+        } else {
+            float v[V];
+            for (uint32_t run = 0; run < runs; ++run) {
+                low(run, v);
+                put(run, v);
+            }
         }
     }
     // A run of 16 entries of rank of a row of adapter a's B, asked for without a branch, and made what it is once it has come.  EVEN: the rank is a multiple of a group, so that groups are whole.  Else they reach into
@@ -344,7 +360,7 @@ void adapters_out_kernel(Call<T> f)
     typename Shared::template Sums<4> sums;
     at.ask(j0, 0, 0, sums);
     at.list(j0, f.base == f.Y ? (uint64_t)tile * kCols : j0);
-    at.gather(j0, sums);
+    at.template gather<RC>(j0, sums);
     __syncthreads();
     u32x4 whole[4];
     if constexpr (RC == 1) at.take(whole);
@@ -440,7 +456,7 @@ void adapters_out_few_kernel(Call<T> f)
             load_b(wave + i * 4u, row, 0, b[i]);
     };
     if (at.count) load_first(row_begin + l);
-    at.gather(j0, sums);
+    at.template gather<RC>(j0, sums);
     __syncthreads();
     u32x4 whole[4];
     if constexpr (RC == 1) at.take(whole);
@@ -502,10 +518,12 @@ Cut cut_of(const so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t C, uint
     Cut c = {};
     c.tiles = so_ceil_div(C, kCols);
     // a tile may have as many adapters as columns, and a workgroup without one ends at once; where a request ends and the next begins a tile has two
-    c.turns = (uint32_t)std::min<uint64_t>(std::min(C, kCols), std::max<uint64_t>(2, cus / 2 / c.tiles));
+    c.turns = (uint32_t)std::min<uint64_t>(std::min({C, kCols, std::max(count, 1u)}), std::max<uint64_t>(2, cus / 2 / c.tiles));
     c.padded = so_ceil_div(rank, kPad) * kPad;
+    // Parts of the features: of a rank beyond 16 the second launch takes 8 at a time of every 16 entries, one wait each (16 columns of 4096 x 4096, rank 64 fp16: 8 parts 21.3 us, 16 26.4; one column, rank 16 fp16: 12.2 and
+    // 12.0).
     const uint64_t most = std::max<uint64_t>(1, so_ceil_div(n, 2 * step)), want = std::max<uint64_t>(1, 2 * cus / ((uint64_t)c.tiles * c.turns));
-    c.parts = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(most, std::max<uint64_t>(want, c.tiles < cus ? 4 : 1)), 16);
+    c.parts = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(most, std::max<uint64_t>(want, c.tiles < cus ? 4 : 1)), rank <= 16 ? 16 : 8);
     c.depth = so_ceil_div(so_ceil_div(n, c.parts), step) * step;
     c.parts = so_ceil_div(n, c.depth);
     // With few columns the second launch deals adapters to waves, 16 rows at a time, else rows (us of the second launch, 4096 rows, rank 16 fp16, by rows / by adapters, of 1, 8 and 64 requests: 128 columns 5.3 / 6.6,
