@@ -51,7 +51,7 @@ struct Side {
 
     // A row's groups are exchanged by an exclusive or, so that lanes that read at the same place of neighbouring rows meet in different banks: along, 16 rows of one group (8 of rows of 128 bytes, pairs of rows of 64); across, in 16 bits
     // 16 rows (4 neighbours, of 4 eights) of 32 bytes, in 32 bits 4 rows (each fourth) of 64 bytes.
-    static __device__ __forceinline__ uint32_t swap(uint32_t row)
+    static __host__ __device__ __forceinline__ uint32_t swap(uint32_t row)
     {
         if constexpr (!ACROSS) return PER == 16 ? row & 15u : PER == 8 ? row & 7u : row >> 1 & 3u;
         else if constexpr (E == 2) return PER >= 16 ? ((row & 3u) | (row >> 1 & 4u)) << 1 : PER == 8 ? ((row >> 1 & 1u) | (row >> 2 & 2u)) << 1 : PER == 4 ? (row >> 3 & 1u) << 1 : 0u;
@@ -76,11 +76,12 @@ struct Side {
         }
     }
     __device__ __forceinline__ uint32_t steps() const { return (depth + BK - 1u) / BK; }
-    // Whether a step is all there.  Groups that reach beyond `own` hold what lies between the rows or in the next one, entries of no use that nothing depends on; behind the last row there is no next.
-    __device__ __forceinline__ bool whole(uint32_t step) const
+    // Whether a step is all there, so that its groups can be read whole.  Across, the group at a row's end holds what lies behind it, entries of no use that nothing depends on: the rows below have to be as many as it
+    // reaches into, one where a row's stride is a group at least, seven of a single 16-bit column without gaps.
+    __host__ __device__ __forceinline__ bool whole(uint32_t step) const
     {
         const uint64_t end = (uint64_t)(step + 1u) * BK;
-        return end <= depth && (!ACROSS || own >= (uint32_t)LEN || own % V == 0 || end < depth);
+        return end <= depth && (!ACROSS || own >= (uint32_t)LEN || own % V == 0 || (depth - end) * ld >= V - own % V);
     }
     // Request `piece` of this wave for such a step, or all of them, straight to LDS at `to`.  Whole rows beyond `own` are kept off by the buffer's size.
     __device__ __forceinline__ void bring(uint32_t step, uint32_t to, int piece) const
@@ -106,16 +107,20 @@ struct Side {
         return __builtin_bit_cast(u32x4, so_group_load(at + (ACROSS ? (size_t)k * ld + i : (size_t)i * ld + k), (uint32_t)min(end - along, (uint64_t)V)));
     }
     static __device__ __forceinline__ uint32_t group_of(uint32_t a) { return (a * WAVES + threadIdx.x / 64u) * 64u + threadIdx.x % 64u; }
-    // The groups of a step that is whole, at any address.  Rows, or groups of a row, that do not exist are replaced by others that do, for nothing.
+    // Where a step begins, from `at` on, and where behind that group q of one that is whole is read.  Rows, or groups of a row, that do not exist are replaced by others that do, for nothing.
+    __host__ __device__ __forceinline__ size_t begin(uint32_t step) const { return ACROSS ? (size_t)step * BK * ld : (size_t)step * BK; }
+    __host__ __device__ __forceinline__ size_t place(uint32_t q) const
+    {
+        const uint32_t row = q / PER, group = q % PER ^ swap(row);
+        const uint32_t i = ACROSS ? (group * V < own ? group * V : 0u) : (row < own ? row : own - 1u), k = ACROSS ? row : group * V;
+        return ACROSS ? (size_t)k * ld + i : (size_t)i * ld + k;
+    }
+    // The groups of a step that is whole, at any address.
     __device__ __forceinline__ void take(uint32_t step, u32x4 (&r)[ASKS]) const
     {
+        const T *from = at + begin(step);
 #pragma unroll
-        for (int a = 0; a < ASKS; ++a) {
-            const uint32_t q = group_of(a), row = q / PER, group = q % PER ^ swap(row);
-            const uint32_t i = ACROSS ? (group * V < own ? group * V : 0u) : min(row, own - 1u), k = ACROSS ? row : group * V;
-            const T *p = at + (ACROSS ? (size_t)step * BK * ld : (size_t)step * BK) + (ACROSS ? (size_t)k * ld + i : (size_t)i * ld + k);
-            r[a] = __builtin_bit_cast(u32x4, *reinterpret_cast<const typename so_elements<T>::vec *>(p));
-        }
+        for (int a = 0; a < ASKS; ++a) r[a] = __builtin_bit_cast(u32x4, *reinterpret_cast<const typename so_elements<T>::vec *>(from + place(group_of(a))));
     }
     static __device__ __forceinline__ void put(char *to, const u32x4 (&r)[ASKS])
     {
@@ -225,8 +230,13 @@ struct Loop {
         for (int h = 0; h < PARTS; ++h) a[h].settle(step, slot + h * SideA::BYTES);
         b.settle(step, slot + B0);
     }
-    // Steps, and how many of them are whole: all, or all but the last.
-    __device__ __forceinline__ uint32_t whole_of(uint32_t steps) const { return steps && !(a[0].whole(steps - 1u) && b.whole(steps - 1u)) ? steps - 1u : steps; }
+    // How many steps are whole: all or all but the last of aligned operands, whose strides are a group at least; else all but the last two at least, since a step has more rows than a group has entries.
+    __device__ __forceinline__ uint32_t whole_of(uint32_t steps) const
+    {
+        uint32_t whole = steps;
+        for (int i = 0; i < 2; ++i) whole -= whole && !(a[0].whole(whole - 1u) && b.whole(whole - 1u)) ? 1u : 0u;
+        return whole;
+    }
 
     // acc += the product of rows from i0 on (of both operands, with HALVES) and columns from j0 on, both operands aligned.  All steps go straight to LDS, but for a last one that is not whole.
     // A run (64 bytes of k) is multiplied from registers while the next one's operands are read: those of the rows into a second set, those of the columns into the places that have been multiplied
@@ -368,10 +378,10 @@ struct Loop {
                     compute(s + i);
                 }
         }
-        if (whole < steps) {
-            settle(whole, stage + whole % 2u * STAGE);
+        for (uint32_t rest = whole; rest < steps; ++rest) {
+            settle(rest, stage + rest % 2u * STAGE);
             __syncthreads();
-            compute(whole);
+            compute(rest);
         }
     }
     template <bool DIRECT>
