@@ -58,7 +58,7 @@ struct Seat {
     uint32_t at, tile, c0, left, first, last, wide; // its number; columns; heads first .. last - 1
     bool query;
     uint2 row[PPT];                                 // inside a head
-    bool has[PPT], two[PPT];
+    bool has[PPT], two[PPT], turned[PPT];
     __device__ __forceinline__ Seat(const Shape &s, size_t ld)
     {
         // Workgroups go round-robin to the 8 XCDs.  With strips neighbouring tiles, which share the lines of memory that rows' tiles end in, are on the same one: the gradient of 24 + 8 heads of 96 x 4099 fp16 with neighbours on
@@ -78,6 +78,7 @@ struct Seat {
             row[k] = rows_of(s, threadIdx.x / LC + k * RL);
             has[k] = left && row[k].x < s.D;
             two[k] = left && row[k].y < s.D;
+            turned[k] = threadIdx.x / LC + k * RL < s.rot / 2u;
         }
     }
     __device__ __forceinline__ void turns(const Shape &s, const int32_t *pos, const float *freq, float amplitude, float2 (&t)[PPT][V]) const
@@ -88,10 +89,9 @@ struct Seat {
 #pragma unroll
         for (int k = 0; k < PPT; ++k) {
             const uint32_t i = threadIdx.x / LC + k * RL;
-            const bool turned = i < s.rot / 2u;
-            const double f = turned ? (double)freq[i] * kTurnsPerRadian : 0.0;
+            const double f = turned[k] ? (double)freq[i] * kTurnsPerRadian : 0.0;
 #pragma unroll
-            for (int e = 0; e < V; ++e) t[k][e] = turned ? turn_of<sizeof(T) == 2>(p[e], f, amplitude) : make_float2(1.0f, 0.0f);
+            for (int e = 0; e < V; ++e) t[k][e] = turned[k] ? turn_of<sizeof(T) == 2>(p[e], f, amplitude) : make_float2(1.0f, 0.0f);
         }
     }
     __device__ __forceinline__ void load(const Shape &s, uint32_t head, const T *X, size_t ld, group (&x)[PPT][2]) const
@@ -153,8 +153,8 @@ void rotary_kernel(Shape s, const T *X, size_t ldx, const float *gain_q, const f
             for (int e = 0; e < V; ++e) {
                 const float u = NORM ? (float)x[k][0][e] * r[e] * g[k].x : (float)x[k][0][e], v = NORM ? (float)x[k][1][e] * r[e] * g[k].y : (float)x[k][1][e];
                 const float c = turn[k][e].x, d = direction * turn[k][e].y;
-                a[e] = fmaf(u, c, -(v * d));
-                b[e] = fmaf(v, c, u * d);
+                a[e] = at.turned[k] ? fmaf(u, c, -(v * d)) : u;      // not a turn by nothing, which would make NaN of what lies beside an infinity
+                b[e] = at.turned[k] ? fmaf(v, c, u * d) : v;
             }
             if (at.has[k]) so_group_store(Y + (size_t)(head * s.D + at.row[k].x) * ldy + at.c0, at.left, a);
             if (at.two[k]) so_group_store(Y + (size_t)(head * s.D + at.row[k].y) * ldy + at.c0, at.left, b);
@@ -209,6 +209,7 @@ void rotary_grad_kernel(Shape s, const T *X, size_t ldx, const T *dY, size_t ldd
         // the gradients of the products, turned back
         const auto back = [&](int k, int e) {
             const float u = (float)d[k][0][e], v = (float)d[k][1][e];
+            if (!at.turned[k]) return make_float2(u, v);
             return make_float2(fmaf(u, turn[k][e].x, v * turn[k][e].y), fmaf(v, turn[k][e].x, -(u * turn[k][e].y)));
         };
 #pragma unroll
