@@ -11,16 +11,32 @@ static inline bool known(int act) { return act >= SO_ACT_NONE && act <= SO_ACT_G
 
 constexpr float kLog2e = 1.44269504f, kRootHalf = 0.70710678f, kRootTwoOverPi = 0.79788456f, kCubic = 0.044715f, kNormal = 0.39894228f;      // 1 / sqrt(2), sqrt(2 / pi), 1 / sqrt(2 pi)
 
-// 1 / (1 + exp(-v)) by the exponential and the reciprocal of the vector unit, a step each.  Rounding v log2 e costs |v| steps of the exponential, which matter only where that is small
+// 1 / (1 + exp(-v)).  For results of 16 bits by the exponential and the reciprocal of the vector unit, a step each.  Rounding v log2 e costs |v| steps of the exponential, which matter only where that is small
 // beside 1 (v > 0) or the result is as small as it (v < 0): v times it is within 2^-23 for all v.  expf and a division, 25 instructions more, made the forward pass of 8192 x 4096 x 4096 bf16
-// 45 us slower.
-__device__ __forceinline__ float logistic(float v) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * v)); }
+// 45 us slower.  For fp32, whose results are to be right to their own last bits, those, and of a negative v the exponential that cannot overflow.
+template <bool HALF>
+__device__ __forceinline__ float logistic(float v)
+{
+    if constexpr (HALF) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * v));
+    const float e = expf(-fabsf(v));
+    return (v < 0.0f ? e : 1.0f) / (1.0f + e);
+}
 
 // That and what is left to 1, both to a few steps of their own.
 struct Share { float of, rest; };
+template <bool HALF>
 __device__ __forceinline__ Share shares(float v)
 {
-    const float e = __builtin_amdgcn_exp2f(-kLog2e * fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e), s = e * r;
+    float r, s;
+    if constexpr (HALF) {
+        const float e = __builtin_amdgcn_exp2f(-kLog2e * fabsf(v));
+        r = __builtin_amdgcn_rcpf(1.0f + e);
+        s = e * r;
+    } else {
+        const float e = expf(-fabsf(v));
+        r = 1.0f / (1.0f + e);
+        s = e / (1.0f + e);
+    }
     return v >= 0.0f ? Share{r, s} : Share{s, r};
 }
 
@@ -37,17 +53,26 @@ __device__ __forceinline__ float normal(float v)
     return v > 0.0f ? 1.0f - tail : tail;
 }
 
+// Its density.  In fp32 what rounding v v leaves, v^2 / 2 steps of the exponential, is put back.
+template <bool HALF>
+__device__ __forceinline__ float bell(float v)
+{
+    if constexpr (HALF) return kNormal * __builtin_amdgcn_exp2f(-0.5f * kLog2e * v * v);
+    const float square = v * v, e = expf(-0.5f * square);
+    return e == 0.0f ? 0.0f : kNormal * fmaf(-0.5f * fmaf(v, v, -square), e, e);
+}
+
 // f(function of v) for the activation, the same for a whole launch, so that the branch on it costs a few scalar instructions.
 template <bool HALF, class F>
 __device__ __forceinline__ void with(int act, F &&f)
 {
     switch (act) {
     case SO_ACT_RELU: return f([](float v) { return v <= 0.0f ? 0.0f : v; });
-    case SO_ACT_SIGMOID: return f([](float v) { return logistic(v); });
+    case SO_ACT_SIGMOID: return f([](float v) { return logistic<HALF>(v); });
     case SO_ACT_TANH: return f([](float v) { return tanhf(v); });
-    case SO_ACT_SILU: return f([](float v) { return v * logistic(v); });
+    case SO_ACT_SILU: return f([](float v) { return v * logistic<HALF>(v); });
     case SO_ACT_GELU: return f([](float v) { return v * normal<HALF>(v); });
-    case SO_ACT_GELU_TANH: return f([](float v) { return v * logistic(2.0f * tanh_argument(v)); });
+    case SO_ACT_GELU_TANH: return f([](float v) { return v * logistic<HALF>(2.0f * tanh_argument(v)); });
     default: return f([](float v) { return v; });
     }
 }
@@ -70,23 +95,23 @@ __device__ __forceinline__ void with_slope(int act, F &&f)
     switch (act) {
     case SO_ACT_RELU: return f([](float v) { return Both{v <= 0.0f ? 0.0f : v, v <= 0.0f ? 0.0f : v > 0.0f ? 1.0f : v}; });
     case SO_ACT_SIGMOID: return f([](float v) {
-        const Share p = shares(v);
+        const Share p = shares<HALF>(v);
         return Both{p.of, p.of * p.rest};
     });
     case SO_ACT_TANH: return f([](float v) {
-        const Share p = shares(2.0f * v);
+        const Share p = shares<HALF>(2.0f * v);
         return Both{tanhf(v), 4.0f * p.of * p.rest};
     });
     case SO_ACT_SILU: return f([](float v) {
-        const Share p = shares(v);
+        const Share p = shares<HALF>(v);
         return Both{v * p.of, p.of * fmaf(v, p.rest, 1.0f)};
     });
     case SO_ACT_GELU: return f([](float v) {
-        const float below = normal<HALF>(v), bell = kNormal * __builtin_amdgcn_exp2f(-0.5f * kLog2e * v * v);
-        return Both{v * below, bell == 0.0f ? below : fmaf(v, bell, below)};
+        const float below = normal<HALF>(v), beside = bell<HALF>(v);
+        return Both{v * below, beside == 0.0f ? below : fmaf(v, beside, below)};
     });
     case SO_ACT_GELU_TANH: return f([](float v) {
-        const Share p = shares(2.0f * tanh_argument(v));
+        const Share p = shares<HALF>(2.0f * tanh_argument(v));
         const float both = p.of * p.rest;
         return Both{v * p.of, both == 0.0f ? p.of : fmaf(2.0f * v * both, kRootTwoOverPi * fmaf(3.0f * kCubic * v, v, 1.0f), p.of)};
     });
