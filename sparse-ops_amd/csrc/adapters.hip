@@ -219,13 +219,13 @@ struct Tile64 {
 #pragma unroll
             for (int e = 0; e < V; ++e) v[e] = mine ? v[e] : 0.0f;
         };
-        // What entries are multiplied with on their way in, and results on theirs out: the adapter's scale; in fp16 a power of two that brings a column's largest entry to 2^14 .. 2^15, and the rest
+        // What entries are multiplied with on their way in, and results on theirs out: the adapter's scale; in fp16 a power of two that brings a column's largest finite entry to 2^14 .. 2^15, and the rest
         // behind the product.
         float in = scale, out = 1.0f;
         const auto choose = [&](float largest) {
             const auto h = __builtin_amdgcn_permlane16_swap(__float_as_uint(largest), __float_as_uint(largest), false, false);
             const uint32_t top = max(h[0], h[1]) >> 23;                  // the largest's exponent, biased
-            const int up = top >= 255u ? 0 : min(max(141 - (int)top, -100), 100);
+            const int up = min(max(141 - (int)top, -100), 100);
             in = __uint_as_float((uint32_t)(127 + up) << 23);
             out = scale * __uint_as_float((uint32_t)(127 - up) << 23);
         };
@@ -249,17 +249,18 @@ struct Tile64 {
         if constexpr (SHIFTED) {
             // the first HOLD runs stay in registers between the two passes
             float held[HOLD][V], v[V], largest = 0.0f;
+            const auto see = [&](float entry) { largest = fmaxf(largest, fabsf(entry) < INFINITY ? fabsf(entry) : 0.0f); };
 #pragma unroll
             for (uint32_t run = 0; run < HOLD; ++run)
                 if (run < runs) {
                     low(run, held[run]);
 #pragma unroll
-                    for (int e = 0; e < V; ++e) largest = fmaxf(largest, fabsf(held[run][e]));
+                    for (int e = 0; e < V; ++e) see(held[run][e]);
                 }
             for (uint32_t run = HOLD; run < runs; ++run) {
                 low(run, v);
 #pragma unroll
-                for (int e = 0; e < V; ++e) largest = fmaxf(largest, fabsf(v[e]));
+                for (int e = 0; e < V; ++e) see(v[e]);
             }
             choose(largest);
             if (g == 0) factor[col] = out;
