@@ -75,7 +75,7 @@ struct Side {
             from[a] = row * (uint32_t)(ld * E) + (q % PER ^ swap(row)) * 16u;
         }
     }
-    __device__ __forceinline__ uint32_t steps() const { return (depth + BK - 1u) / BK; }
+    __host__ __device__ __forceinline__ uint32_t steps() const { return depth / BK + (depth % BK ? 1u : 0u); }
     // Whether a step is all there, so that its groups can be read whole.  Across, the group at a row's end holds what lies behind it, entries of no use that nothing depends on: the rows below have to be as many as it
     // reaches into, one where a row's stride is a group at least, seven of a single 16-bit column without gaps.
     __host__ __device__ __forceinline__ bool whole(uint32_t step) const

@@ -9,6 +9,23 @@ using so_dense::Side;
 
 static long checked = 0;
 
+// The steps of a contraction as long as 32 bits count.
+template <class S>
+static void count(const char *what)
+{
+    for (uint64_t depth = (1ull << 32) - 2 * S::BK; depth < 1ull << 32; ++depth) {
+        S side;
+        side.own = 1;
+        side.ld = (size_t)depth;
+        side.depth = (uint32_t)depth;
+        const uint64_t steps = (depth + S::BK - 1) / S::BK;
+        if (side.steps() != steps || side.whole((uint32_t)steps - 1) != (depth % S::BK == 0)) {
+            std::printf("%s: %u steps of a contraction of %llu\n", what, side.steps(), (unsigned long long)depth);
+            std::exit(1);
+        }
+    }
+}
+
 // An operand of `own` entries of its own index and `depth` of the contraction, its rows `ld` apart.
 template <class S, bool ACROSS>
 static void check(uint32_t own, size_t ld, uint32_t depth, const char *what)
@@ -17,7 +34,7 @@ static void check(uint32_t own, size_t ld, uint32_t depth, const char *what)
     side.own = own;
     side.ld = ld;
     side.depth = depth;
-    const uint32_t steps = (uint32_t)(((uint64_t)depth + S::BK - 1) / S::BK);
+    const uint32_t steps = side.steps();
     const size_t end = ACROSS ? (depth - 1) * ld + own : (own - 1) * ld + depth;
     for (uint32_t step = 0; step < steps; ++step) {
         if (!side.whole(step)) {
@@ -43,6 +60,7 @@ static void sweep(const char *what)
 {
     typedef Side<T, ACROSS, LEN, KB, WAVES> S;
     const uint32_t step = S::BK;
+    if (!ACROSS) count<S>(what);
     for (uint32_t own = 1; own <= (uint32_t)LEN + 9; own += own < 20 ? 1 : 7)
         for (uint32_t gap = 0; gap < 10; ++gap)
             for (uint32_t turns = 0; turns <= 2; ++turns)
