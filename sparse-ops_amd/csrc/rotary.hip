@@ -279,9 +279,9 @@ void rotary_gains_kernel(uint32_t D, uint32_t shares_q, uint32_t shares, uint32_
 
 // Lanes of a row and threads, and the pairs of a thread: 32 lanes down a head of up to 64 features, 64 of one of up to 256, 128 of a larger one, 64 where a row is one group.
 struct Cut { uint32_t lanes, threads, pairs; };
-Cut cut_of(int type, uint32_t D, uint32_t rot, uint32_t B)
+Cut cut_of(int type, uint32_t D, uint32_t B)
 {
-    const uint32_t V = 16u / (uint32_t)so_type_bytes(type), pairs = rot / 2u + (D - rot + 1u) / 2u;
+    const uint32_t V = 16u / (uint32_t)so_type_bytes(type), pairs = (D + 1u) / 2u;
     Cut c;
     c.lanes = B <= V ? 1 : pairs > 128 ? 4 : B <= 2 * V ? 2 : B <= 4 * V ? 4 : 8;
     c.threads = c.lanes == 1 ? 64 : pairs > 128 ? 512 : (pairs > 32 ? 64 : 32) * c.lanes;
@@ -362,10 +362,7 @@ extern "C" so_status so_head_rotary_reserve(so_ctx *ctx, int type, uint32_t head
     if (heads_q + heads_k == 0 || B == 0) return SO_OK;
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
-    // the number of pairs depends on rot where D is odd, and with it the cut
-    size_t bytes = 0;
-    for (const uint32_t rot : {0u, D & ~1u}) bytes = std::max(bytes, share_bytes(shape_of(ctx, cut_of(type, D, rot, B), type, heads_q, heads_k, D, B, rot, 0)));
-    return workspace(ctx, "so_head_rotary_reserve", bytes);
+    return workspace(ctx, "so_head_rotary_reserve", share_bytes(shape_of(ctx, cut_of(type, D, B), type, heads_q, heads_k, D, B, 0, SO_ROTARY_HALVES)));
 }
 
 extern "C" so_status so_head_rotary(so_ctx *ctx, int type, uint32_t heads_q, uint32_t heads_k, uint32_t D, uint32_t B, const void *dX, size_t x_stride, int norm, const float *dGainQ,
@@ -383,7 +380,7 @@ extern "C" so_status so_head_rotary(so_ctx *ctx, int type, uint32_t heads_q, uin
     SO_REQUIRE(!norm || !dRstd || (dRstd != dX && dRstd != dY), "so_head_rotary: a result is an input, or one array for both results");
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
-    const Cut c = cut_of(type, D, rot, B);
+    const Cut c = cut_of(type, D, B);
     Shape s = shape_of(ctx, c, type, heads_q, heads_k, D, B, rot, layout);
     place(s, type, {dX, dY}, {x_stride, y_stride});
     SO_REQUIRE(launch_fits(s, c), "so_head_rotary: %u x %u is too large for one launch", s.heads * D, B);
@@ -423,7 +420,7 @@ extern "C" so_status so_head_rotary_grad(so_ctx *ctx, int type, uint32_t heads_q
     }
     const so_on_device on(ctx->device);
     SO_HIP(on.status);
-    const Cut c = cut_of(type, D, rot, std::max(B, 1u));
+    const Cut c = cut_of(type, D, std::max(B, 1u));
     Shape s = shape_of(ctx, c, type, heads_q, heads_k, D, B, rot, layout);
     place(s, type, {norm ? dX : nullptr, dDy, dDx}, {norm ? x_stride : 0, dy_stride, dDx ? dx_stride : 0});
     SO_REQUIRE(launch_fits(s, c), "so_head_rotary_grad: %u x %u is too large for one launch", s.heads * D, B);

@@ -125,3 +125,33 @@ def test_gains_of_their_neighbours(ctx, D, rot, B, layout, type_):
     assert np.array_equal(dx0, dx1)
     for x in (dPos, dFreq, dGq, dGk, dR):
         x.free()
+
+
+@pytest.mark.parametrize("D,B", [(33, 40), (129, 9), (257, 300)])
+def test_one_reserve_for_every_number_of_turned_features(D, B):
+    """Of heads with an odd number of features: the gradient recorded behind one reserve, whatever is turned."""
+    rng = np.random.default_rng(D)
+    for rot in (0, 2, D - 1):
+        ctx = hipabi.Context()
+        try:
+            X, pos, freq, gq, gk = inputs(rng, Q, K, D, rot, B, "bf16")
+            a = Arrays(ctx, "bf16")
+            dX, out = a.put(X)[0], a.put(np.zeros(X.shape))[0]
+            dPos, dFreq, dR, oq, ok = ctx.array(pos, np.int32), ctx.array(freq if rot else np.zeros(1)), ctx.array(np.ones((Q + K, B))), ctx.empty((D,)), ctx.empty((D,))
+            call = lambda: ctx.head_rotary_grad(dX, dX, Q, K, D, B, dPos, dFreq, rot, out, "pairs", 1.0, True, None, None, dR, oq, ok, type="bf16")
+            ctx.head_rotary_reserve(Q, K, D, B, type="bf16")
+            ctx.graph_begin()
+            try:
+                call()
+            finally:
+                graph = ctx.graph_end()
+            seen = []
+            for again in (lambda: ctx.graph_launch(graph), call, lambda: ctx.graph_launch(graph)):
+                again()
+                seen.append([o.download().copy() for o in (out, oq, ok)])
+            for other in seen[1:]:
+                assert all(np.array_equal(x, y) for x, y in zip(seen[0], other))
+            assert seen[0][1].any() and seen[0][0].any()
+            ctx.graph_free(graph)
+        finally:
+            ctx.close()
