@@ -132,14 +132,16 @@ template <class T>
 struct Tile64 {
     static constexpr int V = so_elements<T>::V, RUNS = 16 / V;           // groups of 16 bytes that a lane has of a row
     static constexpr bool HALF = sizeof(T) == 2, SHIFTED = std::is_same<T, _Float16>::value;
+    static constexpr bool THIRD = std::is_same<T, __bf16>::value;         // bf16 holds an fp32 sum in three numbers
     typedef typename so_elements<T>::plain group;
     typedef typename so_elements<T>::vec group_anywhere;
-    // LDS: the operand [4][runs of 16][64 lanes], what a column's results are multiplied with, the adapters and their columns
-    static __host__ __device__ uint32_t lds(uint32_t runs) { return 4u * runs * 1024u + kCols * 4u + kCols * 12u; }
+    // LDS: the operand [4][runs of 16][64 lanes], its third numbers [4][pairs of runs][64 lanes], what a column's results are multiplied with, the adapters and their columns
+    static __host__ __device__ uint32_t operand_bytes(uint32_t runs) { return 4u * (runs + (THIRD ? (runs + 1u) / 2u : 0u)) * 1024u; }
+    static __host__ __device__ uint32_t lds(uint32_t runs) { return operand_bytes(runs) + kCols * 4u + kCols * 12u; }
 
     const Call<T> &f;
-    uint32_t runs, count;                                                // runs of 16 entries of rank; adapters
-    u32x4 *operand;
+    uint32_t runs, pairs, count;                                         // runs of 16 entries of rank, pairs of them; adapters
+    u32x4 *operand, *third;
     float *factor;
     uint64_t *columns;
     uint32_t *adapter;
@@ -150,8 +152,10 @@ struct Tile64 {
     __device__ __forceinline__ Tile64(const Call<T> &f_, char *lds) : f(f_)
     {
         runs = f.cut.padded / 16u;
+        pairs = (runs + 1u) / 2u;
         operand = reinterpret_cast<u32x4 *>(lds);
-        factor = reinterpret_cast<float *>(lds + 4u * runs * 1024u);
+        third = operand + 4u * runs * 64u;
+        factor = reinterpret_cast<float *>(lds + operand_bytes(runs));
         columns = reinterpret_cast<uint64_t *>(factor + kCols);
         adapter = reinterpret_cast<uint32_t *>(columns + kCols);
     }
@@ -230,21 +234,29 @@ struct Tile64 {
             out = scale * __uint_as_float((uint32_t)(127 - up) << 23);
         };
         const auto put = [&](uint32_t run, const float (&v)[V]) {
-            u32x4 r;
+            u32x4 &to = operand[(wave * runs + run) * 64u + lane];
             if constexpr (HALF) {
-                // 16 entries as 32: lanes 0 .. 31 have them rounded to T, the others what that leaves, so that the product, with B's entries twice, has them to 2^-16
-                group q;
+                // 16 entries as 32: lanes 0 .. 31 have them rounded to T, the others what that leaves, so that the product, with B's entries twice, has fp16's 22 bits and a
+                // sign, half a step of fp32.  What bf16's 16 leave goes into an instruction of its own, of two runs, the second one's in lanes 32 .. 63: without it results that cancel lost bits.
+                // It costs both launches of 4096 x 4096 x 8192, rank 16, 3 us of 53, rank 64 none of 100, rank 256, whose operand then leaves room for one workgroup a compute unit, 80 of 253; 48 requests none.
+                group q, rest;
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     const float w = v[e] * in;
                     const T high = (T)w;
-                    q[e] = g < 2u ? high : __builtin_isinf((float)high) ? (T)0.0f : (T)(w - (float)high);
+                    const float left = __builtin_isinf((float)high) ? 0.0f : w - (float)high;
+                    const T next = (T)left;
+                    q[e] = g < 2u ? high : next;
+                    rest[e] = (T)(left - (float)next);
                 }
-                r = __builtin_bit_cast(u32x4, q);
+                to = __builtin_bit_cast(u32x4, q);
+                if constexpr (THIRD) {
+                    const bool mine_too = run % 2u == g / 2u;
+                    if (mine_too || (run % 2u == 0 && run + 1u == runs)) third[(wave * pairs + run / 2u) * 64u + lane] = mine_too ? __builtin_bit_cast(u32x4, rest) : u32x4{};
+                }
             } else {
-                r = __builtin_bit_cast(u32x4, f32x4{v[0] * in, v[1] * in, v[2] * in, v[3] * in});
+                to = __builtin_bit_cast(u32x4, f32x4{v[0] * in, v[1] * in, v[2] * in, v[3] * in});
             }
-            operand[(wave * runs + run) * 64u + lane] = r;
         };
         if constexpr (SHIFTED) {
             // the first HOLD runs stay in registers between the two passes
@@ -320,21 +332,37 @@ struct Tile64 {
     }
     __device__ __forceinline__ float add(float product, uint32_t col, float to) const { return SHIFTED ? fmaf(product, factor[col], to) : product + to; }
     // The operand of a single run can stay in registers.
-    __device__ __forceinline__ void take(u32x4 (&t)[4]) const
+    struct Kept { u32x4 first[4], third[THIRD ? 4 : 1]; };
+    __device__ __forceinline__ void take(Kept &t) const
     {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) t[k] = operand[k * runs * 64u + threadIdx.x % 64u];
+        for (int k = 0; k < 4; ++k) {
+            t.first[k] = operand[k * runs * 64u + threadIdx.x % 64u];
+            if constexpr (THIRD) t.third[k] = third[k * pairs * 64u + threadIdx.x % 64u];
+        }
     }
-    // acc += runs from `run` on of 16 rows of B
+    // acc += runs from `run` on, an even number if there are several, of 16 rows of B
     template <int RC, bool EVEN>
-    __device__ __forceinline__ void multiply(const Run<EVEN> (&b)[RC], uint32_t run, const u32x4 (&t)[4], f32x4 (&acc)[4]) const
+    __device__ __forceinline__ void multiply(const Run<EVEN> (&b)[RC], uint32_t run, const Kept &t, f32x4 (&acc)[4]) const
     {
+        u32x4 before = {};
 #pragma unroll
         for (int c = 0; c < RC; ++c)
             if (RC == 1 || run + c < runs) {
                 const u32x4 w = settle(b[c], run + c);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) acc[k] = so_dense::multiply<T>(w, RC == 1 ? t[k] : operand[(k * runs + run + c) * 64u + threadIdx.x % 64u], acc[k]);
+                for (int k = 0; k < 4; ++k) acc[k] = so_dense::multiply<T>(w, RC == 1 ? t.first[k] : operand[(k * runs + run + c) * 64u + threadIdx.x % 64u], acc[k]);
+                if constexpr (THIRD) {
+                    // a pair's second run's entries of B for lanes 32 .. 63; where there is none they meet zeros
+                    const bool last = RC == 1 || run + c + 1u == runs;
+                    if (c % 2 || last) {
+                        u32x4 both = w;
+                        if (c % 2 && threadIdx.x % 64u < 32u) both = before;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) acc[k] = so_dense::multiply<T>(both, RC == 1 ? t.third[k] : third[(k * pairs + (run + c) / 2u) * 64u + threadIdx.x % 64u], acc[k]);
+                    }
+                    before = w;
+                }
             }
     }
 };
@@ -363,7 +391,7 @@ void adapters_out_kernel(Call<T> f)
     at.list(j0, f.base == f.Y ? (uint64_t)tile * kCols : j0);
     at.template gather<RC>(j0, sums);
     __syncthreads();
-    u32x4 whole[4];
+    typename Shared::Kept whole;
     if constexpr (RC == 1) at.take(whole);
     const uint32_t blocks = (at.runs + RC - 1u) / RC;
     typedef typename Shared::template Run<EVEN> Run;
@@ -459,7 +487,7 @@ void adapters_out_few_kernel(Call<T> f)
     if (at.count) load_first(row_begin + l);
     at.template gather<RC>(j0, sums);
     __syncthreads();
-    u32x4 whole[4];
+    typename Shared::Kept whole;
     if constexpr (RC == 1) at.take(whole);
     for (uint64_t from = row_begin; from < row_end; from += 16u) {
         const uint64_t row = from + l;
