@@ -1,4 +1,4 @@
-"""The gated block's activations and slopes in fp32, where they are small: every value within a few steps of its own, not of the largest one.
+"""The gated block's activations and slopes where they are small, in fp32 above all: every value within a few steps of its own, not of the largest one.
 
 u = 2^-24.  W, X and the other projection are ones, so that a sum is the number that its G0 is, exactly.  exp is off by at most a step, 2 u of its value; a sum, a product, a quotient and the fused
 multiply-add by u each; an argument of the exponential that is itself rounded costs its size times u.  What is left of 2^-126 and below is held to half a step of the subnormal numbers, times what multiplies it."""
@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from gated_reference import gate
-from elements import U
+from elements import HALF_STEP, SMALLEST, U, stored, values
 from test_gpu_gated import Arrays
 
 pytestmark = pytest.mark.gpu
@@ -72,4 +72,26 @@ def test_the_normal_distributions_bell(ctx):
     off = np.abs(dG.download().reshape(G.shape).astype(np.float64) - (below + G * bell))
     # erfc's own error, by its argument's rounding v^2 u of it and 4 steps, is that of the library's function
     assert np.all(off <= U * (10 * np.abs(G) * bell + (12 + 2 * G * G) * below) + TINY * (1 + np.abs(G))), np.max(off / (U * (np.abs(G) * bell + below) + TINY))
+    a.free()
+
+
+@pytest.mark.parametrize("type_", ["f16", "bf16"])
+def test_gelu_of_16_bits(ctx, type_):
+    """Half a step of the type and 2^-14 of the value: the normal distribution is within 2^-19 of itself, and its exponential's argument, v^2 / 2 < 82, carries 6 u of itself, less than 2^-15."""
+    G = pad_to(values(stored(np.concatenate([np.linspace(-12.7, 6.0, 3000), -np.logspace(-3, 1.1, 500)]), type_), type_), 16)
+    m, B = G.shape
+    a = Arrays(ctx, type_)
+    ones = a.put(np.ones(G.shape))[0]
+    w, x, zero = a.put(np.ones((m, 1)))[0], a.put(np.ones((1, B)))[0], a.put(np.zeros((m, 1)))[0]
+    H, dG, dU = (a.put(np.zeros(G.shape))[0] for _ in range(3))
+    at = a.put(G)[0]
+    ctx.gated(zero, zero, m, 1, x, B, "gelu", H, dG0=at, dU0=ones, type=type_)
+    ctx.gated_grad(w, w, m, 1, x, B, "gelu", at, ones, ones, None, None, None, dG, dU, type=type_)
+    want, slope = gate(G, "gelu")
+    bell = np.abs(G) * np.exp(-0.5 * G * G) / np.sqrt(2 * np.pi)
+    terms = np.where(G == 0, 0.5, np.abs(want / np.where(G == 0, 1, G))) + bell
+    for got, value, off in ((H, want, np.abs(want)), (dU, want, np.abs(want)), (dG, slope, terms)):
+        off = 2.0 ** -14 * off
+        got = values(got.download(), type_).reshape(G.shape)
+        assert np.all(np.abs(got - value) <= off + HALF_STEP[type_] * (np.abs(value) + off) + SMALLEST[type_]), np.max(np.abs(got - value) / (np.abs(value) + SMALLEST[type_]))
     a.free()
