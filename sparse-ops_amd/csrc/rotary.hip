@@ -151,16 +151,11 @@ void rotary_kernel(Shape s, const T *X, size_t ldx, const float *gain_q, const f
             float a[V], b[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                a[e] = NORM ? (float)x[k][0][e] * r[e] * g[k].x : (float)x[k][0][e];
-                b[e] = NORM ? (float)x[k][1][e] * r[e] * g[k].y : (float)x[k][1][e];
+                const float u = NORM ? (float)x[k][0][e] * r[e] * g[k].x : (float)x[k][0][e], v = NORM ? (float)x[k][1][e] * r[e] * g[k].y : (float)x[k][1][e];
+                const float c = turn[k][e].x, d = direction * turn[k][e].y;
+                a[e] = at.turned[k] ? fmaf(u, c, -(v * d)) : u;      // not a turn by nothing, which would make NaN of what lies beside an infinity
+                b[e] = at.turned[k] ? fmaf(v, c, u * d) : v;
             }
-            if (at.turned[k])                                            // not a turn by nothing, which would make NaN of what lies beside an infinity
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float u = a[e], v = b[e], c = turn[k][e].x, d = direction * turn[k][e].y;
-                    a[e] = fmaf(u, c, -(v * d));
-                    b[e] = fmaf(v, c, u * d);
-                }
             if (at.has[k]) so_group_store(Y + (size_t)(head * s.D + at.row[k].x) * ldy + at.c0, at.left, a);
             if (at.two[k]) so_group_store(Y + (size_t)(head * s.D + at.row[k].y) * ldy + at.c0, at.left, b);
         }
