@@ -408,8 +408,9 @@ so_status so_mxfp4_matvec(so_ctx *ctx, const so_mxfp4 *W, const float *dx, const
 
 /* ---- gated feed-forward block ---------------------------------------------------
  * No counterpart in the reference.  Activations are [features x B], batch contiguous, their rows a stride apart, weights
- * [m x n] row-major; all are of one element type.  Sums are taken in fp32, in the same order on every call, and a result of
- * 16 bits is rounded once. */
+ * [m x n] row-major; all are of one element type.  Sums are taken in fp32, and a result of 16 bits is rounded once.  Their order goes by
+ * the sizes, the type, whether the operands' rows begin at multiples of 16 bytes and the device's number of compute units, not by values: calls
+ * that are alike in these give the same bits, the same values at other addresses or strides may not. */
 
 /* H [m x B] = act(Wg X + G0) * (Wu X + U0), both projections of X [n x B], the activation (any SO_ACT_*) and the product.
  * dG0, dU0 [m x B], either may be NULL for zeros: what is added to the projections, as low-rank adapters make it of X (so_adapters).
@@ -419,8 +420,8 @@ so_status so_mxfp4_matvec(so_ctx *ctx, const so_mxfp4 *W, const float *dx, const
 so_status so_gated(so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t B, const void *dWg, const void *dWu, size_t w_stride,
                    const void *dX, size_t x_stride, int act, const void *dG0, const void *dU0, size_t g0_stride,
                    void *dH, size_t h_stride, void *dG, void *dU, size_t g_stride);
-/* Its gradient, from that of H and the saved sums G and U: dG = dH U act'(G) and dU = dH act(G), rounded to the element type
- * (relu's slope at 0 is 0); dX = Wg^T dG + Wu^T dU, dWg = dG X^T, dWu = dU X^T, written, not added to.  Any result may be NULL:
+/* Its gradient, from that of H and the saved sums G and U: dG = dH U act'(G) and dU = dH act(G), rounded to the element type, with
+ * which they go into the products (relu's slope at 0 is 0); dX = Wg^T dG + Wu^T dU, dWg = dG X^T, dWu = dU X^T, written, not added to.  Any result may be NULL:
  * dDg and dDu [m x B] are the gradients of G0 and U0 too; dWg, dWu may be NULL where dDx is, dX where both dDwg and dDwu are.
  * dDg and dDu may be dG, dU or dDh with the same stride; other overlaps are not allowed.  With B = 0 the weights' gradients are zeros. */
 so_status so_gated_grad(so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t B, const void *dWg, const void *dWu, size_t w_stride,
@@ -436,8 +437,9 @@ so_status so_gated_reserve(so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32
  * of the same X.  A [count][rank x n] and B [count][m x rank] lie row-major without gaps, in the element type of X, base and Y;
  * an adapter of a smaller rank is filled up with zeros.  A column whose which[c] is not in 0 .. count - 1 has none: Y = base there, and the
  * adapters' values do not touch it.  dBase NULL: zeros; dY may be dBase with the same stride, other overlaps are not allowed.
- * dScale [count] (fp32) NULL: ones.  rank is 1 .. 256; m, C and count may be 0, n may not.  Sums are taken in fp32, a
- * column's in the same order whatever the other columns are; a result of 16 bits is rounded once. */
+ * dScale [count] (fp32) NULL: ones.  rank is 1 .. 256; m, C and count may be 0, n may not.  Sums are taken in fp32, A x held with all of
+ * its bits between the products (fp16: half a step of fp32), a column's in the same order whatever the other columns are; a result of 16 bits is
+ * rounded once.  An infinity in a B of 16 bits may come out as NaN. */
 so_status so_adapters(so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t C, uint32_t count, uint32_t rank, const void *dA,
                       const void *dB, const float *dScale, const int32_t *dWhich, const void *dX, size_t x_stride,
                       const void *dBase, size_t base_stride, void *dY, size_t y_stride);
@@ -447,14 +449,15 @@ so_status so_adapters_reserve(so_ctx *ctx, int type, uint32_t m, uint32_t n, uin
 /* ---- rotary positions, with norms of queries and keys ----------------------------------
  * No counterpart in the reference.  X holds the heads_q heads of the queries and behind them the heads_k heads of the keys, D features each:
  * [(heads_q + heads_k) D x B], batch contiguous, of an element type; column b stands at position pos[b].  What a fused projection leaves behind
- * them (the values) is not touched.  Arithmetic is fp32, but for the angles, which are reduced in fp64: positions may be as far as int32 has them. */
+ * them (the values) is not touched.  Arithmetic is fp32, but for the angles, which are reduced in fp64: positions may be as far as int32 has
+ * them; an angle is off by |pos freq| 2^-54 turns and fp32's rounding of what is left of it. */
 enum { SO_ROTARY_HALVES = 0, SO_ROTARY_PAIRS = 1 };
 
 /* With `norm`, first every head: h = x rstd, rstd = 1 / sqrt(sum_d x^2 / D + eps), times gain_d, dGainQ's or dGainK's [D] (fp32, NULL: ones); the factors
  * [heads x B] (fp32) go to dRstd, unless it is NULL.  Without it eps, the gains and dRstd are not looked at.
  * Then the first `rot` features (even, 0 .. D) of every head are turned: features i and i + rot / 2 (SO_ROTARY_HALVES), or 2 i and 2 i + 1
  * (SO_ROTARY_PAIRS), as (a cos - b sin, b cos + a sin) times `amplitude`, by the angle pos[b] * freq[i].  freq [rot / 2] (fp32, radians) and amplitude carry
- * whatever scaling a long context asks for.  The other features are left as they are.  D is 1 .. 512.  dPos and dFreq may be NULL where rot is 0.
+ * whatever scaling a long context asks for.  The other features are left as they are, whatever lies beside them.  D is 1 .. 512.  dPos and dFreq may be NULL where rot is 0.
  * dY may be dX with the same stride, other overlaps are not allowed.  heads_q, heads_k or B may be 0. */
 so_status so_head_rotary(so_ctx *ctx, int type, uint32_t heads_q, uint32_t heads_k, uint32_t D, uint32_t B, const void *dX, size_t x_stride,
                          int norm, const float *dGainQ, const float *dGainK, float eps, const int32_t *dPos, const float *dFreq, uint32_t rot,

@@ -91,7 +91,7 @@ __device__ __forceinline__ void fetch_arguments(const Call<T> &f)
     asm volatile("" : : "s"(f.A), "s"(f.scale), "s"(f.ldx), "s"(f.m), "s"(f.cut.rows));
 }
 
-// A x of one part of the features for the columns of the adapters in turn.  Bound by memory for many columns: 4096 features of 8192 bf16, 67 MB, rank 16, 18.7 us or 3.6 TB/s (15.8 where no tile has two adapters, and is
+// A x of one part of the features for the columns of the adapters in turn.  Bound by memory for many columns: 4096 features of 8192 bf16, 67 MB, rank 16, 19.3 us or 3.5 TB/s (15.8 where no tile has two adapters, and is
 // read twice); by latency for few: 48 columns with 48 adapters fp16 5 us.
 template <class T, class TILE, bool DIRECT>
 __global__ __launch_bounds__(kThreads)
@@ -368,7 +368,7 @@ struct Tile64 {
 };
 
 // Y of many columns.  A workgroup takes 64 of them and a run of rows, a wave 16 rows at a time, one adapter after the other (few tiles have two); the next products' entries of B and the next 16 rows' base are on their
-// way while these are worked on.  Bound by memory: 4096 x 8192 bf16 with a base, 134 MB, 31.5 us or 4.3 TB/s.  Registers for as many waves as come without spilling.
+// way while these are worked on.  Bound by memory: 4096 x 8192 bf16 with a base, 134 MB, 34.6 us or 3.9 TB/s.  Registers for as many waves as come without spilling.
 template <class T, int RC, bool BASE, bool EVEN>
 __global__ __launch_bounds__(kThreads, (std::is_same<T, __bf16>::value && RC <= 2 ? 4 : RC <= 2 ? 3 : 2))
 void adapters_out_kernel(Call<T> f)
@@ -556,8 +556,9 @@ Cut cut_of(const so_ctx *ctx, int type, uint32_t m, uint32_t n, uint32_t C, uint
     c.depth = so_ceil_div(so_ceil_div(n, c.parts), step) * step;
     c.parts = so_ceil_div(n, c.depth);
     // With few columns the second launch deals adapters to waves, 16 rows at a time, else rows (us of the second launch, 4096 rows, rank 16 fp16, by rows / by adapters, of 1, 8 and 64 requests: 128 columns 5.3 / 6.6,
-    // 6.7 / 6.8, 19 / 11.5; 256 columns 5.8 / 10.5, 6.2 / 10.8, 13 / 14; 512 columns of one 6.5 / 16).  Of these a workgroup takes as many as leave four workgroups a compute unit, two of a larger rank, whose operand
-    // takes longer to gather.
+    // 6.7 / 6.8, 19 / 11.5; 256 columns 5.8 / 10.5, 6.2 / 10.8, 13 / 14; 512 columns of one 6.5 / 16).  Which requests there are is known on the device alone, so that the rule goes by the columns: below 256 it
+    // spares many requests 8 us at the price of 1 to 4 of few, from 256 on rows are faster for any.  Of rows a workgroup takes as many as leave four workgroups a compute unit, two of a larger rank, whose operand takes
+    // longer to gather.
     c.few = C < kFewColumns;
     const uint64_t rows = (uint64_t)m * c.tiles / ((c.few ? 8 : rank <= 16 ? 4 : 2) * cus);
     c.rows = c.few ? 16u * (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(rows / 16, 16)) : 64u * (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(rows / 64, 8));

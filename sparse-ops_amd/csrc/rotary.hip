@@ -21,8 +21,9 @@ __device__ __forceinline__ uint2 rows_of(const Shape &s, uint32_t p)
     return s.pairs ? make_uint2(2u * p, 2u * p + 1u) : make_uint2(p, p + half);
 }
 
-// cos and sin of pos * freq, times the amplitude.  The product is exact in fp64; of it the whole turns are taken off there, so that a position of 2^31 costs 2^-22 of a turn and one of 2^20 less
-// than fp32 can tell.  For results of 16 bits the vector unit's sine and cosine of what is left do: over half a turn to either side they are off by 2^-22.9 at most.
+// cos and sin of pos * freq, times the amplitude.  The turns pos * freq / (2 pi) are rounded three times in fp64, the constant among them, by 2^-53 of themselves at most each, and the whole ones are taken off there: an
+// angle is off by |pos freq| 2^-54 turns at most, less than fp32 can tell (2^-25 of a turn) up to |pos freq| = 2^29, and by 2^-23 of a turn at a position of 2^31 and a frequency of 1.  Frequencies above 1 are taken, and
+// cost in proportion.  For results of 16 bits the vector unit's sine and cosine of what is left do: over half a turn to either side they are off by 2^-22.9 at most.
 template <bool HALF>
 __device__ __forceinline__ float2 turn_of(int32_t pos, double turns, float amplitude)
 {
@@ -165,7 +166,7 @@ void rotary_kernel(Shape s, const T *X, size_t ldx, const float *gain_q, const f
 }
 
 // With norms: h = turn^-1(dY); dX = rstd (gain h - n mean(gain h n)), n = x rstd, and of every workgroup its share of the gains' gradients sum(h n), [tiles * groups][D], which the kernel below adds
-// up in a fixed order.  24 + 8 heads of 96 x 4099 fp16, 75 MB: 25.5 us and 4.5 for the shares; with the next head in registers ahead, which leaves one workgroup a compute unit, 47, and with h
+// up in a fixed order.  24 + 8 heads of 96 x 4099 fp16, 75 MB: 25.9 us and 4.7 for the shares; with the next head in registers ahead, which leaves one workgroup a compute unit, 47, and with h
 // kept instead of turned back again after the sum, 38.
 template <class T, int LC, int PPT, int NT>
 __global__ __launch_bounds__(NT, PPT == 1 ? 4 : 1)
